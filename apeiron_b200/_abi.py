@@ -46,12 +46,18 @@ EXPORTS = [
     "apx_gather_publish_async", "apx_matvec_gather_async", "apx_matvec_group_async",
     "apx_swiglu_quant_async", "apx_swiglu_quant_cols_async", "apx_swiglu_quant_shard_async", "apx_matmat_f32_group_async", "apx_act_describe_cols_async",
     "apx_ffn_status_decode", "apx_ctx_set_gemm_route", "apx_plan_create", "apx_plan_run_async", "apx_plan_destroy",
+    "apx_add_rms_norm_quant_async", "apx_kv4_page_bytes", "apx_rope_table_async",
+    "apx_rope_kv4_append_async", "apx_attn_kv4_async", "apx_sample_async",
 ]
 PLAN_GATE, PLAN_UP = 0, 1
 PLAN_MAX_PEERS = 7
 PLAN_ACT_UNPADDED = 1
 GEMM_AUTO, GEMM_DIGITS, GEMM_FOLD = 0, 1, 2
 CARRIER_F32, CARRIER_Q32 = 0, 1
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BANDS, ROPE_RAMP = 0, 1, 2, 3
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+SAMPLE_MAX_VOCAB = 524288
 
 MAX_PEERS = 8
 MAX_GATHER_PROJ = 4
@@ -123,6 +129,41 @@ class PlanFfn(C.Structure):
                 ("d_peer_desc", C.c_void_p * PLAN_MAX_PEERS)]
 
 
+def _struct(name, doc, *fields):
+    """A ctypes mirror of a C struct: fields grouped as (type, "names")."""
+    return type(name, (C.Structure,), {"__doc__": doc, "_fields_": [
+        (f, t) for t, names in fields for f in names.split()]})
+
+
+NormArgs = _struct(
+    "NormArgs", "Mirror of ``apx_norm_args``.",
+    (C.c_void_p, "d_x d_add d_weight d_resid d_y d_deq d_codes d_exps d_descs"),
+    (C.c_size_t, "n k ldx ld_add ld_resid ldy ld_deq"), (C.c_float, "eps"),
+    (C.c_int32, "deq_type"))
+Kv4Cache = _struct(
+    "Kv4Cache", "Mirror of ``apx_kv4_cache``.",
+    (C.c_void_p, "d_pages"), (C.c_size_t, "n_pages"),
+    (C.c_int32, "n_kv_heads head_dim page_tokens reserved"))
+SeqBatch = _struct(
+    "SeqBatch", "Mirror of ``apx_seq_batch``.",
+    (C.c_void_p, "d_cu d_kv_len d_table"), (C.c_size_t, "n_tokens"),
+    (C.c_int32, "n_seqs max_pages max_q reserved"))
+RopeFreqs = _struct(
+    "RopeFreqs", "Mirror of ``apx_rope_freqs``.",
+    (C.c_double, "base factor low high original mscale"), (C.c_int32, "rot_dim scaling"))
+RopeArgs = _struct(
+    "RopeArgs", "Mirror of ``apx_rope_args``.",
+    (C.c_void_p, "d_q d_k d_v d_table d_q_out d_k_deq d_v_deq d_status"),
+    (C.c_size_t, "n_pos ldq ldk ldv ldq_out"), (C.c_int32, "rot_dim layout n_heads q_type"))
+AttnArgs = _struct(
+    "AttnArgs", "Mirror of ``apx_attn_args``.",
+    (C.c_void_p, "d_q d_out d_status"), (C.c_size_t, "ldq ldo"), (C.c_int32, "type n_heads"),
+    (C.c_float, "scale"), (C.c_int32, "window sinks reserved"))
+SampleArgs = _struct(
+    "SampleArgs", "Mirror of ``apx_sample_args``.",
+    (C.c_void_p, "d_logits d_u d_temperature d_top_p d_min_p d_top_k d_token d_prob d_kept"),
+    (C.c_size_t, "rows vocab ld"))
+
 SZ = C.c_size_t
 U64 = C.c_uint64
 EP = C.POINTER(ApxErr)
@@ -173,6 +214,14 @@ _SIGS = {
     "apx_matvec_f32_noalloc": (C.c_int, [P, U64, SZ, SZ, P, P, P, P]),
     "apx_matmat_f32": (C.c_int, [P, U64, SZ, SZ, SZ, P, P, EP]),
     "apx_quant_f32_cols_async": (C.c_int, [P, P, SZ, SZ, P, P, P, P]),
+    "apx_add_rms_norm_quant_async": (C.c_int, [P, C.POINTER(NormArgs), P]),
+    "apx_kv4_page_bytes": (SZ, [C.c_int, C.c_int]),
+    "apx_rope_table_async": (C.c_int, [P, C.POINTER(RopeFreqs), SZ, P, P]),
+    "apx_rope_kv4_append_async": (C.c_int, [P, C.POINTER(RopeArgs), C.POINTER(Kv4Cache),
+                                            C.POINTER(SeqBatch), P]),
+    "apx_attn_kv4_async": (C.c_int, [P, C.POINTER(AttnArgs), C.POINTER(Kv4Cache),
+                                     C.POINTER(SeqBatch), P]),
+    "apx_sample_async": (C.c_int, [P, C.POINTER(SampleArgs), P]),
 }
 
 _lib = None

@@ -17,7 +17,8 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libapeiron_cuda.so")
 SOURCES = ["apx_runtime.cu", "apx_gemv.cu", "apx_quant.cu", "apx_gemm.cu", "apx_lgemm.cu", "apx_ffn.cu",
            "apx_noalloc.cu",
-           "apx_peer.cu", "apx_plan.cu"]
+           "apx_peer.cu", "apx_plan.cu",
+           "apx_step.cu", "apx_norm.cu", "apx_rope.cu", "apx_attn.cu", "apx_sample.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -42,7 +43,7 @@ def build(force: bool = False, verbose: bool = False, extra=None) -> str:
     if not force and not _objects_stale(srcs, LIB):
         return LIB
     cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "-Xcompiler", "-fvisibility=hidden", "-cudart=static",
+           "-Xcompiler", "-fvisibility=hidden", "-cudart=static", "--threads", "0",
            "-I", os.path.join(ROOT, "include"), "-o", LIB + ".tmp", *srcs]
     if extra:
         cmd[1:1] = list(extra)

@@ -495,6 +495,172 @@ APX_API int apx_matvec_gather_async(apx_ctx *ctx, uint64_t tensor, size_t n_out,
  * for them on the device).  Work that follows on `stream` sees every rank's rows. */
 APX_API int apx_gather_publish_async(apx_ctx *ctx, const apx_gather_desc *gd, void *stream);
 
+/* ---- between the projections: norm, positions and KV cache, attention, sampler ----------------
+ *
+ * The steps that carry a token from one projection to the next, on device buffers and a caller's
+ * stream, for an engine that keeps the whole step on the GPU (the reference runs them on the
+ * CPU around its projections: src/engine/step.rs, src/engine/attn.rs, src/engine/ops/).  They
+ * take the projections' f32 outputs and write the activations the projections read.  All sums
+ * and softmax statistics are held in 32 bits or more.  A call over no rows does nothing. */
+
+#define APX_DTYPE_F32 0
+#define APX_DTYPE_F16 1
+#define APX_DTYPE_BF16 2
+
+/* Residual add + RMS norm + quant_act, k rows of n:
+ *   h = x + add (one f32 rounding; h = x when d_add is NULL), r = 1 / sqrt(sum(h^2) / n + eps),
+ *   y = h * r * weight rounded once to f32 (ones when d_weight is NULL),
+ *   codes / exponent bytes / descriptor = those of apx_quant_f32_cols_async on y (the same
+ *   layout, rounding and refusals; codes past n are set to zero here).
+ * Optional outputs: d_resid = h (may be d_x itself), d_y = y, d_deq = the activation that the
+ * codes stand for (S * code / 2^32, exact in f32 and bf16), and the codes / exponents /
+ * descriptors (all three or none). */
+typedef struct apx_norm_args {
+  const float *d_x, *d_add, *d_weight;
+  float *d_resid, *d_y;
+  void *d_deq;
+  int8_t *d_codes;
+  uint8_t *d_exps;
+  apx_act_desc *d_descs;
+  size_t n, k;
+  size_t ldx, ld_add, ld_resid, ldy, ld_deq; /* elements between rows, each >= n */
+  float eps;
+  int32_t deq_type; /* APX_DTYPE_F32 or APX_DTYPE_BF16 */
+} apx_norm_args;
+APX_API int apx_add_rms_norm_quant_async(apx_ctx *ctx, const apx_norm_args *args, void *stream);
+
+/* A layer's KV cache in 4 bits, in pages.  Page p, KV head h: page_tokens / 16 tiles of 16
+ * tokens at d_pages + (p * n_kv_heads + h) * apx_kv4_page_bytes(head_dim, page_tokens).
+ * A value is d * (c - 8) with a 4-bit code c and one f16 scale d for 32 dims of one token.
+ * The append writes d with 8 significant bits, so that the product is exact in f16.
+ * A tile of head_dim D:
+ *   K codes (8 D bytes): token r's dims 2i (low nibble) and 2i + 1 at byte r * D / 2 + i;
+ *   V codes (8 D bytes): 32-bit words; with dim = 16 m + g (low nibble) and 16 m + g + 8 (high),
+ *     g < 8, and t < 4, word ((m / 4) * 32 + g * 4 + t) * 4 + m % 4 holds tokens
+ *     2t, 2t + 8, 2t + 1, 2t + 9 in its bytes 0..3 (the operand order of the matrix unit);
+ *   K scales, then V scales: f16 [D / 32][16 tokens] each.
+ * page_tokens: 16, 32, 64 or 128.  head_dim: 64 or 128.  Sequence s's token j lives in page
+ * d_table[s * max_pages + j / page_tokens], at j % page_tokens. */
+typedef struct apx_kv4_cache {
+  void *d_pages; /* 16-byte aligned */
+  size_t n_pages;
+  int32_t n_kv_heads, head_dim, page_tokens, reserved;
+} apx_kv4_cache;
+/* Bytes of one page of one KV head; 0 for sizes that are not served. */
+APX_API size_t apx_kv4_page_bytes(int head_dim, int page_tokens);
+
+/* The requests of one call.  Sequence s has the query tokens d_cu[s] .. d_cu[s + 1] - 1 of the
+ * call's n_tokens rows (d_cu[0] = 0, ascending, d_cu[n_seqs] = n_tokens) and d_kv_len[s] cached
+ * tokens, the query tokens being the last of them: query i stands at position
+ * d_kv_len[s] - (d_cu[s + 1] - d_cu[s]) + i.  max_q bounds a sequence's query tokens. */
+typedef struct apx_seq_batch {
+  const int32_t *d_cu;     /* n_seqs + 1 */
+  const int32_t *d_kv_len; /* n_seqs */
+  const int32_t *d_table;  /* n_seqs x max_pages page numbers */
+  size_t n_tokens;
+  int32_t n_seqs, max_pages, max_q, reserved;
+} apx_seq_batch;
+
+/* Cosines and sines for n_pos positions: d_table[pos][i] = (cos a, sin a) * mscale as f32 pairs,
+ * a = pos * f_i in f64, f_i = base^(-2i / rot_dim), i < rot_dim / 2, scaled for long contexts:
+ *   APX_ROPE_PLAIN   f_i
+ *   APX_ROPE_LINEAR  f_i / factor
+ *   APX_ROPE_BANDS   wavelength 2 pi / f_i below original / high: f_i; above original / low:
+ *                    f_i / factor; between: f_i * (s + (1 - s) / factor),
+ *                    s = (original * f_i / (2 pi) - low) / (high - low)
+ *   APX_ROPE_RAMP    f_i * (1 - s) + f_i / factor * s, s = clamp((i - i(high)) / (i(low) -
+ *                    i(high)), 0, 1) with i(b) = rot_dim * ln(original / (2 pi b)) /
+ *                    (2 ln base), rounded down for high and up for low and kept in the table
+ *                    (high and low being turns within the original length, as 32 and 1) */
+#define APX_ROPE_PLAIN 0
+#define APX_ROPE_LINEAR 1
+#define APX_ROPE_BANDS 2
+#define APX_ROPE_RAMP 3
+typedef struct apx_rope_freqs {
+  double base, factor, low, high, original, mscale;
+  int32_t rot_dim, scaling;
+} apx_rope_freqs;
+APX_API int apx_rope_table_async(apx_ctx *ctx, const apx_rope_freqs *freqs, size_t n_pos,
+                                 float *d_table, void *stream);
+
+/* Rotary positions on q and k, and the append of k and v to the cache.  The first rot_dim dims
+ * (a multiple of 8, at most head_dim) of each head turn: pairs (i, i + rot_dim / 2) under
+ * APX_ROPE_HALF, (2i, 2i + 1) under APX_ROPE_INTERLEAVED; (a, b) -> (a c - b s, b c + a s),
+ * each operation rounded once.  Per 32 dims of k and v: m the value of largest magnitude (the
+ * positive one of two), d = f16(bf16(-m / 8)), c = clamp(rint(x * (1 / d)) + 8, 0, 15), c = 8
+ * when d = 0.  Token t's head h starts at d_q[t * ldq + h * head_dim].  Optional: d_q (with
+ * d_q_out), and d_k_deq / d_v_deq = the values the cache now holds, f16
+ * [n_tokens][n_kv_heads][head_dim].  d_status (optional, all ones on entry): the first token
+ * refused, in row order, with APX_ERR_INVALID_ARGUMENT (its position outside the table or the
+ * cache, its page not one of n_pages) or APX_ERR_QUANT_REFUSED (a k or v value that is not
+ * finite or past 65280 in magnitude: its group is stored as zeros). */
+#define APX_ROPE_HALF 0
+#define APX_ROPE_INTERLEAVED 1
+typedef struct apx_rope_args {
+  const float *d_q, *d_k, *d_v;
+  const float *d_table; /* n_pos x rot_dim / 2 pairs, 16-byte aligned */
+  void *d_q_out;
+  uint16_t *d_k_deq, *d_v_deq;
+  apx_call_status *d_status;
+  size_t n_pos;
+  size_t ldq, ldk, ldv, ldq_out; /* elements between tokens */
+  int32_t rot_dim, layout;
+  int32_t n_heads, q_type; /* query heads; APX_DTYPE_* of d_q_out */
+} apx_rope_args;
+APX_API int apx_rope_kv4_append_async(apx_ctx *ctx, const apx_rope_args *args,
+                                      const apx_kv4_cache *cache, const apx_seq_batch *batch,
+                                      void *stream);
+
+/* Attention of the batch's query tokens over the cache: out = softmax(scale * q k^T) v per query
+ * head (n_heads a multiple of n_kv_heads; query head h reads KV head h / (n_heads /
+ * n_kv_heads)).  The query at position p sees key j <= p when window is 0 or j > p - window or
+ * j < sinks.  A query that sees no key gets zeros.  Keys past d_kv_len never take part, whatever
+ * the pages hold there.  q and out share one type.  For APX_DTYPE_F32 the products carry 22 bits
+ * of q and of the probabilities (one below 2^-38 of its row's largest counts as zero), the sums
+ * f32; for the 16-bit types the probabilities are rounded to 11 bits before the product with v.  Uses a context workspace: calls on one context must not overlap in time.
+ * d_status (optional, all ones on entry): APX_ERR_INVALID_ARGUMENT with the first sequence whose
+ * lengths or page numbers lie outside the batch or the cache (its rows are then undefined), or
+ * APX_ERR_DEVICE_TIMEOUT. */
+typedef struct apx_attn_args {
+  const void *d_q;
+  void *d_out;
+  apx_call_status *d_status;
+  size_t ldq, ldo; /* elements between tokens; head h at h * head_dim */
+  int32_t type, n_heads;
+  float scale;
+  int32_t window, sinks, reserved;
+} apx_attn_args;
+APX_API int apx_attn_kv4_async(apx_ctx *ctx, const apx_attn_args *args,
+                               const apx_kv4_cache *cache, const apx_seq_batch *batch,
+                               void *stream);
+
+/* One token per row of f32 logits, from a given uniform number u in [0, 1).  With the row's
+ * largest logit m and T its temperature, e_i = exp((l_i - m) * (1 / T)) in binary32 (the F32
+ * carrier's exp) and the integer weight w_i = rint(e_i * 2^31); every sum below is an exact
+ * integer sum, so no order of summation can change the answer.  Tokens ordered by e, the lower
+ * index first of equals:
+ *   top_k > 0: the first top_k stay;
+ *   top_p < 1: of those, a token stays while the weights before it sum to less than top_p times
+ *              the weights of all (in f64; the first always stays);
+ *   min_p > 0: of those, a token stays when w_i >= min_p * 2^31 (in f64).
+ * token = the first index, in vocabulary order, at which the running sum of the weights that
+ * stay passes floor(u * W), W their sum; prob = w / W; kept = the tokens that stay with w > 0.
+ * T <= 0 takes the largest logit (lowest index).  NaN logits count as -inf, -inf as excluded;
+ * where +inf occurs, only +inf tokens have weight.  A row with nothing left gives token -1,
+ * prob 0, kept 0.  Absent (NULL) parameter arrays: T = 1, no filter.  d_prob, d_kept: optional.
+ * vocab <= APX_SAMPLE_MAX_VOCAB. */
+#define APX_SAMPLE_MAX_VOCAB 524288u
+typedef struct apx_sample_args {
+  const float *d_logits, *d_u;
+  const float *d_temperature, *d_top_p, *d_min_p;
+  const int32_t *d_top_k;
+  int32_t *d_token;
+  float *d_prob;
+  int32_t *d_kept;
+  size_t rows, vocab, ld;
+} apx_sample_args;
+APX_API int apx_sample_async(apx_ctx *ctx, const apx_sample_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
