@@ -1,145 +1,872 @@
-// apx_attn.cu — attention over the paged 4-bit cache (layout: apx_kv4.cuh).
+// apx_attn.cu — attention over the paged 4-bit cache (layout: apx_kv4.cuh): the kernel for few
+// query rows and for f32.
 //
 // out_i = sum_j p_ij v_j, p = softmax over the visible keys of scale q_i.k_j, in one pass over
-// the keys with a running maximum m and sum l: a chunk of keys with scores s_j turns (m, l, o)
-// into m' = max(m, max s_j), l' = l e^(m-m') + sum e^(s_j-m'), o' = o e^(m-m') + sum e^(s_j-m') v_j.
+// the keys with a running maximum m and sum l: keys with scores s_j turn (m, l, o) into
+// m' = max(m, max s_j), l' = l e^(m-m') + sum e^(s_j-m'), o' = o e^(m-m') + sum e^(s_j-m') v_j.
+//
+// What bounds it: a decoded token reads every visible key once (D * 1.125 bytes a token and KV
+// head) and its group's query heads share the read, so the cache's bytes are the floor.  What a
+// byte costs in instructions decides how near it comes: a key's D dims unpack to f16 (three
+// instructions for two values) and go through the matrix unit as the 16-row operand, S^T = K Q^T
+// and O^T = V^T P, with 8 query rows per column tile.  mma.sync, not tcgen05: with 8 rows the
+// unpacked keys would cross shared memory and tensor memory for an 8th of a 64-row tile; from
+// registers they go straight in.
+//
+// Numbers.  d (c - 8) is exact in f16 (the append's d has 8 significant bits).  A query row is
+// scaled by a power of two to the top of f16's range and, for f32, split in two halves of 11 bits
+// each; so are the probabilities, taken at 2^14 e^(s - m): 22 bits down to 2^-38 of the largest.
+// The unit's f32 accumulation is cut into short chains joined by f32 additions.
+//
+// Split.  Work is counted in steps of 32 keys of one item (sequence, KV head, block of query
+// rows), in that order; every warp of the grid takes the same number of consecutive steps, so
+// ragged lengths and one long context balance alike.  Where an item spans warps of a CTA they
+// join in shared memory, where it spans CTAs through a workspace, joined by the last to arrive in
+// the items' order (not in the order of arrival: the same bits every time).  Blocks of a prompt's
+// rows pair first with last, so that the causal halves fill up to equal work.
+//
+// Copies: each warp has its own ring of slots in shared memory, two tiles (32 keys) each, filled
+// by bulk copies a ring ahead; nothing in the loop waits for another warp.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "apx_common.cuh"
 #include "apx_kv4.cuh"
+#include "apx_pack.cuh"
+#include "apx_kernels.h"
 #include "apx_step.h"
 
 namespace apx {
 
+namespace {
+
+constexpr int kStepKeys = 32;
+constexpr float kTopExp = 14.0f;  // probabilities are held at 2^14 e^(s - m)
+
 struct AttnArgs {
-  apx_attn_args a;
-  const int *cu, *kv_len, *table;
+  const void *q;
+  void *out;
   const uint8_t *pages;
-  size_t n_pages, page_bytes;
-  int n_seqs, max_pages, kv_heads, group, dim, page_tokens;
+  const int *cu, *kv_len, *table;
+  unsigned long long *status;
+  unsigned long long ldq, ldo;
+  unsigned long long page_bytes;
+  float *part;     // per CTA: two partial items
+  unsigned *count; // per item: CTAs that have arrived (zero between calls)
+  int n_pages, n_seqs, max_pages, kv_heads, group, page_shift;
+  int window, sinks, type, warps_min, n_tokens;
+  float scale;
 };
 
-__device__ __forceinline__ float load_q(const void *q, size_t i, int type) {
-  if (type == APX_DTYPE_F32) return static_cast<const float *>(q)[i];
-  if (type == APX_DTYPE_F16) return __half2float(static_cast<const __half *>(q)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16 *>(q)[i]);
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// One query row (token, head) per CTA of 128 threads, 128 keys at a time: thread j scores key
-// j, then thread i gathers output dim i.
-__global__ void __launch_bounds__(128) attn_row_kernel(AttnArgs p) {
-  __shared__ float s_q[128], s_p[128], s_red[4];
-  const int t = blockIdx.x, head = blockIdx.y, h = head / p.group, tid = threadIdx.x;
-  int lo = 0, hi = p.n_seqs;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (p.cu[mid] <= t) lo = mid;
-    else hi = mid;
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
+
+// Two codes of x (bits 0-3 and 16-19, or 4-7 and 20-23) as (c - 8) * s: the bits behind 0x6400
+// read 1024 + c, or 1024 + 16 c.
+__device__ __forceinline__ uint32_t low2(uint32_t x, __half2 s) {
+  const __half2 v = u2h((x & 0x000F000Fu) | 0x64006400u);
+  return h2u(__hmul2(__hsub2(v, u2h(0x64086408u)), s));
+}
+__device__ __forceinline__ uint32_t high2(uint32_t x, __half2 s) {
+  const __half2 v = u2h((x & 0x00F000F0u) | 0x64006400u);
+  return h2u(__hmul2(__hfma2(v, u2h(0x2C002C00u), u2h(0xD480D480u)), s));
+}
+
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = h2u(h);
+  lo = h2u(__floats2half2_rn(x - f.x, y - f.y));
+}
+
+__device__ __forceinline__ void store_out(void *o, unsigned long long i, float v, int type) {
+  if (type == APX_DTYPE_F32) static_cast<float *>(o)[i] = v;
+  else if (type == APX_DTYPE_F16) static_cast<__half *>(o)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16 *>(o)[i] = __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ void refuse(const AttnArgs &p, int seq) {
+  if (p.status)
+    atomicMin(p.status, (unsigned long long)seq << 24 |
+                            (unsigned long long)APX_ERR_INVALID_ARGUMENT << 16);
+}
+
+// A sequence's shape: its query rows (token, head of the group) in blocks of R, and the steps of
+// each.  Blocks pair first with last: a pair has `pair` steps, the first block's, then the
+// second's, then none.
+template <int R>
+struct SeqShape {
+  int first, rows, kv, p0, nblk;  // first query token, rows, usable keys, position of row 0
+  int pair;
+  bool bad;
+
+  __device__ void load(const AttnArgs &p, int s) {
+    const int a = p.cu[s], b = p.cu[s + 1], n = p.kv_len[s];
+    const long long room = (long long)p.max_pages << p.page_shift;
+    bad = a < 0 || b < a || b > p.n_tokens || n < 0 || n > room;
+    first = a;
+    rows = bad ? 0 : (b - a) * p.group;
+    kv = bad ? 0 : n;
+    p0 = n - (b - a);
+    nblk = (rows + R - 1) / R;
+    if (nblk == 0) pair = 0;
+    else if (nblk == 1) pair = steps(p, 0);
+    else if (!p.window) pair = steps(p, 0) + steps(p, nblk - 1) + 2;
+    else {
+      // a window's keys: what the block's positions span, in whole steps
+      const int most = p.window + (R - 1) / p.group + 1;
+      pair = 2 * (min(most / kStepKeys + 2 + (min(p.sinks, kv) + kStepKeys - 1) / kStepKeys,
+                      steps_to(kv)) + 1);
+    }
   }
-  const long long room = (long long)p.max_pages * p.page_tokens;
-  const int kv = (int)min((long long)p.kv_len[lo], room);
-  if (p.kv_len[lo] > room && tid == 0 && p.a.d_status)
-    atomicMin(&p.a.d_status->first,
-              (unsigned long long)lo << 24 | (unsigned long long)APX_ERR_INVALID_ARGUMENT << 16);
-  const int pos = p.kv_len[lo] - p.cu[lo + 1] + t;
-  const int end = min(pos + 1, kv);
-  if (tid < p.dim) s_q[tid] = load_q(p.a.d_q, (size_t)t * p.a.ldq + (size_t)head * p.dim + tid, p.a.type);
-  __syncthreads();
-  float m = -INFINITY, l = 0.0f, o = 0.0f;
-  const int tb = kv4_tile_bytes(p.dim);
-  auto tile_of = [&](int j) -> const uint8_t * {
-    const int page = p.table[(size_t)lo * p.max_pages + j / p.page_tokens];
-    if (page < 0 || (size_t)page >= p.n_pages) return nullptr;
-    return p.pages + ((size_t)page * p.kv_heads + h) * p.page_bytes +
-           (size_t)(j % p.page_tokens / kKvTile) * tb;
-  };
-  for (int j0 = 0; j0 < end; j0 += 128) {
-    if (p.a.window && j0 >= p.a.sinks && j0 + 127 <= pos - p.a.window) continue;
-    const int j = j0 + tid;
-    const bool seen = j < end && (!p.a.window || j < p.a.sinks || j > pos - p.a.window);
-    float s = -INFINITY;
-    if (seen) {
-      const uint8_t *tile = tile_of(j);
-      if (!tile) {
-        if (p.a.d_status)
-          atomicMin(&p.a.d_status->first, (unsigned long long)lo << 24 |
-                                              (unsigned long long)APX_ERR_INVALID_ARGUMENT << 16);
-      } else {
-        const int r = j % kKvTile;
-        const __half *ks = reinterpret_cast<const __half *>(tile + kv4_ks_off(p.dim));
-        s = 0.0f;
-        for (int g = 0; g < p.dim / kKvGroup; g++) {
-          float dot = 0.0f;
-          for (int i = 0; i < kKvGroup / 2; i++) {
-            const unsigned b = tile[r * (p.dim / 2) + g * (kKvGroup / 2) + i];
-            dot = fmaf((float)((int)(b & 15) - 8), s_q[g * kKvGroup + 2 * i], dot);
-            dot = fmaf((float)((int)(b >> 4) - 8), s_q[g * kKvGroup + 2 * i + 1], dot);
-          }
-          s = fmaf(dot, __half2float(ks[g * kKvTile + r]), s);
+  __device__ static int steps_to(int n) { return (max(n, 0) + kStepKeys - 1) / kStepKeys; }
+  // Keys [0, end) and steps [from, ..) that block b sees past the sinks' steps [0, sink).
+  __device__ void range(const AttnArgs &p, int b, int &end, int &sink, int &from) const {
+    const int lo = p0 + b * R / p.group, hi = p0 + min((b + 1) * R - 1, rows - 1) / p.group;
+    end = max(min(kv, hi + 1), 0);
+    sink = from = 0;
+    if (p.window) {
+      from = max(lo - p.window + 1, 0) / kStepKeys;
+      sink = min(steps_to(min(p.sinks, end)), from);
+    }
+  }
+  __device__ int steps(const AttnArgs &p, int b) const {
+    int end, sink, from;
+    range(p, b, end, sink, from);
+    return max(sink + max(steps_to(end) - from, 0), 1);  // one writes the zeros of unseeing rows
+  }
+  __device__ int pairs() const { return (nblk + 1) / 2; }
+};
+
+template <int D, int NT, int SPLIT>
+struct Cfg {
+  static constexpr int kWarps = NT == 1 ? 16 : 8;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kTile = kv4_tile_bytes(D);
+  static constexpr int kSlot = 2 * kTile;
+  static constexpr int kSlots = (D == 128 ? 2 : 4) * (NT == 1 ? 1 : 2);  // a power of two
+  static constexpr int kRing = kSlots * kSlot;
+  // a partial item: O (rows x D), then m and l of each row, all f32
+  static constexpr int kPart = kRows * D + 2 * kRows;
+  static constexpr int kWarpSmem = kRing + kPart * 4;
+  static constexpr int kSmem = kWarps * kWarpSmem;
+  static_assert(kPart * 4 <= kRing, "a partial item fits the ring");
+  static_assert(kSmem <= 227 * 1024 - 8192, "shared memory");
+};
+
+// One item that crosses a warp's boundary, kept for the join at the end of the CTA.
+struct Edge {
+  unsigned long long begin, end;  // the item's steps, numbered over the whole call
+  int first, rows, head, used;    // its sequence's first token and rows, its first row and head
+  int row0, pad;
+};
+
+template <int D, int NT, int SPLIT>
+__global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_kernel(AttnArgs p) {
+  using C = Cfg<D, NT, SPLIT>;
+  constexpr int W = C::kWarps, R = C::kRows, K4 = D / 32;  // words of K per thread and row
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ unsigned long long s_pre[C::kThreads];
+  __shared__ unsigned long long s_warp[W];
+  __shared__ __align__(8) uint64_t s_bar[W * C::kSlots];
+  __shared__ Edge s_edge[W][2];
+  __shared__ int s_last[2];
+
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, gid = lane / 4, tig = lane % 4;
+  pdl_launch_dependents();
+  uint8_t *ring = smem + warp * C::kWarpSmem;
+  uint64_t *bar = s_bar + warp * C::kSlots;
+  if (lane == 0)
+    for (int i = 0; i < C::kSlots; i++) mbar_init(bar + i, 1);
+  if (lane < 2) s_edge[warp][lane].used = 0;
+  pdl_wait();
+
+  // ---- the call's steps, summed over the sequences before each thread's share of them ----
+  const int per = (p.n_seqs + C::kThreads - 1) / C::kThreads;
+  {
+    unsigned long long mine = 0;
+    for (int i = 0; i < per; i++) {
+      const int s = tid * per + i;
+      if (s >= p.n_seqs) break;
+      SeqShape<R> q;
+      q.load(p, s);
+      if (q.bad && blockIdx.x == 0) refuse(p, s);
+      mine += (unsigned long long)q.pairs() * q.pair * p.kv_heads;
+    }
+    unsigned long long run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long u = __shfl_up_sync(0xFFFFFFFFu, run, o);
+      if (lane >= o) run += u;
+    }
+    if (lane == 31) s_warp[warp] = run;
+    __syncthreads();
+    unsigned long long base = 0;
+    for (int i = 0; i < warp; i++) base += s_warp[i];
+    s_pre[tid] = base + run;  // inclusive
+    __syncthreads();
+  }
+  const unsigned long long total = s_pre[C::kThreads - 1];
+  // at least warps_min steps for a warp that works at all
+  unsigned long long nwarps = (unsigned long long)gridDim.x * W;
+  if (total < nwarps * p.warps_min) nwarps = max((total + p.warps_min - 1) / p.warps_min, 1ull);
+  const unsigned long long gw = (unsigned long long)blockIdx.x * W + warp;
+  auto bound = [&](unsigned long long w) { return min(w, nwarps) * total / nwarps; };
+  const unsigned long long u0 = bound(gw), u1 = bound(gw + 1);
+
+  uint32_t phase = 0;  // bit i: the parity that slot i's next wait takes
+  int slot = 0;
+  bool alive = true;   // no wait has given up
+
+  // ---- this warp's steps, item by item ----
+  unsigned long long u = u0;
+  SeqShape<R> q;
+  int seq = -1;
+  unsigned long long seq0 = 0, seq1 = 0;  // the sequence's steps
+  while (u < u1 && alive) {
+    if (u >= seq1) {  // the sequence that holds u
+      int lo = 0, hi = C::kThreads - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (s_pre[mid] > u) hi = mid;
+        else lo = mid + 1;
+      }
+      unsigned long long at = lo ? s_pre[lo - 1] : 0;
+      for (int i = 0; i < per; i++) {
+        seq = lo * per + i;
+        q.load(p, seq);
+        const unsigned long long n = (unsigned long long)q.pairs() * q.pair * p.kv_heads;
+        if (u < at + n) {
+          seq0 = at;
+          seq1 = at + n;
+          break;
         }
-        s *= p.a.scale;
+        at += n;
       }
     }
-    float top = s;
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-    if (tid % 32 == 0) s_red[tid / 32] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-    __syncthreads();
-    if (top == -INFINITY) continue;
-    const float mn = fmaxf(m, top), keep = m == -INFINITY ? 0.0f : expf(m - mn);
-    const float e = s == -INFINITY ? 0.0f : expf(s - mn);
-    s_p[tid] = e;
-    float sum = e;
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
-    if (tid % 32 == 0) s_red[tid / 32] = sum;
-    __syncthreads();
-    l = l * keep + (s_red[0] + s_red[1] + s_red[2] + s_red[3]);
-    m = mn;
-    if (tid < p.dim) {
-      float acc = 0.0f;
-      for (int k = 0; k < 128 && j0 + k < end; k++) {
-        if (s_p[k] == 0.0f) continue;  // masked keys may hold anything
-        const uint8_t *tile = tile_of(j0 + k);
-        if (!tile) continue;
-        const int r = (j0 + k) % kKvTile;
-        const unsigned b = tile[kv4_v_off(p.dim) + kv4_v_byte(tid, r)];
-        const int c = (int)(tid % 16 < 8 ? b & 15 : b >> 4) - 8;
-        const __half *vs = reinterpret_cast<const __half *>(tile + kv4_vs_off(p.dim));
-        acc = fmaf(s_p[k], (float)c * __half2float(vs[tid / kKvGroup * kKvTile + r]), acc);
+    // the item: KV head, pair of blocks, block
+    const unsigned long long in_seq = u - seq0;
+    const int pr = (int)(in_seq / q.pair % q.pairs());
+    const int head = (int)(in_seq / q.pair / q.pairs());
+    const unsigned long long pair0 = u - in_seq % q.pair;
+    int blk = pr;
+    unsigned long long i0 = pair0, i1 = pair0 + q.steps(p, pr);
+    if (u >= i1) {
+      blk = q.nblk - 1 - pr;
+      i0 = i1;
+      i1 = blk == pr ? i0 : min(i0 + q.steps(p, blk), pair0 + q.pair);
+    }
+    if (u >= i1) {  // the pair's filling
+      u = min(pair0 + q.pair, u1);
+      continue;
+    }
+    const unsigned long long stop = min(i1, u1);
+    int end, sink, from;
+    q.range(p, blk, end, sink, from);
+    const int n_steps = (int)(stop - u), step0 = (int)(u - i0);
+
+    // the first key of step i of this warp's share
+    auto key_of = [&](int i) {
+      const int st = step0 + i;
+      return (st < sink ? st : st - sink + from) * kStepKeys;
+    };
+    const uint8_t *head_pages = p.pages + (unsigned long long)head * p.page_bytes;
+    const int *table = p.table + (size_t)seq * p.max_pages;
+    int page_at = 0;  // lane i: the page of tile i % 2 of step `page_base` + i / 2
+    int page_base = -16;
+    auto fetch = [&](int i) {  // step i into its slot
+      if (i - page_base >= 16) {
+        page_base = i;
+        const int st = i + lane / 2;
+        page_at = -1;
+        if (st < n_steps) {
+          const int key = key_of(st) + lane % 2 * kKvTile;
+          if (key < end) {
+            page_at = table[key >> p.page_shift];
+            if (page_at < 0 || page_at >= p.n_pages) {
+              refuse(p, seq);
+              page_at = -1;
+            }
+          }
+        }
       }
-      o = o * keep + acc;
+      const int pg = __shfl_sync(0xFFFFFFFFu, page_at, 2 * (i - page_base) + lane % 2);
+      int sl = slot + i;  // i is at most kSlots ahead of the step being read
+      sl %= C::kSlots;
+      const unsigned have = __ballot_sync(0xFFFFFFFFu, pg >= 0) & 3u;
+      if (lane == 0) mbar_expect_tx(bar + sl, (uint32_t)__popc(have) * C::kTile);
+      __syncwarp();
+      if (lane < 2 && pg >= 0) {
+        const int key = key_of(i) + lane * kKvTile;
+        const int tile = (key & ((1 << p.page_shift) - 1)) / kKvTile;
+        bulk_g2s(ring + sl * C::kSlot + lane * C::kTile,
+                 head_pages + (unsigned long long)pg * p.kv_heads * p.page_bytes +
+                     (unsigned)tile * C::kTile,
+                 C::kTile, bar + sl);
+      }
+      return have;
+    };
+    // which tiles of the slots in flight were copied at all (2 bits each, by step modulo slots)
+    unsigned present = 0;
+    auto start = [&](int i) {
+      const unsigned have = fetch(i);
+      const int sl = (slot + i) % C::kSlots;
+      present = (present & ~(3u << (2 * sl))) | have << (2 * sl);
+    };
+    for (int i = 0; i < min(n_steps, C::kSlots); i++) start(i);
+
+    // ---- the block's query rows as the second operand ----
+    uint32_t qh[NT][2 * K4][2], ql[SPLIT == 2 ? NT : 1][2 * K4][2];
+    float cq[NT][2];  // of columns 2 tig, 2 tig + 1: score units per product unit, times log2 e
+    int vis_lo[NT][2], vis_hi[NT][2];
+    int all_lo = 0, all_hi = 1 << 30;  // keys that every row of the block sees
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      const int r = blk * R + 8 * n + gid;
+      float v[2 * K4][4];
+      float top = 0.0f;
+      // matrix steps 2 w and 2 w + 1 take dims (0,4),(1,5) and (2,6),(3,7) of word w
+      auto put = [&v](int i, float x) { v[2 * (i / 8) + i % 4 / 2][2 * (i % 2) + i % 8 / 4] = x; };
+#pragma unroll
+      for (int i = 0; i < D / 4; i++) put(i, 0.0f);
+      if (r < q.rows) {
+        const unsigned long long at = (unsigned long long)(q.first + r / p.group) * p.ldq +
+                                      (unsigned long long)(head * p.group + r % p.group) * D +
+                                      tig * (D / 4);
+        if (SPLIT == 2) {
+          const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + at);
+#pragma unroll
+          for (int i = 0; i < D / 16; i++) {
+            const float4 x = src[i];
+            put(4 * i, x.x), put(4 * i + 1, x.y), put(4 * i + 2, x.z), put(4 * i + 3, x.w);
+          }
+        } else {
+          const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + at);
+#pragma unroll
+          for (int i = 0; i < D / 32; i++) {
+            const uint4 x = src[i];
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              float2 f;
+              if (p.type == APX_DTYPE_BF16)
+                f = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+              else
+                f = __half22float2(u2h(w[j]));
+              put(8 * i + 2 * j, f.x);
+              put(8 * i + 2 * j + 1, f.y);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < 2 * K4; w++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) top = fmaxf(top, fabsf(v[w][j]));
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+      // the largest |q| to [2^9, 2^10); exponents outside the f32 normals are clamped
+      const int e = min(max((int)(__float_as_uint(top) >> 23 & 255), 32), 254) - 127;
+      const float up = __int_as_float((9 - e + 127) << 23);
+#pragma unroll
+      for (int w = 0; w < 2 * K4; w++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          uint32_t lo;
+          split2(v[w][2 * j] * up, v[w][2 * j + 1] * up, qh[n][w][j], lo);
+          if (SPLIT == 2) ql[SPLIT == 2 ? n : 0][w][j] = lo;
+        }
+      const float c = p.scale * 1.44269504088896341f * __int_as_float((e - 9 + 127) << 23);
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        cq[n][j] = __shfl_sync(0xFFFFFFFFu, c, (2 * tig + j) * 4);
+        const int col = blk * R + 8 * n + 2 * tig + j;
+        const int pos = q.p0 + col / p.group;
+        const bool live = col < q.rows;
+        vis_hi[n][j] = live ? min(pos, end - 1) : -1;
+        vis_lo[n][j] = p.window ? pos - p.window + 1 : 0;
+        if (live) {
+          all_hi = min(all_hi, vis_hi[n][j]);
+          all_lo = max(all_lo, vis_lo[n][j]);
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      all_hi = min(all_hi, __shfl_xor_sync(0xFFFFFFFFu, all_hi, o));
+      all_lo = max(all_lo, __shfl_xor_sync(0xFFFFFFFFu, all_lo, o));
+    }
+
+    float o[NT][D / 16][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+      for (int i = 0; i < D / 16; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[n][i][j] = 0.0f;
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.0f;
+    }
+
+    for (int i = 0; i < n_steps; i++) {
+      const int sl = (slot + i) % C::kSlots;
+      alive = alive && mbar_wait(bar + sl, phase >> sl & 1);
+      phase ^= 1u << sl;
+      const uint8_t *tile = ring + sl * C::kSlot;
+      const unsigned here = present >> (2 * sl) & 3u;
+      const int key = key_of(i);
+
+      // scores of 32 keys, S^T = K Q^T: rows gid and gid + 8 of two tiles
+      float s[2][NT][4];
+      {
+        uint32_t kw[2][2][K4];
+        __half2 ks[2][2];
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int r = 0; r < 2; r++) {
+            const uint8_t *k = tile + t * C::kTile + (gid + 8 * r) * (D / 2) + tig * (D / 8);
+            if (D == 128) {
+              const uint4 x = *reinterpret_cast<const uint4 *>(k);
+              kw[t][r][0] = x.x, kw[t][r][1] = x.y;
+              kw[t][r][2 % K4] = x.z, kw[t][r][3 % K4] = x.w;
+            } else {
+              const uint2 x = *reinterpret_cast<const uint2 *>(k);
+              kw[t][r][0] = x.x, kw[t][r][1] = x.y;
+            }
+            const int g = tig * (D / 4) / kKvGroup;
+            ks[t][r] = __half2half2(*reinterpret_cast<const __half *>(
+                tile + t * C::kTile + kv4_ks_off(D) + (g * kKvTile + gid + 8 * r) * 2));
+          }
+        float lo[2][NT][4];
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[t][n][j] = lo[t][n][j] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < K4; w++)
+#pragma unroll
+          for (int t = 0; t < 2; t++) {
+            const uint32_t x = kw[t][0][w], y = kw[t][1][w];
+            const uint32_t a[4] = {low2(x, ks[t][0]), low2(y, ks[t][1]), high2(x, ks[t][0]),
+                                   high2(y, ks[t][1])};
+            const uint32_t b[4] = {low2(x >> 8, ks[t][0]), low2(y >> 8, ks[t][1]),
+                                   high2(x >> 8, ks[t][0]), high2(y >> 8, ks[t][1])};
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+              // two chains: for 16-bit queries the odd steps', for f32 the low halves'
+              mma_f16(s[t][n], a, qh[n][2 * w][0], qh[n][2 * w][1]);
+              mma_f16(SPLIT == 2 ? s[t][n] : lo[t][n], b, qh[n][2 * w + 1][0],
+                      qh[n][2 * w + 1][1]);
+              if (SPLIT == 2) {
+                mma_f16(lo[t][n], a, ql[SPLIT == 2 ? n : 0][2 * w][0],
+                        ql[SPLIT == 2 ? n : 0][2 * w][1]);
+                mma_f16(lo[t][n], b, ql[SPLIT == 2 ? n : 0][2 * w + 1][0],
+                        ql[SPLIT == 2 ? n : 0][2 * w + 1][1]);
+              }
+            }
+          }
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[t][n][j] = (s[t][n][j] + lo[t][n][j]) * cq[n][j & 1];
+      }
+      // masks, where some row does not see all 32 keys
+      if (key + kStepKeys - 1 > all_hi || (key < all_lo && key + kStepKeys > p.sinks) ||
+          here != 3u) {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const int k = key + kKvTile * t + gid + 8 * (j / 2);
+              const bool seen = (here >> t & 1) && k <= vis_hi[n][j & 1] &&
+                                (k >= vis_lo[n][j & 1] || k < p.sinks);
+              if (!seen) s[t][n][j] = -INFINITY;
+            }
+      }
+      // the running maximum; the sums and outputs turn only when it grows
+      bool grew = false;
+      float mn[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          float x = fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2]));
+#pragma unroll
+          for (int sh = 4; sh < 32; sh <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, sh));
+          mn[n][j] = fmaxf(m[n][j], x);
+          grew |= mn[n][j] > m[n][j];
+        }
+      if (__any_sync(0xFFFFFFFFu, grew)) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          float f[2];
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            f[j] = m[n][j] == -INFINITY ? 0.0f : ex2(m[n][j] - mn[n][j]);
+            l[n][j] *= f[j];
+            m[n][j] = mn[n][j];
+          }
+#pragma unroll
+          for (int d = 0; d < D / 16; d++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[n][d][j] *= f[j & 1];
+        }
+      }
+      // probabilities, turned into the second operand of O^T = V^T P
+      uint32_t ph[2][NT][2], pl[2][SPLIT == 2 ? NT : 1][2];
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        float base[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) base[j] = kTopExp - (m[n][j] == -INFINITY ? 0.0f : m[n][j]);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          float e[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            e[j] = ex2(s[t][n][j] + base[j & 1]);
+            l[n][j & 1] += e[j];
+          }
+#pragma unroll
+          for (int r = 0; r < 2; r++) {
+            uint32_t hi, lo;
+            if (SPLIT == 2) {
+              split2(e[2 * r], e[2 * r + 1], hi, lo);
+              pl[t][SPLIT == 2 ? n : 0][r] = transpose8(lo);
+            } else {
+              hi = h2u(__floats2half2_rn(e[2 * r], e[2 * r + 1]));
+            }
+            ph[t][n][r] = transpose8(hi);
+          }
+        }
+      }
+      // tokens past the last key may hold anything: their scales count as zero
+      const bool tail = key + kStepKeys > end || here != 3u;
+#pragma unroll
+      for (int mq = 0; mq < D / 64; mq++) {
+        uint32_t vw[2][4];
+        uint32_t vs[2][2][2];  // tile, group of 32 dims, token half
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          const uint4 x = *reinterpret_cast<const uint4 *>(tile + t * C::kTile + kv4_v_off(D) +
+                                                           (mq * 32 + lane) * 16);
+          vw[t][0] = x.x, vw[t][1] = x.y, vw[t][2] = x.z, vw[t][3] = x.w;
+#pragma unroll
+          for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              uint32_t w = *reinterpret_cast<const uint32_t *>(
+                  tile + t * C::kTile + kv4_vs_off(D) +
+                  ((2 * mq + g) * kKvTile + 8 * h + 2 * tig) * 2);
+              if (tail) {
+                const int k = key + kKvTile * t + 8 * h + 2 * tig;
+                if (!(here >> t & 1) || k >= end) w &= 0xFFFF0000u;
+                if (!(here >> t & 1) || k + 1 >= end) w &= 0x0000FFFFu;
+              }
+              vs[t][g][h] = w;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int d = 4 * mq + j;
+          uint32_t a[2][4];
+#pragma unroll
+          for (int t = 0; t < 2; t++) {
+            const uint32_t x = vw[t][j];
+            const __half2 s0 = u2h(vs[t][j / 2][0]), s1 = u2h(vs[t][j / 2][1]);
+            a[t][0] = low2(x, s0);
+            a[t][1] = high2(x, s0);
+            a[t][2] = low2(x >> 8, s1);
+            a[t][3] = high2(x >> 8, s1);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            if (SPLIT == 2) {
+              float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+              for (int t = 0; t < 2; t++) {
+                mma_f16(acc, a[t], pl[t][SPLIT == 2 ? n : 0][0], pl[t][SPLIT == 2 ? n : 0][1]);
+                mma_f16(acc, a[t], ph[t][n][0], ph[t][n][1]);
+              }
+#pragma unroll
+              for (int c = 0; c < 4; c++) o[n][d][c] += acc[c];
+            } else {
+#pragma unroll
+              for (int t = 0; t < 2; t++) mma_f16(o[n][d], a[t], ph[t][n][0], ph[t][n][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();  // every lane has read the slot
+      if (i + C::kSlots < n_steps) start(i + C::kSlots);
+    }
+    slot = (slot + n_steps) % C::kSlots;
+
+    // ---- the item's rows of this warp ----
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int sh = 4; sh < 32; sh <<= 1)
+          l[n][j] += __shfl_xor_sync(0xFFFFFFFFu, l[n][j], sh);
+    if (u == i0 && stop == i1) {  // the whole item
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const int r = blk * R + 8 * n + 2 * tig + j;
+          if (r >= q.rows) continue;
+          const float inv = l[n][j] == 0.0f ? 0.0f : 1.0f / l[n][j];
+          const unsigned long long at = (unsigned long long)(q.first + r / p.group) * p.ldo +
+                                        (unsigned long long)(head * p.group + r % p.group) * D;
+#pragma unroll
+          for (int d = 0; d < D / 16; d++) {
+            store_out(p.out, at + 16 * d + gid, o[n][d][j] * inv, p.type);
+            store_out(p.out, at + 16 * d + gid + 8, o[n][d][j + 2] * inv, p.type);
+          }
+        }
+    } else {
+      // kept for the join at the end: an item that began before this warp, behind the ring; one
+      // that goes on after it (its last), in the ring, whose copies have all arrived
+      const int e = u == i0 ? 1 : 0;
+      float *part = reinterpret_cast<float *>(e ? ring : ring + C::kRing);
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const int r = 8 * n + 2 * tig + j;
+#pragma unroll
+          for (int d = 0; d < D / 16; d++) {
+            part[r * D + 16 * d + gid] = o[n][d][j];
+            part[r * D + 16 * d + gid + 8] = o[n][d][j + 2];
+          }
+          if (gid == 0) {
+            part[R * D + r] = m[n][j];
+            part[R * D + R + r] = l[n][j];
+          }
+        }
+      if (lane == 0) s_edge[warp][e] = Edge{i0, i1, q.first, q.rows, head, 1, blk * R, 0};
+    }
+    u = stop;
+  }
+  if (!alive && lane == 0 && p.status)
+    atomicMin(p.status, (unsigned long long)APX_ERR_DEVICE_TIMEOUT << 16);
+
+  // ---- the join: items that cross warps, then items that cross CTAs ----
+  __syncthreads();
+  const unsigned long long c0 = bound((unsigned long long)blockIdx.x * W);
+  const unsigned long long c1 = bound((unsigned long long)(blockIdx.x + 1) * W);
+  auto part_of = [&](int w, int e) {
+    return reinterpret_cast<const float *>(smem + w * C::kWarpSmem + (e ? 0 : C::kRing));
+  };
+  auto write4 = [&](const Edge &ed, int r, int d, const float4 v, float sum) {
+    const int row = ed.row0 + r;
+    if (row >= ed.rows) return;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const unsigned long long at = (unsigned long long)(ed.first + row / p.group) * p.ldo +
+                                  (unsigned long long)(ed.head * p.group + row % p.group) * D + d;
+    if (SPLIT == 2) {
+      *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) =
+          make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    } else {
+      uint2 w;
+      if (p.type == APX_DTYPE_BF16) {
+        __nv_bfloat162 x = __floats2bfloat162_rn(v.x * inv, v.y * inv);
+        __nv_bfloat162 y = __floats2bfloat162_rn(v.z * inv, v.w * inv);
+        w = make_uint2(*reinterpret_cast<uint32_t *>(&x), *reinterpret_cast<uint32_t *>(&y));
+      } else {
+        w = make_uint2(h2u(__floats2half2_rn(v.x * inv, v.y * inv)),
+                       h2u(__floats2half2_rn(v.z * inv, v.w * inv)));
+      }
+      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) = w;
+    }
+  };
+  bool out_of_cta[2] = {false, false};
+  Edge edge[2];
+  for (int w = 0; w < W; w++)
+    for (int e = w == 0 ? 0 : 1; e < 2; e++) {  // the first part of each item in this CTA
+      if (!s_edge[w][e].used) continue;
+      const Edge ed = s_edge[w][e];
+      int last = w;
+      while (last + 1 < W && s_edge[last + 1][0].used && s_edge[last + 1][0].begin == ed.begin)
+        last++;
+      const bool whole = ed.begin >= c0 && ed.end <= c1;
+      const int at = ed.begin >= c0 ? 1 : 0;
+      float *dst = p.part + ((size_t)blockIdx.x * 2 + at) * C::kPart;
+      if (!whole) {
+        out_of_cta[at] = true;
+        edge[at] = ed;
+      }
+      for (int i = tid; i < R * D / 4; i += C::kThreads) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float top = -INFINITY;
+        for (int k = w; k <= last; k++) top = fmaxf(top, part_of(k, k == w ? e : 0)[R * D + r]);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float sum = 0.0f;
+        for (int k = w; k <= last; k++) {
+          const float *src = part_of(k, k == w ? e : 0);
+          const float mk = src[R * D + r], f = mk == -INFINITY ? 0.0f : ex2(mk - top);
+          const float4 x = *reinterpret_cast<const float4 *>(src + r * D + d);
+          sum = fmaf(f, src[R * D + R + r], sum);
+          v = make_float4(fmaf(f, x.x, v.x), fmaf(f, x.y, v.y), fmaf(f, x.z, v.z),
+                          fmaf(f, x.w, v.w));
+        }
+        if (whole) {
+          write4(ed, r, d, v, sum);
+        } else {
+          *reinterpret_cast<float4 *>(dst + r * D + d) = v;
+          if (d == 0) {
+            dst[R * D + r] = top;
+            dst[R * D + R + r] = sum;
+          }
+        }
+      }
+    }
+  // an item's CTAs: the first holds it in its second part, the others in their first
+  auto cta_of = [&](unsigned long long step) {
+    return (int)(((step + 1) * nwarps - 1) / total / W);
+  };
+  if (out_of_cta[0] || out_of_cta[1]) {  // the same in every thread
+    fence_acq_rel_gpu();
+    __syncthreads();
+    if (tid < 2) {
+      s_last[tid] = 0;
+      const bool mine = tid ? out_of_cta[1] : out_of_cta[0];
+      if (mine) {
+        const Edge &ed = tid ? edge[1] : edge[0];
+        const int a = cta_of(ed.begin), n = cta_of(ed.end - 1) - a + 1;
+        if (atomicAdd(p.count + a, 1u) == (unsigned)n - 1) {
+          s_last[tid] = n;
+          p.count[a] = 0;  // for the next call
+        }
+        fence_acq_rel_gpu();
+      }
     }
     __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int n = s_last[e];
+      if (!n) continue;
+      const Edge ed = edge[e];
+      const int a = cta_of(ed.begin);
+      for (int i = tid; i < R * D / 4; i += C::kThreads) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        auto src_of = [&](int k) {
+          return p.part + ((size_t)(a + k) * 2 + (k == 0 ? 1 : 0)) * C::kPart;
+        };
+        float top = -INFINITY;
+        for (int k = 0; k < n; k++) top = fmaxf(top, __ldcg(src_of(k) + R * D + r));
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float sum = 0.0f;
+        for (int k = 0; k < n; k++) {
+          const float *src = src_of(k);
+          const float mk = __ldcg(src + R * D + r), f = mk == -INFINITY ? 0.0f : ex2(mk - top);
+          const float4 x = __ldcg(reinterpret_cast<const float4 *>(src + r * D + d));
+          sum = fmaf(f, __ldcg(src + R * D + R + r), sum);
+          v = make_float4(fmaf(f, x.x, v.x), fmaf(f, x.y, v.y), fmaf(f, x.z, v.z),
+                          fmaf(f, x.w, v.w));
+        }
+        write4(ed, r, d, v, sum);
+      }
+    }
   }
-  if (tid < p.dim) {
-    const float y = l > 0.0f ? o / l : 0.0f;
-    const size_t at = (size_t)t * p.a.ldo + (size_t)head * p.dim + tid;
-    if (p.a.type == APX_DTYPE_F32) static_cast<float *>(p.a.d_out)[at] = y;
-    else if (p.a.type == APX_DTYPE_F16) static_cast<__half *>(p.a.d_out)[at] = __float2half_rn(y);
-    else static_cast<__nv_bfloat16 *>(p.a.d_out)[at] = __float2bfloat16_rn(y);
-  }
+}
+
+template <int D, int NT, int SPLIT>
+cudaError_t launch_split(const AttnArgs &p, int grid, cudaStream_t stream) {
+  using C = Cfg<D, NT, SPLIT>;
+  auto kern = attn_split_kernel<D, NT, SPLIT>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_allowed() ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+}  // namespace
+
+// Two partial items per CTA of the largest block, and the arrival counters before them.
+constexpr int kCountBytes = 4096;
+size_t attn_work_bytes(int sms) {
+  return kCountBytes + (size_t)sms * 2 * Cfg<128, 2, 1>::kPart * sizeof(float);
 }
 
 cudaError_t launch_attn_kv4(const apx_attn_args &a, const apx_kv4_cache &c,
-                            const apx_seq_batch &b, cudaStream_t stream) {
+                            const apx_seq_batch &b, void *work, int sms, cudaStream_t stream) {
   AttnArgs p;
-  p.a = a;
+  p.q = a.d_q;
+  p.out = a.d_out;
+  p.pages = static_cast<const uint8_t *>(c.d_pages);
   p.cu = b.d_cu;
   p.kv_len = b.d_kv_len;
   p.table = b.d_table;
-  p.pages = static_cast<const uint8_t *>(c.d_pages);
-  p.n_pages = c.n_pages;
+  p.status = a.d_status ? &a.d_status->first : nullptr;
+  p.ldq = a.ldq;
+  p.ldo = a.ldo;
   p.page_bytes = apx_kv4_page_bytes(c.head_dim, c.page_tokens);
+  p.count = static_cast<unsigned *>(work);
+  p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(work) + kCountBytes);
+  p.n_pages = (int)c.n_pages;
   p.n_seqs = b.n_seqs;
+  p.n_tokens = (int)b.n_tokens;
   p.max_pages = b.max_pages;
   p.kv_heads = c.n_kv_heads;
   p.group = a.n_heads / c.n_kv_heads;
-  p.dim = c.head_dim;
-  p.page_tokens = c.page_tokens;
-  attn_row_kernel<<<dim3((unsigned)b.n_tokens, (unsigned)a.n_heads), 128, 0, stream>>>(p);
-  return cudaGetLastError();
+  p.page_shift = 0;
+  while (1 << p.page_shift < c.page_tokens) p.page_shift++;
+  p.window = a.window;
+  p.sinks = a.window ? a.sinks : 0;
+  p.type = a.type;
+  p.warps_min = 1;
+  p.scale = a.scale;
+  const int grid = std::min(sms, kCountBytes / 4);
+  const bool one = (size_t)b.max_q * p.group <= 8, f32 = a.type == APX_DTYPE_F32;
+  if (c.head_dim == 128) {
+    if (one) return f32 ? launch_split<128, 1, 2>(p, grid, stream) : launch_split<128, 1, 1>(p, grid, stream);
+    return f32 ? launch_split<128, 2, 2>(p, grid, stream) : launch_split<128, 2, 1>(p, grid, stream);
+  }
+  if (one) return f32 ? launch_split<64, 1, 2>(p, grid, stream) : launch_split<64, 1, 1>(p, grid, stream);
+  return f32 ? launch_split<64, 2, 2>(p, grid, stream) : launch_split<64, 2, 1>(p, grid, stream);
 }
 
 }  // namespace apx

@@ -22,6 +22,7 @@
 
 #include "apx_common.cuh"
 #include "apx_kernels.h"
+#include "apx_step.h"
 
 using namespace apx;
 
@@ -138,6 +139,7 @@ struct apx_ctx {
   DevBuf lwork;    // digit-plane GEMM per-call workspace (no state kept between calls)
   DevBuf ascratch; // codes / exps / descriptors of apx_matmat_f32_async off the fused route
   DevBuf fwork;    // per-CTA statistics of apx_swiglu_quant_async
+  DevBuf attn_work; // partial items and arrival counters of apx_attn_kv4_async (zeroed at open)
   int gemm_route = APX_GEMM_AUTO;  // apx_ctx_set_gemm_route
   HostBuf host;    // pinned mirror of `dev`
 };
@@ -525,6 +527,11 @@ bool tensor_launch_info(apx_ctx *ctx, uint64_t handle, uint32_t *type, const uin
 }
 
 int context_device(const apx_ctx *ctx) { return ctx->device; }
+
+void *context_attn_work(apx_ctx *ctx, int *sms) {
+  *sms = ctx->sm_count;
+  return ctx->attn_work.p;
+}
 }  // namespace apx
 
 extern "C" {
@@ -552,6 +559,16 @@ apx_ctx *apx_open(int device, apx_err *err) {
     cuda_err(err, e);
     return nullptr;
   }
+  const size_t attn = attn_work_bytes(ctx->sm_count);
+  e = ctx->attn_work.ensure(attn);
+  if (e == cudaSuccess) e = cudaMemset(ctx->attn_work.p, 0, attn);
+  if (e != cudaSuccess) {
+    ctx->attn_work.release();
+    cudaStreamDestroy(ctx->stream);
+    delete ctx;
+    cuda_err(err, e);
+    return nullptr;
+  }
   return ctx;
 }
 
@@ -566,6 +583,7 @@ void apx_close(apx_ctx *ctx) {
   ctx->lwork.release();
   ctx->ascratch.release();
   ctx->fwork.release();
+  ctx->attn_work.release();
   ctx->host.release();
   cudaStreamDestroy(ctx->stream);
   delete ctx;

@@ -114,8 +114,11 @@ int apx_attn_kv4_async(apx_ctx *ctx, const apx_attn_args *a, const apx_kv4_cache
   if (!a->d_q || !a->d_out || a->ldq < nq || a->ldo < nq || a->ldq * el % 16 ||
       a->ldo * el % 16 || !aligned(a->d_q, 16) || !aligned(a->d_out, 16))
     return APX_ERR_INVALID_ARGUMENT;
-  return apx::launch_attn_kv4(*a, *c, *b, (cudaStream_t)stream) == cudaSuccess ? APX_OK
-                                                                               : APX_ERR_CUDA;
+  int sms;
+  void *work = apx::context_attn_work(ctx, &sms);
+  return apx::launch_attn_kv4(*a, *c, *b, work, sms, (cudaStream_t)stream) == cudaSuccess
+             ? APX_OK
+             : APX_ERR_CUDA;
 }
 
 int apx_sample_async(apx_ctx *ctx, const apx_sample_args *a, void *stream) {

@@ -17,9 +17,14 @@ cudaError_t launch_rope_table(const apx_rope_freqs &f, size_t n_pos, float *tabl
 cudaError_t launch_rope_kv4_append(const apx_rope_args &a, const apx_kv4_cache &c,
                                    const apx_seq_batch &b, cudaStream_t stream);
 
-// apx_attn.cu
+// apx_attn.cu.  work: attn_work_bytes(sms) bytes, zero before the first call that uses them.
+size_t attn_work_bytes(int sms);
 cudaError_t launch_attn_kv4(const apx_attn_args &a, const apx_kv4_cache &c,
-                            const apx_seq_batch &b, cudaStream_t stream);
+                            const apx_seq_batch &b, void *work, int sms, cudaStream_t stream);
+
+// apx_runtime.cu: the context's attention workspace (attn_work_bytes, zeroed when the context was
+// opened) and its SM count.
+void *context_attn_work(apx_ctx *ctx, int *sms);
 
 // apx_sample.cu
 cudaError_t launch_sample(const apx_sample_args &a, cudaStream_t stream);
