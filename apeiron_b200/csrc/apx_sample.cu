@@ -4,211 +4,519 @@
 // The weights are integers, w = rint(e 2^31) with e = exp((l - max) / T) in the F32 carrier's
 // binary32 arithmetic, so sums and comparisons are exact and no order of summation can change
 // the token.  "Sorted by e, lower index first" needs no sort: the filters keep every token whose
-// e exceeds some threshold and the first few, by index, of those equal to it.
+// e exceeds some cut and the first few, by index, of those equal to it.
+//
+// A row's logits are read once, into the registers of a cluster of CTAs.  The bits of e order as
+// e does, 30 of them: the cut is found ten bits at a time from a histogram of counts (top-k) or
+// weight sums (top-p) over the tokens that share the bits found so far.  Each CTA counts in its
+// own shared memory and adds its bins to the first CTA's, which scans them from the top and
+// publishes the bin that crosses the target.  The first level's histogram serves both filters.
+//
+// What bounds it: 4 bytes a logit for many rows; for one row the chain of levels, two cluster
+// barriers each.
+#include <algorithm>
 #include <climits>
 
 #include "apx_common.cuh"
+#include "apx_kernels.h"
+#include "apx_pack.cuh"
 #include "apx_step.h"
 #include "apx_swiglu.cuh"
 
 namespace apx {
 
-constexpr int kSampleThreads = 1024;
-constexpr float kWeightOne = 2147483648.0f;  // 2^31
+namespace {
 
-struct SampleRow {
-  const float *x;
-  size_t vocab;
-  float top, inv_t;
-  // e as its bits: they order as e does (e >= 0)
-  __device__ unsigned key(size_t i) const {
-    const float l = x[i];
-    if (!(l > -INFINITY)) return 0u;  // NaN and -inf
-    if (l == top) return 0x3F800000u;
-    return __float_as_uint(exp_ref(__fmul_rn(__fsub_rn(l, top), inv_t)));
-  }
-};
+constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kBins = 1024;  // ten bits of the key a level
+constexpr int kMaxCluster = 16;
+constexpr unsigned kTopKey = 0x3F800000u;  // e = 1
+constexpr float kWeightOne = 2147483648.0f;  // 2^31
+typedef unsigned long long u64;
 
 __device__ __forceinline__ unsigned weight_of(unsigned key) {
   return __float2uint_rn(__uint_as_float(key) * kWeightOne);
 }
 
-// Sum over the CTA, the same in every thread.
-__device__ unsigned long long cta_sum(unsigned long long v, unsigned long long *s) {
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) s[threadIdx.x / 32] = v;
-  __syncthreads();
-  v = 0;
-  for (int i = 0; i < (int)blockDim.x / 32; i++) v += s[i];
+__device__ __forceinline__ void cluster_sync() {
+  cluster_arrive_release();
+  cluster_wait_acquire();
+}
+__device__ __forceinline__ void red_cluster(uint32_t addr, unsigned v) {
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(addr), "r"(v)
+               : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, u64 v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ u64 ld_cluster(uint32_t addr) {
+  u64 v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
   return v;
 }
 
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(apx_sample_args a) {
-  __shared__ unsigned long long s_sum[32], s_scan[kSampleThreads];
-  __shared__ float s_top[32];
-  __shared__ int s_at;
-  const size_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  SampleRow r;
-  r.x = a.d_logits + row * a.ld;
-  r.vocab = a.vocab;
-  float top = -INFINITY;
-  for (size_t i = tid; i < a.vocab; i += blockDim.x) top = fmaxf(top, r.x[i]);
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  if (tid % 32 == 0) s_top[tid / 32] = top;
-  if (tid == 0) s_at = INT_MAX;
+// What the first CTA publishes of a level: the bin, and the counts and sums above it.
+struct Found {
+  u64 bin, count, sum;
+};
+
+struct Shared {
+  unsigned cnt[kBins], lo[kBins], hi[kBins];     // this CTA's bins: sums in 16-bit halves
+  unsigned mcnt[kBins], mlo[kBins], mhi[kBins];  // the cluster's (first CTA): 24-bit parts
+  u64 warp_sum[kWarps];
+  unsigned warp_cnt[kWarps];
+  Found found[2];  // by turns: one is read while the next is written
+  u64 total;       // the weights of the level scanned last
+  u64 part[kMaxCluster][3];  // of each CTA: the weights above the cut, their number, the ties
+  float top[kMaxCluster];
+  int first[kMaxCluster];
+  float wtop[kWarps];
+  u64 chunk_w[8][kWarps];  // of 128 consecutive tokens
+  unsigned chunk_e[8][kWarps];
+  u64 pick[3];
+};
+
+// Sum over the CTA, in every thread.
+__device__ u64 cta_sum(u64 v, Shared &s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   __syncthreads();
-  for (int i = 0; i < 32; i++) top = fmaxf(top, s_top[i]);
-  r.top = top;
+  if (threadIdx.x % 32 == 0) s.warp_sum[threadIdx.x / 32] = v;
+  __syncthreads();
+  v = s.warp_sum[threadIdx.x % 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+
+// A cluster per row; IPT tokens per thread, in quads: quad j of thread t is 4 (j 1024 + t).
+template <int IPT>
+__global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, int ctas) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int rank = blockIdx.x % ctas;
+  const size_t row = blockIdx.x / ctas;
+  const unsigned vocab = (unsigned)a.vocab;
+  const unsigned per = (vocab + 4 * ctas - 1) / (4 * ctas) * 4;  // tokens of a CTA
+  const unsigned v0 = min(per * rank, vocab), v1 = min(v0 + per, vocab);
+  pdl_launch_dependents();
+  s.cnt[tid] = s.lo[tid] = s.hi[tid] = s.mcnt[tid] = s.mlo[tid] = s.mhi[tid] = 0;
+  pdl_wait();
+  const float *x = a.d_logits + row * a.ld;
   const float temp = a.d_temperature ? a.d_temperature[row] : 1.0f;
-  if (top == -INFINITY) {
-    if (tid == 0) {
+  const int k = a.d_top_k ? a.d_top_k[row] : 0;
+  const float top_p = a.d_top_p ? a.d_top_p[row] : 1.0f;
+  const float min_p = a.d_min_p ? a.d_min_p[row] : 0.0f;
+  const float u = a.d_u[row];
+
+  // ---- the logits, once; tokens past the end are excluded ones ----
+  unsigned key[IPT];  // the logit's bits, then e's
+  const bool quads = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < IPT / 4; j++) {
+    const unsigned i = v0 + 4 * (j * kThreads + tid);
+    float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (quads && i + 4 <= v1) {
+      f = __ldg(reinterpret_cast<const float4 *>(x + i));
+    } else {
+      if (i < v1) f.x = x[i];
+      if (i + 1 < v1) f.y = x[i + 1];
+      if (i + 2 < v1) f.z = x[i + 2];
+      if (i + 3 < v1) f.w = x[i + 3];
+    }
+    top = fmaxf(top, fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w)));
+    key[4 * j] = __float_as_uint(f.x), key[4 * j + 1] = __float_as_uint(f.y);
+    key[4 * j + 2] = __float_as_uint(f.z), key[4 * j + 3] = __float_as_uint(f.w);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  if (lane == 0) s.wtop[warp] = top;
+  __syncthreads();
+  top = s.wtop[lane];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  // every CTA's maximum to every CTA (the first barrier also says that all of them run)
+  cluster_sync();
+  if (tid < ctas)
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_map(&s.top[rank], tid)), "f"(top)
+                 : "memory");
+  cluster_sync();
+  for (int i = 0; i < ctas; i++) top = fmaxf(top, s.top[i]);
+
+  if (top == -INFINITY) {  // nothing left
+    if (rank == 0 && tid == 0) {
       a.d_token[row] = -1;
       if (a.d_prob) a.d_prob[row] = 0.0f;
       if (a.d_kept) a.d_kept[row] = 0;
     }
     return;
   }
-  if (!(temp > 0.0f)) {
-    for (size_t i = tid; i < a.vocab; i += blockDim.x)
-      if (r.x[i] == top) {
-        atomicMin(&s_at, (int)i);
-        break;
-      }
+  if (!(temp > 0.0f)) {  // the largest logit, lowest index
+    int at = INT_MAX;
+#pragma unroll
+    for (int i = IPT - 1; i >= 0; i--)
+      if (__uint_as_float(key[i]) == top) at = (int)(v0 + 4 * (i / 4 * kThreads + tid) + i % 4);
+    at = __reduce_min_sync(0xFFFFFFFFu, at);
+    if (lane == 0) s.warp_cnt[warp] = (unsigned)at;
     __syncthreads();
-    if (tid == 0) {
-      a.d_token[row] = s_at;
+    at = __reduce_min_sync(0xFFFFFFFFu, (int)s.warp_cnt[lane]);
+    if (tid == 0)
+      asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(cluster_map(&s.first[rank], 0)),
+                   "r"(at)
+                   : "memory");
+    cluster_sync();
+    if (rank == 0 && tid == 0) {
+      for (int i = 0; i < ctas; i++) at = min(at, s.first[i]);
+      a.d_token[row] = at;
       if (a.d_prob) a.d_prob[row] = 1.0f;
       if (a.d_kept) a.d_kept[row] = 1;
     }
     return;
   }
-  r.inv_t = __frcp_rn(temp);
+
+  // ---- e ----
+  const float inv = __frcp_rn(temp);
+#pragma unroll
+  for (int i = 0; i < IPT; i++) {
+    const float l = __uint_as_float(key[i]);
+    key[i] = !(l > -INFINITY) ? 0u  // NaN and -inf
+             : l == top       ? kTopKey
+                              : __float_as_uint(exp_ref(__fmul_rn(__fsub_rn(l, top), inv)));
+  }
+
+  const bool by_k = k > 0 && (unsigned)k < vocab, by_p = top_p < 1.0f;
   // tokens with key > cut stay, and the first `ties` of those with key == cut
   unsigned cut = 0;
-  unsigned long long ties = ULLONG_MAX;
-  const long long k = a.d_top_k ? a.d_top_k[row] : 0;
-  if (k > 0 && (size_t)k < a.vocab) {
-    for (int bit = 29; bit >= 0; bit--) {  // the largest cut that k tokens reach
-      const unsigned t = cut | 1u << bit;
-      unsigned long long n = 0;
-      for (size_t i = tid; i < a.vocab; i += blockDim.x) n += r.key(i) >= t;
-      if (cta_sum(n, s_sum) >= (unsigned long long)k) cut = t;
+  u64 ties = ULLONG_MAX;
+
+  // One level's histogram over the keys in (floor, ..) whose bits above shift + 10 are `prefix`,
+  // scanned by the first CTA from the top; thread t there holds bin 1023 - t: `count` and `sum`
+  // of the bins above it, `own_count` and `own_sum` its own.
+  u64 count = 0, sum = 0, own_count = 0, own_sum = 0;
+  auto level = [&](int shift, unsigned prefix, unsigned floor, bool counts, bool sums, u64 lump,
+                   unsigned lump_key) {
+#pragma unroll
+    for (int i = 0; i < IPT; i++) {
+      const unsigned v = key[i];
+      if (v > floor && (shift == 20 || v >> (shift + 10) == prefix)) {
+        const unsigned b = v >> shift & (kBins - 1);
+        if (counts) atomicAdd(&s.cnt[b], 1u);
+        if (sums) {
+          const unsigned w = weight_of(v);
+          atomicAdd(&s.lo[b], w & 0xFFFFu);
+          atomicAdd(&s.hi[b], w >> 16);
+        }
+      }
     }
-    unsigned long long n = 0;
-    for (size_t i = tid; i < a.vocab; i += blockDim.x) n += r.key(i) > cut;
-    ties = (unsigned long long)k - cta_sum(n, s_sum);
+    __syncthreads();
+    // this CTA's bin to the first CTA's: a sum below 2^47 as two parts of 24 bits
+    const unsigned c = s.cnt[tid];
+    const u64 w = ((u64)s.hi[tid] << 16) + s.lo[tid];
+    if (c) red_cluster(cluster_map(&s.mcnt[tid], 0), c);
+    if (w) {
+      red_cluster(cluster_map(&s.mlo[tid], 0), (unsigned)w & 0xFFFFFFu);
+      red_cluster(cluster_map(&s.mhi[tid], 0), (unsigned)(w >> 24));
+    }
+    s.cnt[tid] = s.lo[tid] = s.hi[tid] = 0;
+    cluster_sync();
+    if (rank == 0) {
+      const int b = kBins - 1 - tid;
+      own_count = s.mcnt[b];
+      own_sum = ((u64)s.mhi[b] << 24) + s.mlo[b];
+      s.mcnt[b] = s.mlo[b] = s.mhi[b] = 0;
+      if (lump && (shift == 20 || lump_key >> (shift + 10) == prefix) &&
+          (lump_key >> shift & (kBins - 1)) == (unsigned)b)
+        own_sum += lump;
+      u64 rc = own_count, rs = own_sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned tc = __shfl_up_sync(0xFFFFFFFFu, (unsigned)rc, o);
+        const u64 ts = __shfl_up_sync(0xFFFFFFFFu, rs, o);
+        if (lane >= o) rc += tc, rs += ts;
+      }
+      if (lane == 31) s.warp_cnt[warp] = (unsigned)rc, s.warp_sum[warp] = rs;
+      __syncthreads();
+      unsigned bc = lane < warp ? s.warp_cnt[lane] : 0;
+      u64 bs = lane < warp ? s.warp_sum[lane] : 0;
+      bc = __reduce_add_sync(0xFFFFFFFFu, bc);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) bs += __shfl_xor_sync(0xFFFFFFFFu, bs, o);
+      count = rc + bc - own_count;
+      sum = rs + bs - own_sum;
+      if (tid == kThreads - 1) s.total = sum + own_sum;
+    }
+  };
+  // The first CTA's word on the level just scanned, to every thread of the cluster.
+  int turn = 0;
+  auto publish = [&](bool crosses, u64 bin, u64 over_count, u64 over_sum) {
+    turn ^= 1;
+    if (rank == 0 && crosses) s.found[turn] = Found{bin, over_count, over_sum};
+    cluster_sync();
+    const uint32_t f = cluster_map(&s.found[turn], 0);
+    Found r;
+    r.bin = ld_cluster(f);
+    r.count = ld_cluster(f + 8);
+    r.sum = ld_cluster(f + 16);
+    return r;
+  };
+  auto level_total = [&] { return ld_cluster(cluster_map(&s.total, 0)); };
+
+  if (by_k || by_p) {
+    level(20, 0, 0, by_k, by_p, 0, 0);
+    // the first level, kept for top-p
+    const u64 sum1 = sum, own1 = own_sum;
+    u64 all = 0;         // the weights of all tokens that stay
+    unsigned bin_k = 0;  // the first ten bits of the cut
+    Found f;
+    if (by_k) {
+      // key 0 is not counted: with fewer than k others the cut stays at 0
+      u64 over = 0, over_sum = 0;
+      unsigned prefix = 0;
+      bool short_of_k = false;
+      for (int shift = 20; shift >= 0; shift -= 10) {
+        if (shift < 20) level(shift, prefix, 0, true, by_p, 0, 0);
+        const bool few = shift == 20 && tid == kThreads - 1 && count + own_count < (u64)k;
+        const bool crosses = over + count < (u64)k && over + count + own_count >= (u64)k;
+        f = publish(crosses || few, few ? ULLONG_MAX : kBins - 1 - tid, over + count,
+                    over_sum + sum);
+        if (f.bin == ULLONG_MAX) {
+          short_of_k = true;
+          all = level_total();
+          break;
+        }
+        if (shift == 20) bin_k = (unsigned)f.bin;
+        over = f.count;
+        over_sum = f.sum;
+        prefix = prefix << 10 | (unsigned)f.bin;
+      }
+      if (!short_of_k) {
+        cut = prefix;
+        ties = (u64)k - over;
+        all = over_sum + ties * weight_of(cut);
+      }
+    }
+    if (by_p) {
+      const bool cutting = cut != 0;
+      if (!by_k) {  // the total is the first CTA's
+        publish(false, 0, 0, 0);
+        all = level_total();
+      }
+      const double limit = (double)top_p * (double)all;
+      unsigned t = kTopKey;
+      u64 over = 0, n = 1;
+      if (limit > 0.0) {
+        const u64 lump = cutting ? ties * weight_of(cut) : 0;
+        unsigned prefix = 0;
+        for (int shift = 20; shift >= 0; shift -= 10) {
+          u64 own = own_sum;
+          if (shift == 20) {
+            const unsigned b = kBins - 1 - tid;
+            sum = sum1;
+            own = !cutting || b > bin_k ? own1 : b == bin_k ? all - sum1 : 0;
+            if (cutting && b < bin_k) sum = all;
+          } else {
+            level(shift, prefix, cut, false, true, lump, cut);
+            own = own_sum;
+          }
+          const bool crosses =
+              (double)(over + sum) < limit && (double)(over + sum + own) >= limit;
+          f = publish(crosses, kBins - 1 - tid, 0, over + sum);
+          over = f.sum;
+          prefix = prefix << 10 | (unsigned)f.bin;
+        }
+        t = prefix;
+        // of the tokens at t, those before which less than limit was summed
+        const u64 each = weight_of(t);
+        n = (u64)((limit - (double)over) / (double)each);
+        n = n > 1 ? n - 1 : 0;
+        while ((double)(over + n * each) < limit) n++;
+      }
+      if (t > cut) {
+        cut = t;
+        ties = n;
+      } else {
+        ties = n < ties ? n : ties;
+      }
+    }
   }
-  const float top_p = a.d_top_p ? a.d_top_p[row] : 1.0f;
-  if (top_p < 1.0f) {
-    unsigned long long above = 0, equal = 0;
-    for (size_t i = tid; i < a.vocab; i += blockDim.x) {
-      const unsigned key = r.key(i);
-      if (key > cut) above += weight_of(key);
-      equal += key == cut;
+
+  // ---- the weights that stay, of each CTA to every CTA ----
+  const double min_w = (double)min_p * (double)kWeightOne;
+  // (double)w < min_w for whole w: w below the next whole number
+  const unsigned least = min_w > 0.0 ? (unsigned)fmin(ceil(min_w), 4294967295.0) : 0u;
+  const unsigned cut_w = cut ? weight_of(cut) : 0u, tie_w = cut_w >= least ? cut_w : 0u;
+  auto above = [&](unsigned v) {  // its weight if it stays for being above the cut
+    const unsigned w = v > cut ? weight_of(v) : 0u;
+    return w >= least ? w : 0u;
+  };
+  u64 w_above = 0, n_pair = 0;  // counts: above the cut in the low half, ties in the high
+#pragma unroll
+  for (int i = 0; i < IPT; i++) {
+    const unsigned w = above(key[i]);
+    w_above += w;
+    n_pair += (u64)(w != 0) + ((u64)(cut != 0 && key[i] == cut) << 32);
+  }
+  w_above = cta_sum(w_above, s);
+  n_pair = cta_sum(n_pair, s);
+  if (tid < ctas) {
+    const uint32_t at = cluster_map(&s.part[rank][0], tid);
+    st_cluster(at, w_above);
+    st_cluster(at + 8, n_pair & 0xFFFFFFFFull);
+    st_cluster(at + 16, n_pair >> 32);
+  }
+  cluster_sync();
+  u64 total = 0, kept = 0, before = 0, eq_before = 0, eq_seen = 0;
+  for (int i = 0; i < ctas; i++) {
+    const u64 eq = s.part[i][2];
+    const u64 left = ties > eq_seen ? ties - eq_seen : 0;
+    const u64 some = min(eq, left);  // of this CTA's ties, those that stay
+    if (i == rank) {
+      before = total;
+      eq_before = eq_seen;
     }
-    above = cta_sum(above, s_sum);
-    equal = cta_sum(equal, s_sum);
-    const unsigned long long first = ties < equal ? ties : equal;
-    const double limit = (double)top_p * (double)(above + first * weight_of(cut));
-    // the smallest t whose heavier tokens sum to less than limit
-    unsigned t = 0x3F800000u;
-    unsigned long long over = 0;  // the sum above t
-    if (limit > 0.0) {
-      unsigned lo = cut, hi = 0x3F800000u;
-      while (lo < hi) {
-        const unsigned mid = lo + (hi - lo) / 2;
-        unsigned long long w = 0;
-        for (size_t i = tid; i < a.vocab; i += blockDim.x) {
-          const unsigned key = r.key(i);
-          if (key > mid) w += weight_of(key);
-        }
-        w = cta_sum(w, s_sum);
-        if ((double)w < limit) hi = mid;
-        else lo = mid + 1;
+    total += s.part[i][0] + some * tie_w;
+    kept += s.part[i][1] + (tie_w ? some : 0);
+    eq_seen += eq;
+  }
+  if (total == 0) {
+    if (rank == 0 && tid == 0) {
+      a.d_token[row] = -1;
+      if (a.d_prob) a.d_prob[row] = 0.0f;
+      if (a.d_kept) a.d_kept[row] = 0;
+    }
+    return;
+  }
+  u64 aim = u > 0.0f ? (u64)((double)u * (double)total) : 0;
+  if (aim >= total) aim = total - 1;
+  if (rank == 0 && tid == 0 && a.d_kept) a.d_kept[row] = (int)kept;
+  const u64 eq_left = ties > eq_before ? ties - eq_before : 0;  // ties that stay from here on
+  const u64 here = w_above + min(s.part[rank][2], eq_left) * tie_w;
+  if (aim < before || aim >= before + here) return;
+
+  // ---- the token: in this CTA, by runs of 128, then by lane ----
+#pragma unroll
+  for (int j = 0; j < IPT / 4; j++) {
+    u64 w = 0;
+    unsigned e = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      w += above(key[4 * j + i]);
+      e += cut != 0 && key[4 * j + i] == cut;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
+    e = __reduce_add_sync(0xFFFFFFFFu, e);
+    if (lane == 0) s.chunk_w[j][warp] = w, s.chunk_e[j][warp] = e;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    u64 run = before, eq = 0;
+    for (int j = 0; j < IPT / 4; j++) {
+      const u64 w = s.chunk_w[j][lane];
+      const unsigned e = s.chunk_e[j][lane];
+      unsigned ep = e;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned t = __shfl_up_sync(0xFFFFFFFFu, ep, o);
+        if (lane >= o) ep += t;
       }
-      t = lo;
-      unsigned long long w = 0;
-      for (size_t i = tid; i < a.vocab; i += blockDim.x) {
-        const unsigned key = r.key(i);
-        if (key > t) w += weight_of(key);
+      const u64 e0 = eq + ep - e;  // ties of this CTA before the run
+      const u64 some = min((u64)e, eq_left > e0 ? eq_left - e0 : 0);
+      u64 mine = w + some * tie_w, wp = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 t = __shfl_up_sync(0xFFFFFFFFu, wp, o);
+        if (lane >= o) wp += t;
       }
-      over = cta_sum(w, s_sum);
-    }
-    // of the tokens at t, those before which less than limit was summed; at least one at the top
-    const unsigned long long each = weight_of(t);
-    unsigned long long n = ULLONG_MAX;
-    if (limit <= 0.0) {
-      n = 1;
-    } else if (each) {
-      n = (unsigned long long)((limit - (double)over) / (double)each);
-      n = n > 1 ? n - 1 : 0;
-      while ((double)(over + n * each) < limit) n++;
-    }
-    if (t > cut) {
-      cut = t;
-      ties = n;
-    } else {
-      ties = n < ties ? n : ties;
+      const u64 w0 = run + wp - mine;
+      if (w0 <= aim && aim < w0 + mine) {
+        s.pick[0] = (u64)(j * 32 + lane);
+        s.pick[1] = w0;
+        s.pick[2] = e0;
+      }
+      run += __shfl_sync(0xFFFFFFFFu, wp, 31);
+      eq += __shfl_sync(0xFFFFFFFFu, ep, 31);
     }
   }
-  const double min_w = a.d_min_p ? (double)a.d_min_p[row] * (double)kWeightOne : 0.0;
-  // two passes in vocabulary order: the kept weights' sum, then the token at which it passes
-  // the aim; a CTA scan ranks the tokens that equal the cut
-  unsigned long long total = 0, kept = 0, aim = 0;
-  for (int pass = 0; pass < 2; pass++) {
-    unsigned long long run = 0, seen = 0;
-    for (size_t base = 0; base < a.vocab; base += blockDim.x) {
-      const size_t i = base + tid;
-      const unsigned key = i < a.vocab ? r.key(i) : 0u;
-      const bool here = i < a.vocab;
-      auto scan = [&](unsigned long long v, unsigned long long &sum) {  // exclusive
-        __syncthreads();
-        s_scan[tid] = v;
-        __syncthreads();
-        for (int o = 1; o < kSampleThreads; o <<= 1) {
-          const unsigned long long u = tid >= o ? s_scan[tid - o] : 0;
-          __syncthreads();
-          s_scan[tid] += u;
-          __syncthreads();
-        }
-        sum = s_scan[kSampleThreads - 1];
-        return s_scan[tid] - v;
-      };
-      unsigned long long sum;
-      const unsigned long long rank = seen + scan(here && key == cut, sum);
-      seen += sum;
-      unsigned w = here && (key > cut || (key == cut && rank < ties)) ? weight_of(key) : 0u;
-      if ((double)w < min_w) w = 0;
-      const unsigned long long before = run + scan(w, sum);
-      if (pass == 1 && w && before <= aim && aim < before + w) {
-        a.d_token[row] = (int)i;
-        if (a.d_prob) a.d_prob[row] = (float)((double)w / (double)total);
-      }
-      run += sum;
-      if (pass == 0) kept += w != 0;
+  __syncthreads();
+  if (warp != (int)(s.pick[0] % 32)) return;
+  const int jj = (int)(s.pick[0] / 32);
+#pragma unroll
+  for (int j = 0; j < IPT / 4; j++) {
+    if (j != jj) continue;
+    unsigned e = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) e += cut != 0 && key[4 * j + i] == cut;
+    unsigned ep = e;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned t = __shfl_up_sync(0xFFFFFFFFu, ep, o);
+      if (lane >= o) ep += t;
     }
-    if (pass == 0) {
-      total = run;
-      kept = cta_sum(kept, s_sum);
-      if (tid == 0 && a.d_kept) a.d_kept[row] = (int)kept;
-      if (total == 0) {
-        if (tid == 0) {
-          a.d_token[row] = -1;
-          if (a.d_prob) a.d_prob[row] = 0.0f;
-        }
-        return;
+    u64 at = s.pick[2] + ep - e;
+    unsigned w[4];
+    u64 mine = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      w[i] = above(key[4 * j + i]);
+      if (cut != 0 && key[4 * j + i] == cut) {
+        if (at < eq_left) w[i] = tie_w;
+        at++;
       }
-      aim = (unsigned long long)((double)a.d_u[row] * (double)total);
-      if (aim >= total) aim = total - 1;
+      mine += w[i];
+    }
+    u64 wp = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 t = __shfl_up_sync(0xFFFFFFFFu, wp, o);
+      if (lane >= o) wp += t;
+    }
+    u64 w0 = s.pick[1] + wp - mine;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (w0 <= aim && aim < w0 + w[i]) {
+        a.d_token[row] = (int)(v0 + 4 * (j * kThreads + tid) + i);
+        if (a.d_prob) a.d_prob[row] = (float)((double)w[i] / (double)total);
+      }
+      w0 += w[i];
     }
   }
 }
 
+template <int IPT>
+cudaError_t launch(const apx_sample_args &a, int ctas, cudaStream_t stream) {
+  auto kern = sample_kernel<IPT>;
+  if (ctas > 8) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)ctas, 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.rows * ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_allowed() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, a, ctas);
+}
+
+}  // namespace
+
 cudaError_t launch_sample(const apx_sample_args &a, cudaStream_t stream) {
-  sample_kernel<<<(unsigned)a.rows, kSampleThreads, 0, stream>>>(a);
-  return cudaGetLastError();
+  // the fewest CTAs whose registers hold the row in 20 tokens a thread, in 32 past 16 x 20
+  int ctas = 1;
+  while (ctas < kMaxCluster && (size_t)ctas * kThreads * 20 < a.vocab) ctas *= 2;
+  const size_t per = ((a.vocab + 4 * ctas - 1) / (4 * ctas) * 4 + kThreads - 1) / kThreads;
+  if (per <= 4) return launch<4>(a, ctas, stream);
+  if (per <= 12) return launch<12>(a, ctas, stream);
+  if (per <= 20) return launch<20>(a, ctas, stream);
+  return launch<32>(a, ctas, stream);
 }
 
 }  // namespace apx
