@@ -214,14 +214,13 @@ _SIGS = {
     "apx_matvec_f32_noalloc": (C.c_int, [P, U64, SZ, SZ, P, P, P, P]),
     "apx_matmat_f32": (C.c_int, [P, U64, SZ, SZ, SZ, P, P, EP]),
     "apx_quant_f32_cols_async": (C.c_int, [P, P, SZ, SZ, P, P, P, P]),
-    "apx_add_rms_norm_quant_async": (C.c_int, [P, C.POINTER(NormArgs), P]),
+    # the argument structs of these cross as their bytes or by reference
+    "apx_add_rms_norm_quant_async": (C.c_int, [P, P, P]),
     "apx_kv4_page_bytes": (SZ, [C.c_int, C.c_int]),
     "apx_rope_table_async": (C.c_int, [P, C.POINTER(RopeFreqs), SZ, P, P]),
-    "apx_rope_kv4_append_async": (C.c_int, [P, C.POINTER(RopeArgs), C.POINTER(Kv4Cache),
-                                            C.POINTER(SeqBatch), P]),
-    "apx_attn_kv4_async": (C.c_int, [P, C.POINTER(AttnArgs), C.POINTER(Kv4Cache),
-                                     C.POINTER(SeqBatch), P]),
-    "apx_sample_async": (C.c_int, [P, C.POINTER(SampleArgs), P]),
+    "apx_rope_kv4_append_async": (C.c_int, [P, P, P, P, P]),
+    "apx_attn_kv4_async": (C.c_int, [P, P, P, P, P]),
+    "apx_sample_async": (C.c_int, [P, P, P]),
 }
 
 _lib = None

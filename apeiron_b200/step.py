@@ -11,6 +11,7 @@ allocated otherwise.  A refused argument raises ``ValueError``, a backend condit
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -24,6 +25,16 @@ _SCALINGS = {None: _abi.ROPE_PLAIN, "linear": _abi.ROPE_LINEAR, "bands": _abi.RO
              "ramp": _abi.ROPE_RAMP}
 
 
+# A call's argument struct, packed in one go (the mirrors in _abi hold the same layout).
+_NORM = struct.Struct("@9P7Nfi").pack
+_ROPE = struct.Struct("@8P5N4i").pack
+_ATTN = struct.Struct("@3P2N2if3i0P").pack
+_SAMPLE = struct.Struct("@9P3N").pack
+
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
+
+
 def _need(ok, what):
     if not ok:
         raise ValueError(what)
@@ -33,26 +44,32 @@ def _vector(t, n, dtype, name):
     """The address of a contiguous vector of n elements; 0 for None."""
     if t is None:
         return 0
-    _need(t.is_cuda and t.dtype is dtype and t.numel() == n and t.is_contiguous(),
-          f"{name}: a contiguous CUDA tensor of {n} {dtype} elements is wanted")
+    if not (t.dtype is dtype and t.numel() == n and t.is_cuda and t.is_contiguous()):
+        raise ValueError(f"{name}: a contiguous CUDA tensor of {n} {dtype} elements is wanted")
     return t.data_ptr()
 
 
-def _rows(t, shape, name, dtype=None):
-    """(address, elements between rows) of a tensor of `shape` (rows first) whose rows are each
-    contiguous; (0, 0) for None."""
-    if t is None:
-        return 0, 0
-    _need(t.is_cuda and t.shape == shape and (dtype is None or t.dtype is dtype),
-          f"{name}: a CUDA tensor of shape {tuple(shape)}{f' and {dtype}' if dtype else ''} is "
-          "wanted")
-    width = 1
-    for size, stride in zip(reversed(shape[1:]), reversed(t.stride()[1:])):
-        _need(stride == width or size == 1, f"{name}: its rows are not contiguous")
-        width *= size
-    ld = t.stride(0) if shape[0] > 1 else width
-    _need(ld >= width, f"{name}: its rows overlap")
-    return t.data_ptr(), ld
+def _rows(t, shape, name, dtype):
+    """The elements between rows of a tensor of `shape` (2 or 3 dims, rows first) whose rows are
+    each contiguous."""
+    st = t.stride()
+    if t.dtype is dtype and t.is_cuda and t.shape == shape:
+        if len(st) == 2:
+            width = shape[1]
+            if st[1] == 1 or width == 1:
+                if st[0] >= width:
+                    return st[0]
+                if shape[0] <= 1:
+                    return width
+        else:
+            width = shape[1] * shape[2]
+            if st[2] == 1 and (st[1] == shape[2] or shape[1] == 1):
+                if st[0] >= width:
+                    return st[0]
+                if shape[0] <= 1:
+                    return width
+    raise ValueError(f"{name}: a CUDA tensor {tuple(shape)} of {dtype} is wanted, its rows "
+                     "contiguous and apart")
 
 
 class DeviceAct:
@@ -125,22 +142,25 @@ class StepOps:
     def __init__(self, backend: Backend):
         self.backend, self.lib, self.ctx = backend, backend.lib, backend.ctx
         self.device = torch.device("cuda", backend.device)
+        self._index = backend.device
+        lib = self.lib
+        self._norm, self._rope = lib.apx_add_rms_norm_quant_async, lib.apx_rope_kv4_append_async
+        self._attn, self._sample = lib.apx_attn_kv4_async, lib.apx_sample_async
 
     def _stream(self, stream):
-        return torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream
+        return _raw_stream(self._index) if stream is None else stream
 
     @staticmethod
-    def _done(rc, name):
+    def _failed(rc, name):
         if rc in (_abi.APX_ERR_INVALID_ARGUMENT, _abi.APX_ERR_LAYOUT_MISMATCH,
                   _abi.APX_ERR_TOO_LARGE):
             raise ValueError(f"{name}: refused with code {rc}")
-        if rc:
-            raise BackendError(f"{name}: backend error {rc}")
+        raise BackendError(f"{name}: backend error {rc}")
 
     # -- refusals that the device finds -------------------------------------------------------
     def new_status(self):
         """Status words with nothing refused."""
-        return torch.full((2,), -1, dtype=torch.int64, device=self.device)
+        return torch.full((2,), -1, dtype=_I64, device=self.device)
 
     @staticmethod
     def check_status(status):
@@ -152,115 +172,104 @@ class StepOps:
     def add_rms_norm_quant(self, x, weight, eps, *, add=None, resid=None, act=None, deq=None,
                            y=None, stream=None):
         """h = x + add into ``resid`` (may be x), h * weight / rms(h) into ``y`` (f32), ``act``
-        (a DeviceAct, allocated when no output is given) and ``deq`` (the activation's values).
-        x, add: (k, n) f32.  Returns act."""
-        k, n = x.shape
+        (a DeviceAct, allocated when no output is given) and ``deq`` (the activation's values,
+        f32 or bf16).  x, add: (k, n) f32; weight: n f32, or None.  Returns act."""
+        shape = x.shape
+        k, n = shape
         if act is None and deq is None and y is None:
             act = DeviceAct.empty(self, k, n)
-        a = _abi.NormArgs()
-        f32 = torch.float32
-        a.d_x, a.ldx = _rows(x, x.shape, "x", f32)
-        a.d_weight = _vector(weight, n, f32, "weight")
-        if add is not None:
-            a.d_add, a.ld_add = _rows(add, x.shape, "add", f32)
-        if resid is not None:
-            a.d_resid, a.ld_resid = _rows(resid, x.shape, "resid", f32)
-        if y is not None:
-            a.d_y, a.ldy = _rows(y, x.shape, "y", f32)
-        if deq is not None:
-            a.d_deq, a.ld_deq = _rows(deq, x.shape, "deq")
-            a.deq_type = _TYPES.get(deq.dtype, -1)
+        codes = exps = descs = 0
         if act is not None:
             _need(act.n == n and act.k == k, f"act: ({k}, {n}) is wanted")
-            a.d_codes, a.d_exps = act.codes.data_ptr(), act.exps.data_ptr()
-            a.d_descs = act.descs.data_ptr()
-        a.n, a.k, a.eps = n, k, eps
-        self._done(self.lib.apx_add_rms_norm_quant_async(self.ctx, C.byref(a),
-                                                         self._stream(stream)),
-                   "add_rms_norm_quant")
+            codes, exps, descs = act.codes.data_ptr(), act.exps.data_ptr(), act.descs.data_ptr()
+        rc = self._norm(self.ctx, _NORM(
+            x.data_ptr(), 0 if add is None else add.data_ptr(), _vector(weight, n, _F32, "weight"),
+            0 if resid is None else resid.data_ptr(), 0 if y is None else y.data_ptr(),
+            0 if deq is None else deq.data_ptr(), codes, exps, descs, n, k,
+            _rows(x, shape, "x", _F32),
+            0 if add is None else _rows(add, shape, "add", _F32),
+            0 if resid is None else _rows(resid, shape, "resid", _F32),
+            0 if y is None else _rows(y, shape, "y", _F32),
+            0 if deq is None else _rows(deq, shape, "deq", deq.dtype), eps,
+            0 if deq is None else _TYPES.get(deq.dtype, -1)), self._stream(stream))
+        if rc:
+            self._failed(rc, "add_rms_norm_quant")
         return act
 
     def rope_table(self, n_pos, rot_dim, base=10000.0, *, scaling=None, factor=1.0, low=1.0,
                    high=4.0, original=0.0, mscale=1.0, stream=None):
         """(n_pos, rot_dim / 2, 2) f32 cosines and sines; ``scaling``: None, "linear", "bands" or
         "ramp" (``low`` and ``high``: turns within the ``original`` length)."""
-        table = torch.empty(n_pos, rot_dim // 2, 2, dtype=torch.float32, device=self.device)
+        table = torch.empty(n_pos, rot_dim // 2, 2, dtype=_F32, device=self.device)
         _need(scaling in _SCALINGS, f"scaling: one of {list(_SCALINGS)} is wanted")
         f = _abi.RopeFreqs(base, factor, low, high, original, mscale, rot_dim,
                            _SCALINGS[scaling])
-        self._done(self.lib.apx_rope_table_async(self.ctx, C.byref(f), n_pos, table.data_ptr(),
-                                                 self._stream(stream)), "rope_table")
+        rc = self.lib.apx_rope_table_async(self.ctx, C.byref(f), n_pos, table.data_ptr(),
+                                           self._stream(stream))
+        if rc:
+            self._failed(rc, "rope_table")
         return table
 
     def rope_kv4_append(self, q, k, v, table, cache: KV4Cache, batch: SeqBatch, *, rot_dim,
-                        layout="half", q_out=None, q_type=torch.float32, k_deq=None, v_deq=None,
+                        layout="half", q_out=None, q_type=_F32, k_deq=None, v_deq=None,
                         status=None, stream=None):
         """q (tokens, heads, dim; None to leave out) turned into ``q_out``; k turned and v
         (tokens, kv heads, dim) appended to the cache in 4 bits.  ``k_deq`` / ``v_deq`` (f16):
         the values the cache now holds.  Returns q_out."""
-        f32, t = torch.float32, batch.n_tokens
-        kv = (t, cache.n_kv_heads, cache.head_dim)
-        a = _abi.RopeArgs()
-        a.d_k, a.ldk = _rows(k, kv, "k", f32)
-        a.d_v, a.ldv = _rows(v, kv, "v", f32)
+        t, heads, dim = batch.n_tokens, cache.n_kv_heads, cache.head_dim
+        kv = (t, heads, dim)
+        ldq = ld_out = n_heads = kind = q_ptr = out_ptr = 0
         if q is not None:
-            shape = (t, q.shape[1], cache.head_dim)
+            shape = (t, q.shape[1], dim)
             if q_out is None:
                 q_out = torch.empty(shape, dtype=q_type, device=q.device)
-            a.d_q, a.ldq = _rows(q, shape, "q", f32)
-            a.d_q_out, a.ldq_out = _rows(q_out, shape, "q_out")
-            a.n_heads, a.q_type = shape[1], _TYPES.get(q_out.dtype, -1)
-        n_pos = table.shape[0]
-        a.d_table = _vector(table, n_pos * rot_dim, f32, "table")
-        a.n_pos, a.rot_dim = n_pos, rot_dim
-        a.layout = _LAYOUTS.get(layout, -1)
-        if k_deq is not None:
-            a.d_k_deq = _vector(k_deq, t * kv[1] * kv[2], torch.float16, "k_deq")
-        if v_deq is not None:
-            a.d_v_deq = _vector(v_deq, t * kv[1] * kv[2], torch.float16, "v_deq")
-        if status is not None:
-            a.d_status = _vector(status, 2, torch.int64, "status")
-        self._done(self.lib.apx_rope_kv4_append_async(self.ctx, C.byref(a), cache.ref, batch.ref,
-                                                      self._stream(stream)), "rope_kv4_append")
+            ldq, n_heads = _rows(q, shape, "q", _F32), shape[1]
+            ld_out, kind = _rows(q_out, shape, "q_out", q_out.dtype), _TYPES.get(q_out.dtype, -1)
+            q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
+        n_pos, n = table.shape[0], t * heads * dim
+        rc = self._rope(self.ctx, _ROPE(
+            q_ptr, k.data_ptr(), v.data_ptr(), _vector(table, n_pos * rot_dim, _F32, "table"),
+            out_ptr, _vector(k_deq, n, torch.float16, "k_deq"),
+            _vector(v_deq, n, torch.float16, "v_deq"), _vector(status, 2, _I64, "status"),
+            n_pos, ldq, _rows(k, kv, "k", _F32), _rows(v, kv, "v", _F32), ld_out,
+            rot_dim, _LAYOUTS.get(layout, -1), n_heads, kind), cache.ref, batch.ref,
+            self._stream(stream))
+        if rc:
+            self._failed(rc, "rope_kv4_append")
         return q_out
 
     def attn_kv4(self, q, cache: KV4Cache, batch: SeqBatch, scale, *, window=0, sinks=0,
                  out=None, status=None, stream=None):
         """softmax(scale * q k^T) v of q (tokens, heads, dim; f32, f16 or bf16) over the cache,
         causal, within ``window`` keys (0: all) and the first ``sinks``.  Returns out."""
-        shape = (batch.n_tokens, q.shape[1], cache.head_dim)
+        heads, dtype = q.shape[1], q.dtype
+        shape = (batch.n_tokens, heads, cache.head_dim)
         if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=q.device)
-        a = _abi.AttnArgs()
-        a.d_q, a.ldq = _rows(q, shape, "q")
-        a.d_out, a.ldo = _rows(out, shape, "out", q.dtype)
-        a.type, a.n_heads = _TYPES.get(q.dtype, -1), shape[1]
-        a.scale, a.window, a.sinks = scale, window, sinks
-        if status is not None:
-            a.d_status = _vector(status, 2, torch.int64, "status")
-        self._done(self.lib.apx_attn_kv4_async(self.ctx, C.byref(a), cache.ref, batch.ref,
-                                               self._stream(stream)), "attn_kv4")
+            out = torch.empty(shape, dtype=dtype, device=q.device)
+        rc = self._attn(self.ctx, _ATTN(
+            q.data_ptr(), out.data_ptr(), _vector(status, 2, _I64, "status"),
+            _rows(q, shape, "q", dtype), _rows(out, shape, "out", dtype),
+            _TYPES.get(dtype, -1), heads, scale, window, sinks, 0), cache.ref, batch.ref,
+            self._stream(stream))
+        if rc:
+            self._failed(rc, "attn_kv4")
         return out
 
     def sample(self, logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None,
                token=None, prob=None, kept=None, stream=None):
         """One token per row of f32 ``logits`` (rows, vocab) from ``u`` (rows) in [0, 1); the
         filters are per row, None to leave out.  Returns token (int32)."""
-        rows, vocab = logits.shape
-        f32, i32 = torch.float32, torch.int32
+        shape = logits.shape
+        rows, vocab = shape
         if token is None:
-            token = torch.empty(rows, dtype=i32, device=logits.device)
-        a = _abi.SampleArgs()
-        a.d_logits, a.ld = _rows(logits, logits.shape, "logits", f32)
-        a.d_u = _vector(u, rows, f32, "u")
-        a.d_temperature = _vector(temperature, rows, f32, "temperature")
-        a.d_top_k = _vector(top_k, rows, i32, "top_k")
-        a.d_top_p = _vector(top_p, rows, f32, "top_p")
-        a.d_min_p = _vector(min_p, rows, f32, "min_p")
-        a.d_token = _vector(token, rows, i32, "token")
-        a.d_prob = _vector(prob, rows, f32, "prob")
-        a.d_kept = _vector(kept, rows, i32, "kept")
-        a.rows, a.vocab = rows, vocab
-        self._done(self.lib.apx_sample_async(self.ctx, C.byref(a), self._stream(stream)),
-                   "sample")
+            token = torch.empty(rows, dtype=_I32, device=logits.device)
+        rc = self._sample(self.ctx, _SAMPLE(
+            logits.data_ptr(), _vector(u, rows, _F32, "u"),
+            _vector(temperature, rows, _F32, "temperature"), _vector(top_p, rows, _F32, "top_p"),
+            _vector(min_p, rows, _F32, "min_p"), _vector(top_k, rows, _I32, "top_k"),
+            _vector(token, rows, _I32, "token"), _vector(prob, rows, _F32, "prob"),
+            _vector(kept, rows, _I32, "kept"), rows, vocab,
+            _rows(logits, shape, "logits", _F32)), self._stream(stream))
+        if rc:
+            self._failed(rc, "sample")
         return token

@@ -34,6 +34,20 @@ def test_struct_layouts_match_the_header(tmp_path, mirror, name):
     assert out == [C.sizeof(mirror)] + [getattr(mirror, f).offset for f in fields]
 
 
+def test_packed_arguments_have_the_structs_layout():
+    """apeiron_b200.step packs each call's arguments in one go: the mirrors' size and offsets."""
+    from apeiron_b200 import step
+
+    for pack, mirror in ((step._NORM, _abi.NormArgs), (step._ROPE, _abi.RopeArgs),
+                         (step._ATTN, _abi.AttnArgs), (step._SAMPLE, _abi.SampleArgs)):
+        kinds = [t for _, t in mirror._fields_]
+        values = [0.5 + i if t is C.c_float else 3 + i for i, t in enumerate(kinds)]
+        raw = pack(*values)
+        assert len(raw) == C.sizeof(mirror)
+        got = mirror.from_buffer_copy(raw)
+        assert [getattr(got, f) for f, _ in mirror._fields_] == values
+
+
 @pytest.fixture(scope="module")
 def lib():
     return _abi.load(build.build())
