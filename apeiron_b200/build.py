@@ -18,7 +18,8 @@ LIB = os.path.join(PKG, "libapeiron_cuda.so")
 SOURCES = ["apx_runtime.cu", "apx_gemv.cu", "apx_quant.cu", "apx_gemm.cu", "apx_lgemm.cu", "apx_ffn.cu",
            "apx_noalloc.cu",
            "apx_peer.cu", "apx_plan.cu",
-           "apx_step.cu", "apx_norm.cu", "apx_rope.cu", "apx_attn.cu", "apx_sample.cu"]
+           "apx_step.cu", "apx_norm.cu", "apx_rope.cu", "apx_attn.cu",
+           "apx_attn_tc.cu", "apx_sample.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

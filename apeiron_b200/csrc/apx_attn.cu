@@ -40,31 +40,14 @@
 
 namespace apx {
 
+// apx_attn_tc.cu
+bool attn_tc_serves(const AttnArgs &p, int dim, int max_q);
+cudaError_t launch_attn_tc(const AttnArgs &p, int dim, int max_q, cudaStream_t stream);
+
 namespace {
 
 constexpr int kStepKeys = 32;
 constexpr float kTopExp = 14.0f;  // probabilities are held at 2^14 e^(s - m)
-
-struct AttnArgs {
-  const void *q;
-  void *out;
-  const uint8_t *pages;
-  const int *cu, *kv_len, *table;
-  unsigned long long *status;
-  unsigned long long ldq, ldo;
-  unsigned long long page_bytes;
-  float *part;     // per CTA: two partial items
-  unsigned *count; // per item: CTAs that have arrived (zero between calls)
-  int n_pages, n_seqs, max_pages, kv_heads, group, page_shift;
-  int window, sinks, type, warps_min, n_tokens;
-  float scale;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
@@ -80,20 +63,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
-__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
-
-// Two codes of x (bits 0-3 and 16-19, or 4-7 and 20-23) as (c - 8) * s: the bits behind 0x6400
-// read 1024 + c, or 1024 + 16 c.
-__device__ __forceinline__ uint32_t low2(uint32_t x, __half2 s) {
-  const __half2 v = u2h((x & 0x000F000Fu) | 0x64006400u);
-  return h2u(__hmul2(__hsub2(v, u2h(0x64086408u)), s));
-}
-__device__ __forceinline__ uint32_t high2(uint32_t x, __half2 s) {
-  const __half2 v = u2h((x & 0x00F000F0u) | 0x64006400u);
-  return h2u(__hmul2(__hfma2(v, u2h(0x2C002C00u), u2h(0xD480D480u)), s));
-}
-
 __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
   const __half2 h = __floats2half2_rn(x, y);
   const float2 f = __half22float2(h);
@@ -107,57 +76,32 @@ __device__ __forceinline__ void store_out(void *o, unsigned long long i, float v
   else static_cast<__nv_bfloat16 *>(o)[i] = __float2bfloat16_rn(v);
 }
 
-__device__ __forceinline__ void refuse(const AttnArgs &p, int seq) {
-  if (p.status)
-    atomicMin(p.status, (unsigned long long)seq << 24 |
-                            (unsigned long long)APX_ERR_INVALID_ARGUMENT << 16);
-}
-
-// A sequence's shape: its query rows (token, head of the group) in blocks of R, and the steps of
-// each.  Blocks pair first with last: a pair has `pair` steps, the first block's, then the
-// second's, then none.
+// A sequence's steps.  Its blocks of rows pair first with last: a pair has `pair` steps, the
+// first block's, then the second's, then none.
 template <int R>
-struct SeqShape {
-  int first, rows, kv, p0, nblk;  // first query token, rows, usable keys, position of row 0
+struct SeqShape : SeqRows<R, kStepKeys> {
+  using Base = SeqRows<R, kStepKeys>;
   int pair;
-  bool bad;
 
   __device__ void load(const AttnArgs &p, int s) {
-    const int a = p.cu[s], b = p.cu[s + 1], n = p.kv_len[s];
-    const long long room = (long long)p.max_pages << p.page_shift;
-    bad = a < 0 || b < a || b > p.n_tokens || n < 0 || n > room;
-    first = a;
-    rows = bad ? 0 : (b - a) * p.group;
-    kv = bad ? 0 : n;
-    p0 = n - (b - a);
-    nblk = (rows + R - 1) / R;
-    if (nblk == 0) pair = 0;
-    else if (nblk == 1) pair = steps(p, 0);
-    else if (!p.window) pair = steps(p, 0) + steps(p, nblk - 1) + 2;
+    Base::load(p, s);
+    const int n = this->nblk;
+    if (n == 0) pair = 0;
+    else if (n == 1) pair = steps(p, 0);
+    else if (!p.window) pair = steps(p, 0) + steps(p, n - 1) + 2;
     else {
       // a window's keys: what the block's positions span, in whole steps
       const int most = p.window + (R - 1) / p.group + 1;
-      pair = 2 * (min(most / kStepKeys + 2 + (min(p.sinks, kv) + kStepKeys - 1) / kStepKeys,
-                      steps_to(kv)) + 1);
-    }
-  }
-  __device__ static int steps_to(int n) { return (max(n, 0) + kStepKeys - 1) / kStepKeys; }
-  // Keys [0, end) and steps [from, ..) that block b sees past the sinks' steps [0, sink).
-  __device__ void range(const AttnArgs &p, int b, int &end, int &sink, int &from) const {
-    const int lo = p0 + b * R / p.group, hi = p0 + min((b + 1) * R - 1, rows - 1) / p.group;
-    end = max(min(kv, hi + 1), 0);
-    sink = from = 0;
-    if (p.window) {
-      from = max(lo - p.window + 1, 0) / kStepKeys;
-      sink = min(steps_to(min(p.sinks, end)), from);
+      pair = 2 * (min(most / kStepKeys + 2 + Base::steps_to(min(p.sinks, this->kv)),
+                      Base::steps_to(this->kv)) + 1);
     }
   }
   __device__ int steps(const AttnArgs &p, int b) const {
     int end, sink, from;
-    range(p, b, end, sink, from);
-    return max(sink + max(steps_to(end) - from, 0), 1);  // one writes the zeros of unseeing rows
+    this->range(p, b, end, sink, from);
+    return max(sink + max(Base::steps_to(end) - from, 0), 1);  // one writes unseeing rows' zeros
   }
-  __device__ int pairs() const { return (nblk + 1) / 2; }
+  __device__ int pairs() const { return (this->nblk + 1) / 2; }
 };
 
 template <int D, int NT, int SPLIT>
@@ -213,7 +157,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
       if (s >= p.n_seqs) break;
       SeqShape<R> q;
       q.load(p, s);
-      if (q.bad && blockIdx.x == 0) refuse(p, s);
+      if (q.bad && blockIdx.x == 0) attn_refuse(p, s, APX_ERR_INVALID_ARGUMENT);
       mine += (unsigned long long)q.pairs() * q.pair * p.kv_heads;
     }
     unsigned long long run = mine;
@@ -307,7 +251,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
           if (key < end) {
             page_at = table[key >> p.page_shift];
             if (page_at < 0 || page_at >= p.n_pages) {
-              refuse(p, seq);
+              attn_refuse(p, seq, APX_ERR_INVALID_ARGUMENT);
               page_at = -1;
             }
           }
@@ -388,9 +332,8 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
         for (int j = 0; j < 4; j++) top = fmaxf(top, fabsf(v[w][j]));
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-      // the largest |q| to [2^9, 2^10); exponents outside the f32 normals are clamped
-      const int e = min(max((int)(__float_as_uint(top) >> 23 & 255), 32), 254) - 127;
-      const float up = __int_as_float((9 - e + 127) << 23);
+      const int e = row_exponent(top);
+      const float up = pow2(9 - e);
 #pragma unroll
       for (int w = 0; w < 2 * K4; w++)
 #pragma unroll
@@ -399,7 +342,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
           split2(v[w][2 * j] * up, v[w][2 * j + 1] * up, qh[n][w][j], lo);
           if (SPLIT == 2) ql[SPLIT == 2 ? n : 0][w][j] = lo;
         }
-      const float c = p.scale * 1.44269504088896341f * __int_as_float((e - 9 + 127) << 23);
+      const float c = p.scale * 1.44269504088896341f * pow2(e - 9);
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         cq[n][j] = __shfl_sync(0xFFFFFFFFu, c, (2 * tig + j) * 4);
@@ -681,8 +624,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
     }
     u = stop;
   }
-  if (!alive && lane == 0 && p.status)
-    atomicMin(p.status, (unsigned long long)APX_ERR_DEVICE_TIMEOUT << 16);
+  if (!alive && lane == 0) attn_refuse(p, 0, APX_ERR_DEVICE_TIMEOUT);
 
   // ---- the join: items that cross warps, then items that cross CTAs ----
   __syncthreads();
@@ -860,6 +802,7 @@ cudaError_t launch_attn_kv4(const apx_attn_args &a, const apx_kv4_cache &c,
   p.warps_min = 1;
   p.scale = a.scale;
   const int grid = std::min(sms, kCountBytes / 4);
+  if (attn_tc_serves(p, c.head_dim, b.max_q)) return launch_attn_tc(p, c.head_dim, b.max_q, stream);
   const bool one = (size_t)b.max_q * p.group <= 8, f32 = a.type == APX_DTYPE_F32;
   if (c.head_dim == 128) {
     if (one) return f32 ? launch_split<128, 1, 2>(p, grid, stream) : launch_split<128, 1, 1>(p, grid, stream);

@@ -1,5 +1,5 @@
-// apx_kv4.cuh — the 4-bit KV cache's tile and the batch's positions, shared by the kernels that
-// write it (apx_rope.cu) and read it (apx_attn.cu).
+// apx_kv4.cuh — the 4-bit KV cache's tile, shared by the kernels that write it (apx_rope.cu) and
+// read it (apx_attn.cu, apx_attn_tc.cu), and what the two attention kernels share.
 //
 // A tile is 16 tokens of one KV head (layout in include/apeiron_cuda.h): K codes, V codes, K
 // scales, V scales; page_tokens / 16 tiles follow each other in a page.
@@ -31,5 +31,87 @@ __host__ __device__ constexpr int kv4_v_byte(int i, int r) {
   const int m = i / 16, g = i % 8, t = (r % 8) / 2;
   return 4 * (((m / 4) * 32 + g * 4 + t) * 4 + m % 4) + (r % 2) * 2 + r / 8;
 }
+
+#ifdef __CUDACC__
+
+// One attention call, as both kernels take it.
+struct AttnArgs {
+  const void *q;
+  void *out;
+  const uint8_t *pages;
+  const int *cu, *kv_len, *table;
+  unsigned long long *status;
+  unsigned long long ldq, ldo;
+  unsigned long long page_bytes;
+  float *part;      // apx_attn.cu: two partial items per CTA
+  unsigned *count;  // apx_attn.cu: CTAs that have arrived at an item (zero between calls)
+  int n_pages, n_seqs, max_pages, kv_heads, group, page_shift;
+  int window, sinks, type, warps_min, n_tokens;
+  float scale;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
+
+// Two codes of x (bits 0-3 and 16-19, or 4-7 and 20-23) as (c - 8) * s: the bits behind 0x6400
+// read 1024 + c, or 1024 + 16 c.
+__device__ __forceinline__ uint32_t low2(uint32_t x, __half2 s) {
+  const __half2 v = u2h((x & 0x000F000Fu) | 0x64006400u);
+  return h2u(__hmul2(__hsub2(v, u2h(0x64086408u)), s));
+}
+__device__ __forceinline__ uint32_t high2(uint32_t x, __half2 s) {
+  const __half2 v = u2h((x & 0x00F000F0u) | 0x64006400u);
+  return h2u(__hmul2(__hfma2(v, u2h(0x2C002C00u), u2h(0xD480D480u)), s));
+}
+
+__device__ __forceinline__ void attn_refuse(const AttnArgs &p, int seq, int code) {
+  if (p.status)
+    atomicMin(p.status, (unsigned long long)seq << 24 | (unsigned long long)code << 16);
+}
+
+// A power of two that brings a row's largest |q| to [2^9, 2^10) (exponents outside the f32
+// normals are clamped), as its exponent's distance: q 2^(9 - e).
+__device__ __forceinline__ int row_exponent(float top) {
+  return min(max((int)(__float_as_uint(top) >> 23 & 255), 32), 254) - 127;
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+// A sequence's query rows (token, head of the group) in blocks of R, and the keys each sees, in
+// steps of KEYS.
+template <int R, int KEYS>
+struct SeqRows {
+  int first, rows, kv, p0, nblk;  // first query token, rows, usable keys, position of row 0
+  bool bad;                       // lengths outside the batch or the cache
+
+  __device__ void load(const AttnArgs &p, int s) {
+    const int a = p.cu[s], b = p.cu[s + 1], n = p.kv_len[s];
+    const long long room = (long long)p.max_pages << p.page_shift;
+    bad = a < 0 || b < a || b > p.n_tokens || n < 0 || n > room;
+    first = a;
+    rows = bad ? 0 : (b - a) * p.group;
+    kv = bad ? 0 : n;
+    p0 = n - (b - a);
+    nblk = (rows + R - 1) / R;
+  }
+  __device__ static int steps_to(int n) { return (max(n, 0) + KEYS - 1) / KEYS; }
+  // Block b sees keys below `end`: those of the sinks' steps [0, sink) and of steps `from` on.
+  __device__ void range(const AttnArgs &p, int b, int &end, int &sink, int &from) const {
+    const int lo = p0 + b * R / p.group, hi = p0 + min((b + 1) * R - 1, rows - 1) / p.group;
+    end = max(min(kv, hi + 1), 0);
+    sink = from = 0;
+    if (p.window) {
+      from = max(lo - p.window + 1, 0) / KEYS;
+      sink = min(steps_to(min(p.sinks, end)), from);
+    }
+  }
+};
+
+#endif  // __CUDACC__
 
 }  // namespace apx
