@@ -15,7 +15,7 @@
 //
 // Numbers.  d (c - 8) is exact in f16 (the append's d has 8 significant bits).  A query row is
 // scaled by a power of two to the top of f16's range and, for f32, split in two halves of 11 bits
-// each; so are the probabilities, taken at 2^14 e^(s - m): 22 bits down to 2^-38 of the largest.
+// each; so are the probabilities, taken at 2^13 e^(s - m): 22 bits down to 2^-38 of the largest.
 // The unit's f32 accumulation is cut into short chains joined by f32 additions.
 //
 // Split.  Work is counted in steps of 32 keys of one item (sequence, KV head, block of query
@@ -47,7 +47,9 @@ cudaError_t launch_attn_tc(const AttnArgs &p, int dim, int max_q, cudaStream_t s
 namespace {
 
 constexpr int kStepKeys = 32;
-constexpr float kTopExp = 14.0f;  // probabilities are held at 2^14 e^(s - m)
+// Probabilities are held at 2^13 e^(s - m), where m is a stale maximum: it moves when a score
+// outgrows it by more than 2^2.
+constexpr float kTopExp = 13.0f, kStale = 2.0f;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
@@ -181,6 +183,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
   auto bound = [&](unsigned long long w) { return min(w, nwarps) * total / nwarps; };
   const unsigned long long u0 = bound(gw), u1 = bound(gw + 1);
 
+  const Unpack un;
   uint32_t phase = 0;  // bit i: the parity that slot i's next wait takes
   int slot = 0;
   bool alive = true;   // no wait has given up
@@ -238,47 +241,33 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
       return (st < sink ? st : st - sink + from) * kStepKeys;
     };
     const uint8_t *head_pages = p.pages + (unsigned long long)head * p.page_bytes;
+    const unsigned long long page_stride = p.kv_heads * p.page_bytes;
     const int *table = p.table + (size_t)seq * p.max_pages;
-    int page_at = 0;  // lane i: the page of tile i % 2 of step `page_base` + i / 2
-    int page_base = -16;
-    auto fetch = [&](int i) {  // step i into its slot
-      if (i - page_base >= 16) {
-        page_base = i;
-        const int st = i + lane / 2;
-        page_at = -1;
-        if (st < n_steps) {
-          const int key = key_of(st) + lane % 2 * kKvTile;
+    const uint8_t *src = nullptr;  // lane i: tile i % 2 of step `batch` + i / 2; null: no such
+    unsigned there = 0;            // which lanes' tiles are
+    int batch = -16;
+    auto start = [&](int i) {  // step i into its slot
+      if (i - batch >= 16) {
+        batch = i;
+        src = nullptr;
+        if (i + lane / 2 < n_steps) {
+          const int key = key_of(i + lane / 2) + lane % 2 * kKvTile;
           if (key < end) {
-            page_at = table[key >> p.page_shift];
-            if (page_at < 0 || page_at >= p.n_pages) {
+            const int page = table[key >> p.page_shift];
+            if (page >= 0 && page < p.n_pages)
+              src = head_pages + page * page_stride +
+                    (unsigned)((key & ((1 << p.page_shift) - 1)) / kKvTile) * C::kTile;
+            else
               attn_refuse(p, seq, APX_ERR_INVALID_ARGUMENT);
-              page_at = -1;
-            }
           }
         }
+        there = __ballot_sync(0xFFFFFFFFu, src != nullptr);
       }
-      const int pg = __shfl_sync(0xFFFFFFFFu, page_at, 2 * (i - page_base) + lane % 2);
-      int sl = slot + i;  // i is at most kSlots ahead of the step being read
-      sl %= C::kSlots;
-      const unsigned have = __ballot_sync(0xFFFFFFFFu, pg >= 0) & 3u;
-      if (lane == 0) mbar_expect_tx(bar + sl, (uint32_t)__popc(have) * C::kTile);
-      __syncwarp();
-      if (lane < 2 && pg >= 0) {
-        const int key = key_of(i) + lane * kKvTile;
-        const int tile = (key & ((1 << p.page_shift) - 1)) / kKvTile;
-        bulk_g2s(ring + sl * C::kSlot + lane * C::kTile,
-                 head_pages + (unsigned long long)pg * p.kv_heads * p.page_bytes +
-                     (unsigned)tile * C::kTile,
-                 C::kTile, bar + sl);
-      }
-      return have;
-    };
-    // which tiles of the slots in flight were copied at all (2 bits each, by step modulo slots)
-    unsigned present = 0;
-    auto start = [&](int i) {
-      const unsigned have = fetch(i);
-      const int sl = (slot + i) % C::kSlots;
-      present = (present & ~(3u << (2 * sl))) | have << (2 * sl);
+      const int sl = (slot + i) & (C::kSlots - 1), owner = 2 * (i - batch);
+      if (lane == owner)
+        mbar_expect_tx(bar + sl, (uint32_t)__popc(there >> owner & 3u) * C::kTile);
+      if ((lane & ~1) == owner && src != nullptr)
+        bulk_g2s(ring + sl * C::kSlot + (lane & 1) * C::kTile, src, C::kTile, bar + sl);
     };
     for (int i = 0; i < min(n_steps, C::kSlots); i++) start(i);
 
@@ -376,12 +365,24 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
     }
 
     for (int i = 0; i < n_steps; i++) {
-      const int sl = (slot + i) % C::kSlots;
-      alive = alive && mbar_wait(bar + sl, phase >> sl & 1);
+      const int sl = (slot + i) & (C::kSlots - 1);
+      if (!mbar_try(bar + sl, phase >> sl & 1))
+        alive = alive && mbar_wait_more(bar + sl, phase >> sl & 1);
       phase ^= 1u << sl;
-      const uint8_t *tile = ring + sl * C::kSlot;
-      const unsigned here = present >> (2 * sl) & 3u;
+      uint8_t *tile = ring + sl * C::kSlot;
       const int key = key_of(i);
+      if (key + kStepKeys > end) {
+        // tokens past the last key may hold anything: V's scales there count as zero (K's are
+        // masked)
+        __syncwarp();
+        if (key + lane >= end)
+#pragma unroll
+          for (int g = 0; g < D / kKvGroup; g++)
+            *reinterpret_cast<uint16_t *>(tile + lane / kKvTile * C::kTile + kv4_vs_off(D) +
+                                          (g * kKvTile + lane % kKvTile) * 2) = 0;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the slot's next copy
+        __syncwarp();
+      }
 
       // scores of 32 keys, S^T = K Q^T: rows gid and gid + 8 of two tiles
       float s[2][NT][4];
@@ -417,16 +418,14 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
 #pragma unroll
           for (int t = 0; t < 2; t++) {
             const uint32_t x = kw[t][0][w], y = kw[t][1][w];
-            const uint32_t a[4] = {low2(x, ks[t][0]), low2(y, ks[t][1]), high2(x, ks[t][0]),
-                                   high2(y, ks[t][1])};
-            const uint32_t b[4] = {low2(x >> 8, ks[t][0]), low2(y >> 8, ks[t][1]),
-                                   high2(x >> 8, ks[t][0]), high2(y >> 8, ks[t][1])};
+            const uint32_t a[4] = {un.low2(x, ks[t][0]), un.low2(y, ks[t][1]), un.high2(x, ks[t][0]),
+                                   un.high2(y, ks[t][1])};
+            const uint32_t b[4] = {un.low2(x >> 8, ks[t][0]), un.low2(y >> 8, ks[t][1]),
+                                   un.high2(x >> 8, ks[t][0]), un.high2(y >> 8, ks[t][1])};
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-              // two chains: for 16-bit queries the odd steps', for f32 the low halves'
               mma_f16(s[t][n], a, qh[n][2 * w][0], qh[n][2 * w][1]);
-              mma_f16(SPLIT == 2 ? s[t][n] : lo[t][n], b, qh[n][2 * w + 1][0],
-                      qh[n][2 * w + 1][1]);
+              mma_f16(s[t][n], b, qh[n][2 * w + 1][0], qh[n][2 * w + 1][1]);
               if (SPLIT == 2) {
                 mma_f16(lo[t][n], a, ql[SPLIT == 2 ? n : 0][2 * w][0],
                         ql[SPLIT == 2 ? n : 0][2 * w][1]);
@@ -440,11 +439,11 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
 #pragma unroll
           for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) s[t][n][j] = (s[t][n][j] + lo[t][n][j]) * cq[n][j & 1];
+            for (int j = 0; j < 4; j++)
+              s[t][n][j] = (SPLIT == 2 ? s[t][n][j] + lo[t][n][j] : s[t][n][j]) * cq[n][j & 1];
       }
       // masks, where some row does not see all 32 keys
-      if (key + kStepKeys - 1 > all_hi || (key < all_lo && key + kStepKeys > p.sinks) ||
-          here != 3u) {
+      if (key + kStepKeys - 1 > all_hi || (key < all_lo && key + kStepKeys > p.sinks)) {
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -452,23 +451,20 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
 #pragma unroll
             for (int j = 0; j < 4; j++) {
               const int k = key + kKvTile * t + gid + 8 * (j / 2);
-              const bool seen = (here >> t & 1) && k <= vis_hi[n][j & 1] &&
-                                (k >= vis_lo[n][j & 1] || k < p.sinks);
+              const bool seen =
+                  k <= vis_hi[n][j & 1] && (k >= vis_lo[n][j & 1] || k < p.sinks);
               if (!seen) s[t][n][j] = -INFINITY;
             }
       }
-      // the running maximum; the sums and outputs turn only when it grows
+      // the sums and outputs turn only when some score has outgrown its maximum
       bool grew = false;
-      float mn[NT][2];
+      float top[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-          float x = fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2]));
-#pragma unroll
-          for (int sh = 4; sh < 32; sh <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, sh));
-          mn[n][j] = fmaxf(m[n][j], x);
-          grew |= mn[n][j] > m[n][j];
+          top[n][j] = fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2]));
+          grew |= top[n][j] > m[n][j] + kStale;
         }
       if (__any_sync(0xFFFFFFFFu, grew)) {
 #pragma unroll
@@ -476,9 +472,13 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
           float f[2];
 #pragma unroll
           for (int j = 0; j < 2; j++) {
-            f[j] = m[n][j] == -INFINITY ? 0.0f : ex2(m[n][j] - mn[n][j]);
+#pragma unroll
+            for (int sh = 4; sh < 32; sh <<= 1)
+              top[n][j] = fmaxf(top[n][j], __shfl_xor_sync(0xFFFFFFFFu, top[n][j], sh));
+            const float mn = fmaxf(m[n][j], top[n][j]);
+            f[j] = m[n][j] == -INFINITY ? 0.0f : ex2(m[n][j] - mn);
             l[n][j] *= f[j];
-            m[n][j] = mn[n][j];
+            m[n][j] = mn;
           }
 #pragma unroll
           for (int d = 0; d < D / 16; d++)
@@ -514,8 +514,6 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
           }
         }
       }
-      // tokens past the last key may hold anything: their scales count as zero
-      const bool tail = key + kStepKeys > end || here != 3u;
 #pragma unroll
       for (int mq = 0; mq < D / 64; mq++) {
         uint32_t vw[2][4];
@@ -528,17 +526,10 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
 #pragma unroll
           for (int g = 0; g < 2; g++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-              uint32_t w = *reinterpret_cast<const uint32_t *>(
+            for (int h = 0; h < 2; h++)
+              vs[t][g][h] = *reinterpret_cast<const uint32_t *>(
                   tile + t * C::kTile + kv4_vs_off(D) +
                   ((2 * mq + g) * kKvTile + 8 * h + 2 * tig) * 2);
-              if (tail) {
-                const int k = key + kKvTile * t + 8 * h + 2 * tig;
-                if (!(here >> t & 1) || k >= end) w &= 0xFFFF0000u;
-                if (!(here >> t & 1) || k + 1 >= end) w &= 0x0000FFFFu;
-              }
-              vs[t][g][h] = w;
-            }
         }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -548,10 +539,10 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
           for (int t = 0; t < 2; t++) {
             const uint32_t x = vw[t][j];
             const __half2 s0 = u2h(vs[t][j / 2][0]), s1 = u2h(vs[t][j / 2][1]);
-            a[t][0] = low2(x, s0);
-            a[t][1] = high2(x, s0);
-            a[t][2] = low2(x >> 8, s1);
-            a[t][3] = high2(x >> 8, s1);
+            a[t][0] = un.low2(x, s0);
+            a[t][1] = un.high2(x, s0);
+            a[t][2] = un.low2(x >> 8, s1);
+            a[t][3] = un.high2(x >> 8, s1);
           }
 #pragma unroll
           for (int n = 0; n < NT; n++) {
@@ -574,7 +565,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
       __syncwarp();  // every lane has read the slot
       if (i + C::kSlots < n_steps) start(i + C::kSlots);
     }
-    slot = (slot + n_steps) % C::kSlots;
+    slot = (slot + n_steps) & (C::kSlots - 1);
 
     // ---- the item's rows of this warp ----
 #pragma unroll

@@ -277,6 +277,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_tc_kernel(AttnArgs p) {
     // and + 8 (four i) with all 16 tokens ----
     const int t = tid - 128, tile = t / kKvTile, g = t % 8, mq = t / 8 % 2;
     const bool has_v = D == 128 || mq == 0;
+    const Unpack un;
     constexpr int K16 = D / 32;  // 16-byte loads of a token's K
     uint4 kraw[K16], vraw[4], vsc[4];
     __half ksc[D / 32];
@@ -334,8 +335,8 @@ __global__ void __launch_bounds__(kThreads, 2) attn_tc_kernel(AttnArgs p) {
             const int chunk = 4 * i + c;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (have)
-              v = make_uint4(low2(w[c], sc), high2(w[c], sc), low2(w[c] >> 8, sc),
-                             high2(w[c] >> 8, sc));
+              v = make_uint4(un.low2(w[c], sc), un.high2(w[c], sc), un.low2(w[c] >> 8, sc),
+                             un.high2(w[c] >> 8, sc));
             *reinterpret_cast<uint4 *>(smem + L::kK + chunk / 8 * (kKeys * 128) +
                                        swizzled(t, chunk % 8)) = v;
           }
@@ -359,10 +360,10 @@ __global__ void __launch_bounds__(kThreads, 2) attn_tc_kernel(AttnArgs p) {
             const uint4 lo4 = vsc[i / 2 * 2], hi4 = vsc[i / 2 * 2 + 1];
             const uint32_t s0 = k == 0 ? lo4.x : k == 1 ? lo4.y : k == 2 ? lo4.z : lo4.w;
             const uint32_t s1 = k == 0 ? hi4.x : k == 1 ? hi4.y : k == 2 ? hi4.z : hi4.w;
-            a[0][k] = low2(w, u2h(s0));
-            a[1][k] = high2(w, u2h(s0));
-            a[0][4 + k] = low2(w >> 8, u2h(s1));
-            a[1][4 + k] = high2(w >> 8, u2h(s1));
+            a[0][k] = un.low2(w, u2h(s0));
+            a[1][k] = un.high2(w, u2h(s0));
+            a[0][4 + k] = un.low2(w >> 8, u2h(s1));
+            a[1][4 + k] = un.high2(w >> 8, u2h(s1));
           }
           if (!have || first + kKvTile > end) {  // tokens past the last key may hold anything
 #pragma unroll

@@ -200,6 +200,21 @@ __device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity) {
   return done != 0;
 }
 
+// The rest of mbar_wait, after a first poll, out of line.
+static __device__ __noinline__ bool mbar_wait_more(uint64_t *bar, uint32_t parity) {
+  unsigned long long t0;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  for (int it = 0; it < kWaitLimit; it++) {
+    if (mbar_try(bar, parity)) return true;
+    if ((it & 63) == 63) {
+      unsigned long long now;
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+      if (now - t0 > 1000000000ull) return false;
+    }
+  }
+  return false;
+}
+
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
   if (mbar_try(bar, parity)) return true;
   unsigned long long t0;

@@ -52,23 +52,35 @@ struct AttnArgs {
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
 __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
 
-// Two codes of x (bits 0-3 and 16-19, or 4-7 and 20-23) as (c - 8) * s: the bits behind 0x6400
-// read 1024 + c, or 1024 + 16 c.
-__device__ __forceinline__ uint32_t low2(uint32_t x, __half2 s) {
-  const __half2 v = u2h((x & 0x000F000Fu) | 0x64006400u);
-  return h2u(__hmul2(__hsub2(v, u2h(0x64086408u)), s));
-}
-__device__ __forceinline__ uint32_t high2(uint32_t x, __half2 s) {
-  const __half2 v = u2h((x & 0x00F000F0u) | 0x64006400u);
-  return h2u(__hmul2(__hfma2(v, u2h(0x2C002C00u), u2h(0xD480D480u)), s));
-}
+// The constants of the unpacking, held in registers: what the compiler does not see through it
+// does not build again at every use.
+struct Unpack {
+  uint32_t magic, sixteenth, minus72;
+  __device__ __forceinline__ Unpack() {
+    asm volatile("mov.u32 %0, 0x64006400;" : "=r"(magic));
+    asm volatile("mov.u32 %0, 0x2C002C00;" : "=r"(sixteenth));
+    asm volatile("mov.u32 %0, 0xD480D480;" : "=r"(minus72));
+  }
+  // Two codes of x (bits 0-3 and 16-19, or 4-7 and 20-23) as (c - 8) * s: the bits behind 0x6400
+  // read 1024 + c, or 1024 + 16 c.
+  __device__ __forceinline__ uint32_t low2(uint32_t x, __half2 s) const {
+    uint32_t v;
+    asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(v) : "r"(x), "r"(magic));
+    return h2u(__hmul2(__hsub2(u2h(v), u2h(0x64086408u)), s));
+  }
+  __device__ __forceinline__ uint32_t high2(uint32_t x, __half2 s) const {
+    uint32_t v;
+    asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(v) : "r"(x), "r"(magic));
+    return h2u(__hmul2(__hfma2(u2h(v), u2h(sixteenth), u2h(minus72)), s));
+  }
+};
 
 __device__ __forceinline__ void attn_refuse(const AttnArgs &p, int seq, int code) {
   if (p.status)
