@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
   __shared__ __align__(8) uint64_t s_bar[W * C::kSlots];
   __shared__ Edge s_edge[W][2];
   __shared__ int s_last[2];
+  __shared__ float s_f[W * R], s_l[W * R], s_top[R];
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, gid = lane / 4, tig = lane % 4;
   pdl_launch_dependents();
@@ -176,11 +177,15 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
     __syncthreads();
   }
   const unsigned long long total = s_pre[C::kThreads - 1];
-  // at least warps_min steps for a warp that works at all
-  unsigned long long nwarps = (unsigned long long)gridDim.x * W;
-  if (total < nwarps * p.warps_min) nwarps = max((total + p.warps_min - 1) / p.warps_min, 1ull);
-  const unsigned long long gw = (unsigned long long)blockIdx.x * W + warp;
-  auto bound = [&](unsigned long long w) { return min(w, nwarps) * total / nwarps; };
+  // At least warps_min steps for a warp that works at all; the first `rem` warps take one more.
+  unsigned nwarps = gridDim.x * W;
+  if (total < (unsigned long long)nwarps * p.warps_min)
+    nwarps = max((unsigned)(total + p.warps_min - 1) / p.warps_min, 1u);
+  const bool small = total <= 0xFFFFFFFFull;
+  const unsigned long long base = small ? (unsigned)total / nwarps : total / nwarps;
+  const unsigned rem = (unsigned)(total - base * nwarps);
+  auto bound = [&](unsigned w) { return min(w, nwarps) * base + min(w, rem); };
+  const unsigned gw = blockIdx.x * W + warp;
   const unsigned long long u0 = bound(gw), u1 = bound(gw + 1);
 
   const Unpack un;
@@ -216,9 +221,10 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
     }
     // the item: KV head, pair of blocks, block
     const unsigned long long in_seq = u - seq0;
-    const int pr = (int)(in_seq / q.pair % q.pairs());
-    const int head = (int)(in_seq / q.pair / q.pairs());
-    const unsigned long long pair0 = u - in_seq % q.pair;
+    const bool fits = in_seq <= 0xFFFFFFFFull;
+    const unsigned nth = fits ? (unsigned)in_seq / (unsigned)q.pair : (unsigned)(in_seq / q.pair);
+    const int head = (int)(nth / (unsigned)q.pairs()), pr = (int)(nth - head * q.pairs());
+    const unsigned long long pair0 = seq0 + (unsigned long long)nth * q.pair;
     int blk = pr;
     unsigned long long i0 = pair0, i1 = pair0 + q.steps(p, pr);
     if (u >= i1) {
@@ -619,8 +625,8 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
 
   // ---- the join: items that cross warps, then items that cross CTAs ----
   __syncthreads();
-  const unsigned long long c0 = bound((unsigned long long)blockIdx.x * W);
-  const unsigned long long c1 = bound((unsigned long long)(blockIdx.x + 1) * W);
+  const unsigned long long c0 = bound(blockIdx.x * W), c1 = bound((blockIdx.x + 1) * W);
+  constexpr int E = R * D / 4;  // quads of an item's rows
   auto part_of = [&](int w, int e) {
     return reinterpret_cast<const float *>(smem + w * C::kWarpSmem + (e ? 0 : C::kRing));
   };
@@ -646,94 +652,150 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
       *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) = w;
     }
   };
-  bool out_of_cta[2] = {false, false};
-  Edge edge[2];
-  for (int w = 0; w < W; w++)
-    for (int e = w == 0 ? 0 : 1; e < 2; e++) {  // the first part of each item in this CTA
-      if (!s_edge[w][e].used) continue;
-      const Edge ed = s_edge[w][e];
-      int last = w;
-      while (last + 1 < W && s_edge[last + 1][0].used && s_edge[last + 1][0].begin == ed.begin)
-        last++;
-      const bool whole = ed.begin >= c0 && ed.end <= c1;
-      const int at = ed.begin >= c0 ? 1 : 0;
-      float *dst = p.part + ((size_t)blockIdx.x * 2 + at) * C::kPart;
-      if (!whole) {
-        out_of_cta[at] = true;
-        edge[at] = ed;
-      }
-      for (int i = tid; i < R * D / 4; i += C::kThreads) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float top = -INFINITY;
-        for (int k = w; k <= last; k++) top = fmaxf(top, part_of(k, k == w ? e : 0)[R * D + r]);
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float sum = 0.0f;
-        for (int k = w; k <= last; k++) {
-          const float *src = part_of(k, k == w ? e : 0);
-          const float mk = src[R * D + r], f = mk == -INFINITY ? 0.0f : ex2(mk - top);
-          const float4 x = *reinterpret_cast<const float4 *>(src + r * D + d);
-          sum = fmaf(f, src[R * D + R + r], sum);
-          v = make_float4(fmaf(f, x.x, v.x), fmaf(f, x.y, v.y), fmaf(f, x.z, v.z),
-                          fmaf(f, x.w, v.w));
-        }
-        if (whole) {
-          write4(ed, r, d, v, sum);
-        } else {
-          *reinterpret_cast<float4 *>(dst + r * D + d) = v;
-          if (d == 0) {
-            dst[R * D + r] = top;
-            dst[R * D + R + r] = sum;
-          }
-        }
-      }
-    }
-  // an item's CTAs: the first holds it in its second part, the others in their first
-  auto cta_of = [&](unsigned long long step) {
-    return (int)(((step + 1) * nwarps - 1) / total / W);
+  auto add4 = [](float4 &v, float f, const float4 x) {
+    v = make_float4(fmaf(f, x.x, v.x), fmaf(f, x.y, v.y), fmaf(f, x.z, v.z), fmaf(f, x.w, v.w));
   };
-  if (out_of_cta[0] || out_of_cta[1]) {  // the same in every thread
-    fence_acq_rel_gpu();
-    __syncthreads();
-    if (tid < 2) {
-      s_last[tid] = 0;
-      const bool mine = tid ? out_of_cta[1] : out_of_cta[0];
-      if (mine) {
-        const Edge &ed = tid ? edge[1] : edge[0];
-        const int a = cta_of(ed.begin), n = cta_of(ed.end - 1) - a + 1;
-        if (atomicAdd(p.count + a, 1u) == (unsigned)n - 1) {
-          s_last[tid] = n;
-          p.count[a] = 0;  // for the next call
-        }
-        fence_acq_rel_gpu();
-      }
+  // the edges of the warps, one a lane (the same in every warp)
+  const bool lane_used = lane < W && s_edge[lane % W][0].used;
+  const unsigned long long lane_begin = s_edge[lane % W][0].begin;
+  // the first part of each item in this CTA: the one that began before it, and the last items of
+  // its warps
+  unsigned starts = __ballot_sync(0xFFFFFFFFu, lane < W && s_edge[lane % W][1].used);
+  bool from_before = __shfl_sync(0xFFFFFFFFu, (int)lane_used, 0);
+  int out_of_cta = 0;  // bit 0: the item that began before this CTA; bit 1: its last item
+  Edge edge0, edge1;
+  while (from_before || starts) {
+    const int w = from_before ? 0 : __ffs(starts) - 1, e = from_before ? 0 : 1;
+    if (!from_before) starts &= starts - 1;
+    from_before = false;
+    const Edge ed = s_edge[w][e];
+    // its parts: this one and the first edges of the warps that follow
+    const unsigned same =
+        __ballot_sync(0xFFFFFFFFu, lane_used && lane > w && lane_begin == ed.begin);
+    const int n = __popc(same) + 1;
+    for (int i = tid; i < n * R; i += C::kThreads) {
+      const int k = i / R, r = i % R;
+      float top = -INFINITY;
+#pragma unroll 4
+      for (int j = 0; j < n; j++) top = fmaxf(top, part_of(w + j, j ? 0 : e)[R * D + r]);
+      const float *src = part_of(w + k, k ? 0 : e);
+      const float m = src[R * D + r], f = m == -INFINITY ? 0.0f : ex2(m - top);
+      s_f[k * R + r] = f;
+      s_l[k * R + r] = f * src[R * D + R + r];
+      if (k == 0) s_top[r] = top;
     }
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      const int n = s_last[e];
-      if (!n) continue;
-      const Edge ed = edge[e];
-      const int a = cta_of(ed.begin);
-      for (int i = tid; i < R * D / 4; i += C::kThreads) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        auto src_of = [&](int k) {
-          return p.part + ((size_t)(a + k) * 2 + (k == 0 ? 1 : 0)) * C::kPart;
-        };
-        float top = -INFINITY;
-        for (int k = 0; k < n; k++) top = fmaxf(top, __ldcg(src_of(k) + R * D + r));
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float sum = 0.0f;
-        for (int k = 0; k < n; k++) {
-          const float *src = src_of(k);
-          const float mk = __ldcg(src + R * D + r), f = mk == -INFINITY ? 0.0f : ex2(mk - top);
-          const float4 x = __ldcg(reinterpret_cast<const float4 *>(src + r * D + d));
-          sum = fmaf(f, __ldcg(src + R * D + R + r), sum);
-          v = make_float4(fmaf(f, x.x, v.x), fmaf(f, x.y, v.y), fmaf(f, x.z, v.z),
-                          fmaf(f, x.w, v.w));
-        }
+    const bool whole = ed.begin >= c0 && ed.end <= c1;
+    const int at = ed.begin >= c0 ? 1 : 0;
+    float *dst = p.part + ((size_t)blockIdx.x * 2 + at) * C::kPart;
+    if (!whole) {
+      out_of_cta |= 1 << at;
+      if (at) edge1 = ed;
+      else edge0 = ed;
+    }
+    for (int i = tid; i < E; i += C::kThreads) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float sum = 0.0f;
+#pragma unroll 4
+      for (int k = 0; k < n; k++) {
+        add4(v, s_f[k * R + r],
+             *reinterpret_cast<const float4 *>(part_of(w + k, k ? 0 : e) + r * D + d));
+        sum += s_l[k * R + r];
+      }
+      if (whole) {
         write4(ed, r, d, v, sum);
+      } else {
+        *reinterpret_cast<float4 *>(dst + r * D + d) = v;
+        if (d == 0) {
+          dst[R * D + r] = s_top[r];
+          dst[R * D + R + r] = sum;
+        }
       }
     }
+    __syncthreads();
+  }
+  if (!out_of_cta) return;  // the same in every thread
+
+  // an item's CTAs: the first holds it as its last item, the others as the one from before
+  auto cta_of = [&](unsigned long long step) {
+    const unsigned long long wide = rem * (base + 1);
+    if (small) {
+      const unsigned s = (unsigned)step, b1 = (unsigned)base + 1;
+      return (int)((step < wide ? s / b1 : rem + (s - (unsigned)wide) / (unsigned)base) / W);
+    }
+    return (int)((step < wide ? step / (base + 1) : rem + (step - wide) / base) / W);
+  };
+  fence_acq_rel_gpu();
+  __syncthreads();
+  if (tid < 2) {
+    int n = 0;
+    if (out_of_cta >> tid & 1) {
+      const unsigned long long begin = tid ? edge1.begin : edge0.begin;
+      const unsigned long long end = tid ? edge1.end : edge0.end;
+      const int a = cta_of(begin), all = cta_of(end - 1) - a + 1;
+      if (atomicAdd(p.count + a, 1u) == (unsigned)all - 1) {
+        n = all;
+        p.count[a] = 0;  // for the next call
+      }
+      fence_acq_rel_gpu();
+    }
+    s_last[tid] = n;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int e = 0; e < 2; e++) {
+    const int n = s_last[e];
+    if (!n) continue;
+    const Edge ed = e ? edge1 : edge0;
+    const int a = cta_of(ed.begin);
+    auto src_of = [&](int k) {
+      return p.part + ((size_t)(a + k) * 2 + (k == 0 ? 1 : 0)) * C::kPart;
+    };
+    // the parts' factors, then their sum by groups of threads, each a share of the parts
+    float *f = reinterpret_cast<float *>(smem), *fl = f + n * R;
+    float4 *red = reinterpret_cast<float4 *>(smem + ((n * R * 8 + 15) & ~15));
+    for (int i = tid; i < n * R; i += C::kThreads) {
+      const float *src = src_of(i / R) + R * D + i % R;
+      f[i] = __ldcg(src);
+      fl[i] = __ldcg(src + R);
+    }
+    __syncthreads();
+    for (int r = warp; r < R; r += W) {
+      float top = -INFINITY, sum = 0.0f;
+      for (int k = lane; k < n; k += 32) top = fmaxf(top, f[k * R + r]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      for (int k = lane; k < n; k += 32) {
+        const float m = f[k * R + r], x = m == -INFINITY ? 0.0f : ex2(m - top);
+        f[k * R + r] = x;
+        sum += x * fl[k * R + r];
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+      if (lane == 0) s_l[r] = sum;
+    }
+    __syncthreads();
+    constexpr int G = C::kThreads >= E ? C::kThreads / E : 1;
+    for (int i = tid; i < E * G; i += C::kThreads) {
+      const int q4 = i % E, r = q4 / (D / 4), d = q4 % (D / 4) * 4;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+      for (int k = i / E; k < n; k += G)
+        add4(v, f[k * R + r], __ldcg(reinterpret_cast<const float4 *>(src_of(k) + r * D + d)));
+      if (G == 1) write4(ed, r, d, v, s_l[r]);
+      else red[i] = v;
+    }
+    if (G > 1) {
+      __syncthreads();
+      for (int i = tid; i < E; i += C::kThreads) {
+        float4 v = red[i];
+#pragma unroll
+        for (int g = 1; g < G; g++) add4(v, 1.0f, red[g * E + i]);
+        write4(ed, i / (D / 4), i % (D / 4) * 4, v, s_l[i / (D / 4)]);
+      }
+    }
+    __syncthreads();
   }
 }
 
