@@ -72,9 +72,10 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t 
   lo = h2u(__floats2half2_rn(x - f.x, y - f.y));
 }
 
-__device__ __forceinline__ void store_out(void *o, unsigned long long i, float v, int type) {
-  if (type == APX_DTYPE_F32) static_cast<float *>(o)[i] = v;
-  else if (type == APX_DTYPE_F16) static_cast<__half *>(o)[i] = __float2half_rn(v);
+template <int TYPE>
+__device__ __forceinline__ void store_out(void *o, unsigned long long i, float v) {
+  if (TYPE == APX_DTYPE_F32) static_cast<float *>(o)[i] = v;
+  else if (TYPE == APX_DTYPE_F16) static_cast<__half *>(o)[i] = __float2half_rn(v);
   else static_cast<__nv_bfloat16 *>(o)[i] = __float2bfloat16_rn(v);
 }
 
@@ -88,7 +89,7 @@ struct SeqShape : SeqRows<R, kStepKeys> {
   __device__ void load(const AttnArgs &p, int s) {
     Base::load(p, s);
     const int n = this->nblk;
-    if (n == 0) pair = 0;
+    if (n <= 0) pair = 0;
     else if (n == 1) pair = steps(p, 0);
     else if (!p.window) pair = steps(p, 0) + steps(p, n - 1) + 2;
     else {
@@ -106,7 +107,7 @@ struct SeqShape : SeqRows<R, kStepKeys> {
   __device__ int pairs() const { return (this->nblk + 1) / 2; }
 };
 
-template <int D, int NT, int SPLIT>
+template <int D, int NT>
 struct Cfg {
   static constexpr int kWarps = NT == 1 ? 16 : 8;
   static constexpr int kThreads = 32 * kWarps;
@@ -125,17 +126,71 @@ struct Cfg {
 
 // One item that crosses a warp's boundary, kept for the join at the end of the CTA.
 struct Edge {
-  unsigned long long begin, end;  // the item's steps, numbered over the whole call
-  int first, rows, head, used;    // its sequence's first token and rows, its first row and head
-  int row0, pad;
+  unsigned begin, end;          // the item's steps, numbered over the whole call
+  int first, rows, head, row0;  // its sequence's first token and rows, its KV head and first row
+  int used;
 };
 
-template <int D, int NT, int SPLIT>
-__global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_kernel(AttnArgs p) {
-  using C = Cfg<D, NT, SPLIT>;
+// One item: the steps [i0, i1) of a block of query rows of a KV head.  `real` is false for a pair's
+// filling, steps without keys.
+struct Item {
+  unsigned i0, i1;
+  int seq, first, rows, p0;  // of its sequence: first query token, rows, position of row 0
+  int head, row0;            // its KV head and first row
+  int end, sink, from;       // its keys (SeqRows::range)
+  bool real;
+  __device__ __forceinline__ int key_of(unsigned step) const {
+    const int st = (int)(step - i0);
+    return (st < sink ? st : st - sink + from) * kStepKeys;
+  }
+};
+
+// The item of step g.  pre: the steps of the call up to the end of each thread's `per` sequences.
+template <int R, int THREADS>
+__device__ __noinline__ Item find_item(const AttnArgs &p, const unsigned *pre, int per, unsigned g) {
+  int lo = 0, hi = THREADS - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (pre[mid] > g) hi = mid;
+    else lo = mid + 1;
+  }
+  unsigned seq0, seq1 = lo ? pre[lo - 1] : 0;
+  SeqShape<R> q;
+  Item it;
+  it.seq = lo * per - 1;
+  do {
+    seq0 = seq1;
+    q.load(p, ++it.seq);
+    seq1 = seq0 + (unsigned)q.pairs() * q.pair * p.kv_heads;
+  } while (g >= seq1);
+  const unsigned nth = (g - seq0) / (unsigned)q.pair, n = q.pairs();
+  it.head = (int)(nth / n);
+  int blk = (int)(nth - it.head * n);
+  it.i0 = seq0 + nth * q.pair;
+  const unsigned end = it.i0 + q.pair;
+  it.i1 = it.i0 + q.steps(p, blk);
+  if (g >= it.i1 && blk != q.nblk - 1 - blk) {
+    blk = q.nblk - 1 - blk;
+    it.i0 = it.i1;
+    it.i1 = it.i0 + q.steps(p, blk);
+  }
+  it.real = g < it.i1;
+  if (!it.real) it.i1 = end;
+  it.first = q.first;
+  it.rows = q.rows;
+  it.p0 = q.p0;
+  it.row0 = blk * R;
+  q.range(p, blk, it.end, it.sink, it.from);
+  return it;
+}
+
+template <int D, int NT, int TYPE>
+__global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(const __grid_constant__ AttnArgs p) {
+  using C = Cfg<D, NT>;
+  constexpr int SPLIT = TYPE == APX_DTYPE_F32 ? 2 : 1;
   constexpr int W = C::kWarps, R = C::kRows, K4 = D / 32;  // words of K per thread and row
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ unsigned long long s_pre[C::kThreads];
+  __shared__ unsigned s_pre[C::kThreads];
   __shared__ unsigned long long s_warp[W];
   __shared__ __align__(8) uint64_t s_bar[W * C::kSlots];
   __shared__ Edge s_edge[W][2];
@@ -153,17 +208,18 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
 
   // ---- the call's steps, summed over the sequences before each thread's share of them ----
   const int per = (p.n_seqs + C::kThreads - 1) / C::kThreads;
+  unsigned total;
   {
-    unsigned long long mine = 0;
+    unsigned long long run = 0;
+#pragma unroll 1
     for (int i = 0; i < per; i++) {
       const int s = tid * per + i;
       if (s >= p.n_seqs) break;
       SeqShape<R> q;
       q.load(p, s);
       if (q.bad && blockIdx.x == 0) attn_refuse(p, s, APX_ERR_INVALID_ARGUMENT);
-      mine += (unsigned long long)q.pairs() * q.pair * p.kv_heads;
+      run += (unsigned long long)q.pairs() * q.pair * p.kv_heads;
     }
-    unsigned long long run = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned long long u = __shfl_up_sync(0xFFFFFFFFu, run, o);
@@ -171,156 +227,125 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
     }
     if (lane == 31) s_warp[warp] = run;
     __syncthreads();
-    unsigned long long base = 0;
-    for (int i = 0; i < warp; i++) base += s_warp[i];
-    s_pre[tid] = base + run;  // inclusive
+    unsigned long long before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+      all += s_warp[i];
+      if (i < warp) before += s_warp[i];
+    }
+    s_pre[tid] = (unsigned)(before + run);  // inclusive
+    if (all >> 32) {  // 2^37 keys: past any cache
+      if (tid == 0) attn_refuse(p, 0, APX_ERR_TOO_LARGE);
+      return;
+    }
+    total = (unsigned)all;
     __syncthreads();
   }
-  const unsigned long long total = s_pre[C::kThreads - 1];
   // At least warps_min steps for a warp that works at all; the first `rem` warps take one more.
   unsigned nwarps = gridDim.x * W;
-  if (total < (unsigned long long)nwarps * p.warps_min)
-    nwarps = max((unsigned)(total + p.warps_min - 1) / p.warps_min, 1u);
-  const bool small = total <= 0xFFFFFFFFull;
-  const unsigned long long base = small ? (unsigned)total / nwarps : total / nwarps;
-  const unsigned rem = (unsigned)(total - base * nwarps);
+  if (total / (unsigned)p.warps_min < nwarps)
+    nwarps = max((total + p.warps_min - 1) / (unsigned)p.warps_min, 1u);
+  const unsigned base = total / nwarps, rem = total - base * nwarps;
   auto bound = [&](unsigned w) { return min(w, nwarps) * base + min(w, rem); };
-  const unsigned gw = blockIdx.x * W + warp;
-  const unsigned long long u0 = bound(gw), u1 = bound(gw + 1);
+  const unsigned u0 = bound(blockIdx.x * W + warp), u1 = bound(blockIdx.x * W + warp + 1);
 
-  const Unpack un;
-  uint32_t phase = 0;  // bit i: the parity that slot i's next wait takes
-  int slot = 0;
-  bool alive = true;   // no wait has given up
+  // ---- copies: step u0 + i into slot i of the ring, through every item of this warp ----
+  const uint8_t *src = nullptr;  // lane i: tile i % 2 of step u0 + batch + i / 2; null: no such
+  unsigned there = 0;            // which lanes' tiles are
+  int batch = -16;
+  auto look_ahead = [&](int i) {
+    batch = i;
+    src = nullptr;
+    const unsigned g = u0 + i + lane / 2;
+    if (g < u1) {
+      const Item it = find_item<R, C::kThreads>(p, s_pre, per, g);
+      const int key = it.key_of(g) + lane % 2 * kKvTile;
+      if (it.real && key < it.end) {
+        const int page = p.table[(size_t)it.seq * p.max_pages + (key >> p.page_shift)];
+        if (page >= 0 && page < p.n_pages)
+          src = p.pages + ((unsigned long long)page * p.kv_heads + it.head) * p.page_bytes +
+                (unsigned)((key & ((1 << p.page_shift) - 1)) / kKvTile) * C::kTile;
+        else
+          attn_refuse(p, it.seq, APX_ERR_INVALID_ARGUMENT);
+      }
+    }
+    there = __ballot_sync(0xFFFFFFFFu, src != nullptr);
+  };
+  auto start = [&](int i) {  // i < batch + 16
+    const int sl = i & (C::kSlots - 1), owner = 2 * (i - batch);
+    if (lane == owner)
+      mbar_expect_tx(bar + sl, (uint32_t)__popc(there >> owner & 3u) * C::kTile);
+    if ((lane & ~1) == owner && src != nullptr)
+      bulk_g2s(ring + sl * C::kSlot + (lane & 1) * C::kTile, src, C::kTile, bar + sl);
+  };
+  const int mine = (int)(u1 - u0);  // steps of this warp
+  int at = 0;                       // of them, done
+  bool alive = true;                // no wait has given up
+  auto arrived = [&](int i) {
+    const int sl = i & (C::kSlots - 1);
+    const unsigned parity = (unsigned)i / C::kSlots & 1;
+    if (!mbar_try(bar + sl, parity)) alive = alive && mbar_wait_more(bar + sl, parity);
+  };
 
   // ---- this warp's steps, item by item ----
-  unsigned long long u = u0;
-  SeqShape<R> q;
-  int seq = -1;
-  unsigned long long seq0 = 0, seq1 = 0;  // the sequence's steps
-  while (u < u1 && alive) {
-    if (u >= seq1) {  // the sequence that holds u
-      int lo = 0, hi = C::kThreads - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (s_pre[mid] > u) hi = mid;
-        else lo = mid + 1;
+  const Unpack un;
+#pragma unroll 1
+  while (at < mine && alive) {
+    const Item it = find_item<R, C::kThreads>(p, s_pre, per, u0 + at);
+    const int stop = (int)(min(it.i1, u1) - u0);
+    // the block's query rows, asked for before the first copies
+    constexpr int QV = SPLIT == 2 ? D / 16 : D / 32;  // 16-byte loads a row and thread
+    uint4 qraw[NT][QV];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      const int r = it.row0 + 8 * n + gid;
+#pragma unroll
+      for (int i = 0; i < QV; i++) qraw[n][i] = make_uint4(0, 0, 0, 0);
+      if (it.real && r < it.rows) {
+        const int tok = by_group(p, r);
+        const unsigned long long e =
+            (unsigned long long)(it.first + tok) * p.ldq +
+            (unsigned long long)(it.head * p.group + r - tok * p.group) * D + tig * (D / 4);
+        const uint4 *src4 = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(p.q) +
+                                                            e * (SPLIT == 2 ? 4 : 2));
+#pragma unroll
+        for (int i = 0; i < QV; i++) qraw[n][i] = src4[i];
       }
-      unsigned long long at = lo ? s_pre[lo - 1] : 0;
-      for (int i = 0; i < per; i++) {
-        seq = lo * per + i;
-        q.load(p, seq);
-        const unsigned long long n = (unsigned long long)q.pairs() * q.pair * p.kv_heads;
-        if (u < at + n) {
-          seq0 = at;
-          seq1 = at + n;
-          break;
-        }
-        at += n;
-      }
     }
-    // the item: KV head, pair of blocks, block
-    const unsigned long long in_seq = u - seq0;
-    const bool fits = in_seq <= 0xFFFFFFFFull;
-    const unsigned nth = fits ? (unsigned)in_seq / (unsigned)q.pair : (unsigned)(in_seq / q.pair);
-    const int head = (int)(nth / (unsigned)q.pairs()), pr = (int)(nth - head * q.pairs());
-    const unsigned long long pair0 = seq0 + (unsigned long long)nth * q.pair;
-    int blk = pr;
-    unsigned long long i0 = pair0, i1 = pair0 + q.steps(p, pr);
-    if (u >= i1) {
-      blk = q.nblk - 1 - pr;
-      i0 = i1;
-      i1 = blk == pr ? i0 : min(i0 + q.steps(p, blk), pair0 + q.pair);
+    if (at == 0) {
+      look_ahead(0);
+      for (int i = 0; i < min(mine, C::kSlots); i++) start(i);
     }
-    if (u >= i1) {  // the pair's filling
-      u = min(pair0 + q.pair, u1);
-      continue;
-    }
-    const unsigned long long stop = min(i1, u1);
-    int end, sink, from;
-    q.range(p, blk, end, sink, from);
-    const int n_steps = (int)(stop - u), step0 = (int)(u - i0);
+    const int end = it.end;
 
-    // the first key of step i of this warp's share
-    auto key_of = [&](int i) {
-      const int st = step0 + i;
-      return (st < sink ? st : st - sink + from) * kStepKeys;
-    };
-    const uint8_t *head_pages = p.pages + (unsigned long long)head * p.page_bytes;
-    const unsigned long long page_stride = p.kv_heads * p.page_bytes;
-    const int *table = p.table + (size_t)seq * p.max_pages;
-    const uint8_t *src = nullptr;  // lane i: tile i % 2 of step `batch` + i / 2; null: no such
-    unsigned there = 0;            // which lanes' tiles are
-    int batch = -16;
-    auto start = [&](int i) {  // step i into its slot
-      if (i - batch >= 16) {
-        batch = i;
-        src = nullptr;
-        if (i + lane / 2 < n_steps) {
-          const int key = key_of(i + lane / 2) + lane % 2 * kKvTile;
-          if (key < end) {
-            const int page = table[key >> p.page_shift];
-            if (page >= 0 && page < p.n_pages)
-              src = head_pages + page * page_stride +
-                    (unsigned)((key & ((1 << p.page_shift) - 1)) / kKvTile) * C::kTile;
-            else
-              attn_refuse(p, seq, APX_ERR_INVALID_ARGUMENT);
-          }
-        }
-        there = __ballot_sync(0xFFFFFFFFu, src != nullptr);
-      }
-      const int sl = (slot + i) & (C::kSlots - 1), owner = 2 * (i - batch);
-      if (lane == owner)
-        mbar_expect_tx(bar + sl, (uint32_t)__popc(there >> owner & 3u) * C::kTile);
-      if ((lane & ~1) == owner && src != nullptr)
-        bulk_g2s(ring + sl * C::kSlot + (lane & 1) * C::kTile, src, C::kTile, bar + sl);
-    };
-    for (int i = 0; i < min(n_steps, C::kSlots); i++) start(i);
-
-    // ---- the block's query rows as the second operand ----
+    // ---- the rows as the second operand ----
     uint32_t qh[NT][2 * K4][2], ql[SPLIT == 2 ? NT : 1][2 * K4][2];
     float cq[NT][2];  // of columns 2 tig, 2 tig + 1: score units per product unit, times log2 e
     int vis_lo[NT][2], vis_hi[NT][2];
     int all_lo = 0, all_hi = 1 << 30;  // keys that every row of the block sees
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-      const int r = blk * R + 8 * n + gid;
-      float v[2 * K4][4];
-      float top = 0.0f;
       // matrix steps 2 w and 2 w + 1 take dims (0,4),(1,5) and (2,6),(3,7) of word w
+      float v[2 * K4][4];
       auto put = [&v](int i, float x) { v[2 * (i / 8) + i % 4 / 2][2 * (i % 2) + i % 8 / 4] = x; };
 #pragma unroll
-      for (int i = 0; i < D / 4; i++) put(i, 0.0f);
-      if (r < q.rows) {
-        const unsigned long long at = (unsigned long long)(q.first + r / p.group) * p.ldq +
-                                      (unsigned long long)(head * p.group + r % p.group) * D +
-                                      tig * (D / 4);
-        if (SPLIT == 2) {
-          const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + at);
+      for (int i = 0; i < QV; i++) {
+        const uint32_t w[4] = {qraw[n][i].x, qraw[n][i].y, qraw[n][i].z, qraw[n][i].w};
 #pragma unroll
-          for (int i = 0; i < D / 16; i++) {
-            const float4 x = src[i];
-            put(4 * i, x.x), put(4 * i + 1, x.y), put(4 * i + 2, x.z), put(4 * i + 3, x.w);
-          }
-        } else {
-          const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + at);
-#pragma unroll
-          for (int i = 0; i < D / 32; i++) {
-            const uint4 x = src[i];
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-              float2 f;
-              if (p.type == APX_DTYPE_BF16)
-                f = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
-              else
-                f = __half22float2(u2h(w[j]));
-              put(8 * i + 2 * j, f.x);
-              put(8 * i + 2 * j + 1, f.y);
-            }
+        for (int j = 0; j < 4; j++) {
+          if (TYPE == APX_DTYPE_F32) {
+            put(4 * i + j, __uint_as_float(w[j]));
+          } else if (TYPE == APX_DTYPE_BF16) {
+            put(8 * i + 2 * j, __uint_as_float(w[j] << 16));
+            put(8 * i + 2 * j + 1, __uint_as_float(w[j] & 0xFFFF0000u));
+          } else {
+            const float2 f = __half22float2(u2h(w[j]));
+            put(8 * i + 2 * j, f.x);
+            put(8 * i + 2 * j + 1, f.y);
           }
         }
       }
+      float top = 0.0f;
 #pragma unroll
       for (int w = 0; w < 2 * K4; w++)
 #pragma unroll
@@ -333,17 +358,19 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
       for (int w = 0; w < 2 * K4; w++)
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-          uint32_t lo;
-          split2(v[w][2 * j] * up, v[w][2 * j + 1] * up, qh[n][w][j], lo);
-          if (SPLIT == 2) ql[SPLIT == 2 ? n : 0][w][j] = lo;
+          if (SPLIT == 2)
+            split2(v[w][2 * j] * up, v[w][2 * j + 1] * up, qh[n][w][j],
+                   ql[SPLIT == 2 ? n : 0][w][j]);
+          else
+            qh[n][w][j] = h2u(__floats2half2_rn(v[w][2 * j] * up, v[w][2 * j + 1] * up));
         }
       const float c = p.scale * 1.44269504088896341f * pow2(e - 9);
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         cq[n][j] = __shfl_sync(0xFFFFFFFFu, c, (2 * tig + j) * 4);
-        const int col = blk * R + 8 * n + 2 * tig + j;
-        const int pos = q.p0 + col / p.group;
-        const bool live = col < q.rows;
+        const int col = it.row0 + 8 * n + 2 * tig + j;
+        const int pos = it.p0 + by_group(p, col);
+        const bool live = col < it.rows;
         vis_hi[n][j] = live ? min(pos, end - 1) : -1;
         vis_lo[n][j] = p.window ? pos - p.window + 1 : 0;
         if (live) {
@@ -369,14 +396,21 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
       m[n][0] = m[n][1] = -INFINITY;
       l[n][0] = l[n][1] = 0.0f;
     }
+    const bool from_start = u0 + at == it.i0;
 
-    for (int i = 0; i < n_steps; i++) {
-      const int sl = (slot + i) & (C::kSlots - 1);
-      if (!mbar_try(bar + sl, phase >> sl & 1))
-        alive = alive && mbar_wait_more(bar + sl, phase >> sl & 1);
-      phase ^= 1u << sl;
-      uint8_t *tile = ring + sl * C::kSlot;
-      const int key = key_of(i);
+#pragma unroll 1
+    for (; at < stop; at++) {
+      arrived(at);
+      uint8_t *tile = ring + (at & (C::kSlots - 1)) * C::kSlot;
+      if (!it.real) {  // filling: no keys, no copies
+        __syncwarp();
+        if (at + C::kSlots < mine) {
+          if (at + C::kSlots - batch >= 16) look_ahead(at + C::kSlots);
+          start(at + C::kSlots);
+        }
+        continue;
+      }
+      const int key = it.key_of(u0 + at);
       if (key + kStepKeys > end) {
         // tokens past the last key may hold anything: V's scales there count as zero (K's are
         // masked)
@@ -569,9 +603,12 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
         }
       }
       __syncwarp();  // every lane has read the slot
-      if (i + C::kSlots < n_steps) start(i + C::kSlots);
+      if (at + C::kSlots < mine) {
+        if (at + C::kSlots - batch >= 16) look_ahead(at + C::kSlots);
+        start(at + C::kSlots);
+      }
     }
-    slot = (slot + n_steps) & (C::kSlots - 1);
+    if (!it.real) continue;
 
     // ---- the item's rows of this warp ----
 #pragma unroll
@@ -581,26 +618,28 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
 #pragma unroll
         for (int sh = 4; sh < 32; sh <<= 1)
           l[n][j] += __shfl_xor_sync(0xFFFFFFFFu, l[n][j], sh);
-    if (u == i0 && stop == i1) {  // the whole item
+    if (from_start && u0 + at == it.i1) {  // the whole item
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-          const int r = blk * R + 8 * n + 2 * tig + j;
-          if (r >= q.rows) continue;
+          const int r = it.row0 + 8 * n + 2 * tig + j;
+          if (r >= it.rows) continue;
           const float inv = l[n][j] == 0.0f ? 0.0f : 1.0f / l[n][j];
-          const unsigned long long at = (unsigned long long)(q.first + r / p.group) * p.ldo +
-                                        (unsigned long long)(head * p.group + r % p.group) * D;
+          const int tok = by_group(p, r);
+          const unsigned long long to =
+              (unsigned long long)(it.first + tok) * p.ldo +
+              (unsigned long long)(it.head * p.group + r - tok * p.group) * D + gid;
 #pragma unroll
           for (int d = 0; d < D / 16; d++) {
-            store_out(p.out, at + 16 * d + gid, o[n][d][j] * inv, p.type);
-            store_out(p.out, at + 16 * d + gid + 8, o[n][d][j + 2] * inv, p.type);
+            store_out<TYPE>(p.out, to + 16 * d, o[n][d][j] * inv);
+            store_out<TYPE>(p.out, to + 16 * d + 8, o[n][d][j + 2] * inv);
           }
         }
     } else {
       // kept for the join at the end: an item that began before this warp, behind the ring; one
       // that goes on after it (its last), in the ring, whose copies have all arrived
-      const int e = u == i0 ? 1 : 0;
+      const int e = from_start ? 1 : 0;
       float *part = reinterpret_cast<float *>(e ? ring : ring + C::kRing);
 #pragma unroll
       for (int n = 0; n < NT; n++)
@@ -617,15 +656,14 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
             part[R * D + R + r] = l[n][j];
           }
         }
-      if (lane == 0) s_edge[warp][e] = Edge{i0, i1, q.first, q.rows, head, 1, blk * R, 0};
+      if (lane == 0) s_edge[warp][e] = Edge{it.i0, it.i1, it.first, it.rows, it.head, it.row0, 1};
     }
-    u = stop;
   }
   if (!alive && lane == 0) attn_refuse(p, 0, APX_ERR_DEVICE_TIMEOUT);
 
   // ---- the join: items that cross warps, then items that cross CTAs ----
   __syncthreads();
-  const unsigned long long c0 = bound(blockIdx.x * W), c1 = bound((blockIdx.x + 1) * W);
+  const unsigned c0 = bound(blockIdx.x * W), c1 = bound((blockIdx.x + 1) * W);
   constexpr int E = R * D / 4;  // quads of an item's rows
   auto part_of = [&](int w, int e) {
     return reinterpret_cast<const float *>(smem + w * C::kWarpSmem + (e ? 0 : C::kRing));
@@ -634,14 +672,16 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
     const int row = ed.row0 + r;
     if (row >= ed.rows) return;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const unsigned long long at = (unsigned long long)(ed.first + row / p.group) * p.ldo +
-                                  (unsigned long long)(ed.head * p.group + row % p.group) * D + d;
+    const int tok = by_group(p, row);
+    const unsigned long long at =
+        (unsigned long long)(ed.first + tok) * p.ldo +
+        (unsigned long long)(ed.head * p.group + row - tok * p.group) * D + d;
     if (SPLIT == 2) {
       *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) =
           make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
     } else {
       uint2 w;
-      if (p.type == APX_DTYPE_BF16) {
+      if (TYPE == APX_DTYPE_BF16) {
         __nv_bfloat162 x = __floats2bfloat162_rn(v.x * inv, v.y * inv);
         __nv_bfloat162 y = __floats2bfloat162_rn(v.z * inv, v.w * inv);
         w = make_uint2(*reinterpret_cast<uint32_t *>(&x), *reinterpret_cast<uint32_t *>(&y));
@@ -657,7 +697,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
   };
   // the edges of the warps, one a lane (the same in every warp)
   const bool lane_used = lane < W && s_edge[lane % W][0].used;
-  const unsigned long long lane_begin = s_edge[lane % W][0].begin;
+  const unsigned lane_begin = s_edge[lane % W][0].begin;
   // the first part of each item in this CTA: the one that began before it, and the last items of
   // its warps
   unsigned starts = __ballot_sync(0xFFFFFFFFu, lane < W && s_edge[lane % W][1].used);
@@ -718,12 +758,8 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
   if (!out_of_cta) return;  // the same in every thread
 
   // an item's CTAs: the first holds it as its last item, the others as the one from before
-  auto cta_of = [&](unsigned long long step) {
-    const unsigned long long wide = rem * (base + 1);
-    if (small) {
-      const unsigned s = (unsigned)step, b1 = (unsigned)base + 1;
-      return (int)((step < wide ? s / b1 : rem + (s - (unsigned)wide) / (unsigned)base) / W);
-    }
+  auto cta_of = [&](unsigned step) {
+    const unsigned wide = rem * (base + 1);
     return (int)((step < wide ? step / (base + 1) : rem + (step - wide) / base) / W);
   };
   fence_acq_rel_gpu();
@@ -731,8 +767,8 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
   if (tid < 2) {
     int n = 0;
     if (out_of_cta >> tid & 1) {
-      const unsigned long long begin = tid ? edge1.begin : edge0.begin;
-      const unsigned long long end = tid ? edge1.end : edge0.end;
+      const unsigned begin = tid ? edge1.begin : edge0.begin;
+      const unsigned end = tid ? edge1.end : edge0.end;
       const int a = cta_of(begin), all = cta_of(end - 1) - a + 1;
       if (atomicAdd(p.count + a, 1u) == (unsigned)all - 1) {
         n = all;
@@ -780,7 +816,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
     for (int i = tid; i < E * G; i += C::kThreads) {
       const int q4 = i % E, r = q4 / (D / 4), d = q4 % (D / 4) * 4;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
+#pragma unroll 4
       for (int k = i / E; k < n; k += G)
         add4(v, f[k * R + r], __ldcg(reinterpret_cast<const float4 *>(src_of(k) + r * D + d)));
       if (G == 1) write4(ed, r, d, v, s_l[r]);
@@ -799,10 +835,10 @@ __global__ void __launch_bounds__(Cfg<D, NT, SPLIT>::kThreads, 1) attn_split_ker
   }
 }
 
-template <int D, int NT, int SPLIT>
+template <int D, int NT, int TYPE>
 cudaError_t launch_split(const AttnArgs &p, int grid, cudaStream_t stream) {
-  using C = Cfg<D, NT, SPLIT>;
-  auto kern = attn_split_kernel<D, NT, SPLIT>;
+  using C = Cfg<D, NT>;
+  auto kern = attn_split_kernel<D, NT, TYPE>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
@@ -818,12 +854,19 @@ cudaError_t launch_split(const AttnArgs &p, int grid, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
+template <int D, int NT>
+cudaError_t launch_type(const AttnArgs &p, int grid, cudaStream_t stream) {
+  if (p.type == APX_DTYPE_F32) return launch_split<D, NT, APX_DTYPE_F32>(p, grid, stream);
+  if (p.type == APX_DTYPE_F16) return launch_split<D, NT, APX_DTYPE_F16>(p, grid, stream);
+  return launch_split<D, NT, APX_DTYPE_BF16>(p, grid, stream);
+}
+
 }  // namespace
 
 // Two partial items per CTA of the largest block, and the arrival counters before them.
 constexpr int kCountBytes = 4096;
 size_t attn_work_bytes(int sms) {
-  return kCountBytes + (size_t)sms * 2 * Cfg<128, 2, 1>::kPart * sizeof(float);
+  return kCountBytes + (size_t)sms * 2 * Cfg<128, 2>::kPart * sizeof(float);
 }
 
 cudaError_t launch_attn_kv4(const apx_attn_args &a, const apx_kv4_cache &c,
@@ -854,15 +897,13 @@ cudaError_t launch_attn_kv4(const apx_attn_args &a, const apx_kv4_cache &c,
   p.type = a.type;
   p.warps_min = 1;
   p.scale = a.scale;
+  p.group_mul = (unsigned)(0x100000000ull / (unsigned)p.group + 1);
   const int grid = std::min(sms, kCountBytes / 4);
   if (attn_tc_serves(p, c.head_dim, b.max_q)) return launch_attn_tc(p, c.head_dim, b.max_q, stream);
-  const bool one = (size_t)b.max_q * p.group <= 8, f32 = a.type == APX_DTYPE_F32;
-  if (c.head_dim == 128) {
-    if (one) return f32 ? launch_split<128, 1, 2>(p, grid, stream) : launch_split<128, 1, 1>(p, grid, stream);
-    return f32 ? launch_split<128, 2, 2>(p, grid, stream) : launch_split<128, 2, 1>(p, grid, stream);
-  }
-  if (one) return f32 ? launch_split<64, 1, 2>(p, grid, stream) : launch_split<64, 1, 1>(p, grid, stream);
-  return f32 ? launch_split<64, 2, 2>(p, grid, stream) : launch_split<64, 2, 1>(p, grid, stream);
+  const bool one = (size_t)b.max_q * p.group <= 8;
+  if (c.head_dim == 128)
+    return one ? launch_type<128, 1>(p, grid, stream) : launch_type<128, 2>(p, grid, stream);
+  return one ? launch_type<64, 1>(p, grid, stream) : launch_type<64, 2>(p, grid, stream);
 }
 
 }  // namespace apx

@@ -47,6 +47,7 @@ struct AttnArgs {
   unsigned *count;  // apx_attn.cu: CTAs that have arrived at an item (zero between calls)
   int n_pages, n_seqs, max_pages, kv_heads, group, page_shift;
   int window, sinks, type, warps_min, n_tokens;
+  unsigned group_mul;  // 2^32 / group + 1, for by_group
   float scale;
 };
 
@@ -87,6 +88,13 @@ __device__ __forceinline__ void attn_refuse(const AttnArgs &p, int seq, int code
     atomicMin(p.status, (unsigned long long)seq << 24 | (unsigned long long)code << 16);
 }
 
+// r / group for 0 <= r < 2^31: the product's high word is the quotient or one more.
+__device__ __forceinline__ int by_group(const AttnArgs &p, int r) {
+  if (p.group == 1) return r;
+  const unsigned q = __umulhi((unsigned)r, p.group_mul);
+  return (int)(q - (q * (unsigned)p.group > (unsigned)r ? 1u : 0u));
+}
+
 // A power of two that brings a row's largest |q| to [2^9, 2^10) (exponents outside the f32
 // normals are clamped), as its exponent's distance: q 2^(9 - e).
 __device__ __forceinline__ int row_exponent(float top) {
@@ -114,7 +122,7 @@ struct SeqRows {
   __device__ static int steps_to(int n) { return (max(n, 0) + KEYS - 1) / KEYS; }
   // Block b sees keys below `end`: those of the sinks' steps [0, sink) and of steps `from` on.
   __device__ void range(const AttnArgs &p, int b, int &end, int &sink, int &from) const {
-    const int lo = p0 + b * R / p.group, hi = p0 + min((b + 1) * R - 1, rows - 1) / p.group;
+    const int lo = p0 + by_group(p, b * R), hi = p0 + by_group(p, min((b + 1) * R - 1, rows - 1));
     end = max(min(kv, hi + 1), 0);
     sink = from = 0;
     if (p.window) {
