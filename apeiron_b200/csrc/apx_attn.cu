@@ -73,6 +73,21 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t 
 }
 
 template <int TYPE>
+__device__ __forceinline__ void store4(void *o, unsigned long long i, const float4 v) {
+  if (TYPE == APX_DTYPE_F32) {
+    *reinterpret_cast<float4 *>(static_cast<float *>(o) + i) = v;
+  } else {
+    uint2 w;
+    if (TYPE == APX_DTYPE_BF16) {
+      __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
+      w = make_uint2(*reinterpret_cast<uint32_t *>(&x), *reinterpret_cast<uint32_t *>(&y));
+    } else {
+      w = make_uint2(h2u(__floats2half2_rn(v.x, v.y)), h2u(__floats2half2_rn(v.z, v.w)));
+    }
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o) + i) = w;
+  }
+}
+template <int TYPE>
 __device__ __forceinline__ void store_out(void *o, unsigned long long i, float v) {
   if (TYPE == APX_DTYPE_F32) static_cast<float *>(o)[i] = v;
   else if (TYPE == APX_DTYPE_F16) static_cast<__half *>(o)[i] = __float2half_rn(v);
@@ -80,17 +95,17 @@ __device__ __forceinline__ void store_out(void *o, unsigned long long i, float v
 }
 
 // A sequence's steps.  Its blocks of rows pair first with last: a pair has `pair` steps, the
-// first block's, then the second's, then none.
-template <int R>
+// first block's, then the second's, then none.  ONE: every sequence has one block at most.
+template <int R, bool ONE>
 struct SeqShape : SeqRows<R, kStepKeys> {
   using Base = SeqRows<R, kStepKeys>;
   int pair;
 
-  __device__ void load(const AttnArgs &p, int s) {
+  __device__ __forceinline__ void load(const AttnArgs &p, int s) {
     Base::load(p, s);
     const int n = this->nblk;
     if (n <= 0) pair = 0;
-    else if (n == 1) pair = steps(p, 0);
+    else if (ONE || n == 1) pair = steps(p, 0);
     else if (!p.window) pair = steps(p, 0) + steps(p, n - 1) + 2;
     else {
       // a window's keys: what the block's positions span, in whole steps
@@ -99,12 +114,14 @@ struct SeqShape : SeqRows<R, kStepKeys> {
                       Base::steps_to(this->kv)) + 1);
     }
   }
-  __device__ int steps(const AttnArgs &p, int b) const {
+  __device__ __forceinline__ int steps(const AttnArgs &p, int b) const {
     int end, sink, from;
     this->range(p, b, end, sink, from);
     return max(sink + max(Base::steps_to(end) - from, 0), 1);  // one writes unseeing rows' zeros
   }
-  __device__ int pairs() const { return (this->nblk + 1) / 2; }
+  __device__ __forceinline__ int pairs() const {
+    return ONE ? (this->nblk > 0 ? 1 : 0) : (this->nblk + 1) / 2;
+  }
 };
 
 template <int D, int NT>
@@ -121,7 +138,7 @@ struct Cfg {
   static constexpr int kWarpSmem = kRing + kPart * 4;
   static constexpr int kSmem = kWarps * kWarpSmem;
   static_assert(kPart * 4 <= kRing, "a partial item fits the ring");
-  static_assert(kSmem <= 227 * 1024 - 8192, "shared memory");
+  static_assert(kSmem <= 227 * 1024 - 13 * 1024, "shared memory");
 };
 
 // One item that crosses a warp's boundary, kept for the join at the end of the CTA.
@@ -145,31 +162,30 @@ struct Item {
   }
 };
 
-// The item of step g.  pre: the steps of the call up to the end of each thread's `per` sequences.
-template <int R, int THREADS>
+// The item of step g, the same g in every lane.  pre: the steps of the call up to the end of each
+// thread's `per` sequences.
+template <int R, bool ONE, int THREADS>
 __device__ __noinline__ Item find_item(const AttnArgs &p, const unsigned *pre, int per, unsigned g) {
-  int lo = 0, hi = THREADS - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (pre[mid] > g) hi = mid;
-    else lo = mid + 1;
-  }
-  unsigned seq0, seq1 = lo ? pre[lo - 1] : 0;
-  SeqShape<R> q;
+  constexpr int N = THREADS / 32;
+  const int lane = threadIdx.x % 32;
+  int at = __ffs(__ballot_sync(0xFFFFFFFFu, pre[lane * N + N - 1] > g)) - 1;
+  at = at * N + __ffs(__ballot_sync(0xFFFFFFFFu, lane < N && pre[at * N + lane % N] > g)) - 1;
+  unsigned seq0, seq1 = at ? pre[at - 1] : 0;
+  SeqShape<R, ONE> q;
   Item it;
-  it.seq = lo * per - 1;
+  it.seq = at * per - 1;
   do {
     seq0 = seq1;
     q.load(p, ++it.seq);
     seq1 = seq0 + (unsigned)q.pairs() * q.pair * p.kv_heads;
   } while (g >= seq1);
   const unsigned nth = (g - seq0) / (unsigned)q.pair, n = q.pairs();
-  it.head = (int)(nth / n);
-  int blk = (int)(nth - it.head * n);
+  it.head = (int)(ONE ? nth : nth / n);
+  int blk = ONE ? 0 : (int)(nth - it.head * n);
   it.i0 = seq0 + nth * q.pair;
   const unsigned end = it.i0 + q.pair;
-  it.i1 = it.i0 + q.steps(p, blk);
-  if (g >= it.i1 && blk != q.nblk - 1 - blk) {
+  it.i1 = ONE ? end : it.i0 + q.steps(p, blk);
+  if (!ONE && g >= it.i1 && blk != q.nblk - 1 - blk) {
     blk = q.nblk - 1 - blk;
     it.i0 = it.i1;
     it.i1 = it.i0 + q.steps(p, blk);
@@ -189,13 +205,14 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   using C = Cfg<D, NT>;
   constexpr int SPLIT = TYPE == APX_DTYPE_F32 ? 2 : 1;
   constexpr int W = C::kWarps, R = C::kRows, K4 = D / 32;  // words of K per thread and row
+  constexpr bool ONE = NT == 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ unsigned s_pre[C::kThreads];
   __shared__ unsigned long long s_warp[W];
   __shared__ __align__(8) uint64_t s_bar[W * C::kSlots];
   __shared__ Edge s_edge[W][2];
-  __shared__ int s_last[2];
-  __shared__ float s_f[W * R], s_l[W * R], s_top[R];
+  __shared__ int s_last[2], s_most[W];
+  __shared__ float s_f[W][W * R];
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, gid = lane / 4, tig = lane % 4;
   pdl_launch_dependents();
@@ -209,15 +226,18 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   // ---- the call's steps, summed over the sequences before each thread's share of them ----
   const int per = (p.n_seqs + C::kThreads - 1) / C::kThreads;
   unsigned total;
+  int longest = 0;
   {
     unsigned long long run = 0;
+    int most = 0;
 #pragma unroll 1
     for (int i = 0; i < per; i++) {
       const int s = tid * per + i;
       if (s >= p.n_seqs) break;
-      SeqShape<R> q;
+      SeqShape<R, ONE> q;
       q.load(p, s);
       if (q.bad && blockIdx.x == 0) attn_refuse(p, s, APX_ERR_INVALID_ARGUMENT);
+      most = max(most, q.pair);
       run += (unsigned long long)q.pairs() * q.pair * p.kv_heads;
     }
 #pragma unroll
@@ -225,12 +245,14 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
       const unsigned long long u = __shfl_up_sync(0xFFFFFFFFu, run, o);
       if (lane >= o) run += u;
     }
-    if (lane == 31) s_warp[warp] = run;
+    if (ONE) most = __reduce_max_sync(0xFFFFFFFFu, most);
+    if (lane == 31) s_warp[warp] = run, s_most[warp] = most;
     __syncthreads();
     unsigned long long before = 0, all = 0;
 #pragma unroll
     for (int i = 0; i < W; i++) {
       all += s_warp[i];
+      longest = max(longest, s_most[i]);
       if (i < warp) before += s_warp[i];
     }
     s_pre[tid] = (unsigned)(before + run);  // inclusive
@@ -241,33 +263,47 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
     total = (unsigned)all;
     __syncthreads();
   }
-  // At least warps_min steps for a warp that works at all; the first `rem` warps take one more.
-  unsigned nwarps = gridDim.x * W;
-  if (total / (unsigned)p.warps_min < nwarps)
-    nwarps = max((total + p.warps_min - 1) / (unsigned)p.warps_min, 1u);
-  const unsigned base = total / nwarps, rem = total - base * nwarps;
-  auto bound = [&](unsigned w) { return min(w, nwarps) * base + min(w, rem); };
-  const unsigned u0 = bound(blockIdx.x * W + warp), u1 = bound(blockIdx.x * W + warp + 1);
+  // Equal shares for every warp of the grid, the first `rem` one step more.  Or, while there are
+  // CTAs for all items and the longest costs a warp four steps at most: an item per CTA, which
+  // saves the join through the workspace (0.5B shape, 777 keys: 13.5 -> 8.6 us).
+  const int items = ONE ? p.n_seqs * p.kv_heads : 0;
+  const bool whole_items = ONE && items <= (int)gridDim.x && longest <= 4 * W;
+  const unsigned nwarps = whole_items ? W : min(gridDim.x * W, max(total, 1u));
+  unsigned c0 = 0, c1 = total;
+  if (whole_items) {
+    if ((int)blockIdx.x >= items) return;
+    const int s = blockIdx.x / p.kv_heads, h = blockIdx.x - s * p.kv_heads;
+    const unsigned s0 = s ? s_pre[s - 1] : 0, n = (s_pre[s] - s0) / (unsigned)p.kv_heads;
+    c0 = s0 + h * n;
+    c1 = c0 + n;
+  }
+  const unsigned base = (c1 - c0) / nwarps, rem = c1 - c0 - base * nwarps;
+  auto bound = [&](unsigned w) { return c0 + min(w, nwarps) * base + min(w, rem); };
+  const unsigned w0 = whole_items ? 0 : blockIdx.x * W;  // this CTA's first warp
+  const unsigned u0 = bound(w0 + warp), u1 = bound(w0 + warp + 1);
 
   // ---- copies: step u0 + i into slot i of the ring, through every item of this warp ----
   const uint8_t *src = nullptr;  // lane i: tile i % 2 of step u0 + batch + i / 2; null: no such
   unsigned there = 0;            // which lanes' tiles are
   int batch = -16;
-  auto look_ahead = [&](int i) {
+  auto look_ahead = [&](int i, Item c) {  // c: the item of step u0 + i, or one before
     batch = i;
     src = nullptr;
-    const unsigned g = u0 + i + lane / 2;
-    if (g < u1) {
-      const Item it = find_item<R, C::kThreads>(p, s_pre, per, g);
-      const int key = it.key_of(g) + lane % 2 * kKvTile;
-      if (it.real && key < it.end) {
-        const int page = p.table[(size_t)it.seq * p.max_pages + (key >> p.page_shift)];
-        if (page >= 0 && page < p.n_pages)
-          src = p.pages + ((unsigned long long)page * p.kv_heads + it.head) * p.page_bytes +
-                (unsigned)((key & ((1 << p.page_shift) - 1)) / kKvTile) * C::kTile;
-        else
-          attn_refuse(p, it.seq, APX_ERR_INVALID_ARGUMENT);
+    const unsigned g0 = u0 + i, g = g0 + lane / 2;
+    while (true) {
+      if (c.real && g >= c.i0 && g < min(c.i1, u1)) {
+        const int key = c.key_of(g) + lane % 2 * kKvTile;
+        if (key < c.end) {
+          const int page = p.table[(size_t)c.seq * p.max_pages + (key >> p.page_shift)];
+          if (page >= 0 && page < p.n_pages)
+            src = p.pages + ((unsigned long long)page * p.kv_heads + c.head) * p.page_bytes +
+                  (unsigned)((key & ((1 << p.page_shift) - 1)) / kKvTile) * C::kTile;
+          else
+            attn_refuse(p, c.seq, APX_ERR_INVALID_ARGUMENT);
+        }
       }
+      if (c.i1 >= min(g0 + 16, u1)) break;
+      c = find_item<R, ONE, C::kThreads>(p, s_pre, per, c.i1);
     }
     there = __ballot_sync(0xFFFFFFFFu, src != nullptr);
   };
@@ -291,7 +327,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   const Unpack un;
 #pragma unroll 1
   while (at < mine && alive) {
-    const Item it = find_item<R, C::kThreads>(p, s_pre, per, u0 + at);
+    const Item it = find_item<R, ONE, C::kThreads>(p, s_pre, per, u0 + at);
     const int stop = (int)(min(it.i1, u1) - u0);
     // the block's query rows, asked for before the first copies
     constexpr int QV = SPLIT == 2 ? D / 16 : D / 32;  // 16-byte loads a row and thread
@@ -313,7 +349,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
       }
     }
     if (at == 0) {
-      look_ahead(0);
+      look_ahead(0, it);
       for (int i = 0; i < min(mine, C::kSlots); i++) start(i);
     }
     const int end = it.end;
@@ -402,14 +438,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
     for (; at < stop; at++) {
       arrived(at);
       uint8_t *tile = ring + (at & (C::kSlots - 1)) * C::kSlot;
-      if (!it.real) {  // filling: no keys, no copies
-        __syncwarp();
-        if (at + C::kSlots < mine) {
-          if (at + C::kSlots - batch >= 16) look_ahead(at + C::kSlots);
-          start(at + C::kSlots);
-        }
-        continue;
-      }
+      if (ONE || it.real) {  // not a pair's filling, which has no keys
       const int key = it.key_of(u0 + at);
       if (key + kStepKeys > end) {
         // tokens past the last key may hold anything: V's scales there count as zero (K's are
@@ -602,9 +631,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
           }
         }
       }
+      }
       __syncwarp();  // every lane has read the slot
       if (at + C::kSlots < mine) {
-        if (at + C::kSlots - batch >= 16) look_ahead(at + C::kSlots);
+        if (at + C::kSlots - batch >= 16) look_ahead(at + C::kSlots, it);
         start(at + C::kSlots);
       }
     }
@@ -661,103 +691,90 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   }
   if (!alive && lane == 0) attn_refuse(p, 0, APX_ERR_DEVICE_TIMEOUT);
 
-  // ---- the join: items that cross warps, then items that cross CTAs ----
+  // ---- the join: items that cross warps, each by the warp that has its first part ----
   __syncthreads();
-  const unsigned c0 = bound(blockIdx.x * W), c1 = bound((blockIdx.x + 1) * W);
-  constexpr int E = R * D / 4;  // quads of an item's rows
+  const unsigned e0 = bound(w0), e1 = bound(w0 + W);  // this CTA's steps
+  constexpr int E = R * D / 4, Q = D / 4;             // quads of an item's rows, of a row
   auto part_of = [&](int w, int e) {
     return reinterpret_cast<const float *>(smem + w * C::kWarpSmem + (e ? 0 : C::kRing));
-  };
-  auto write4 = [&](const Edge &ed, int r, int d, const float4 v, float sum) {
-    const int row = ed.row0 + r;
-    if (row >= ed.rows) return;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int tok = by_group(p, row);
-    const unsigned long long at =
-        (unsigned long long)(ed.first + tok) * p.ldo +
-        (unsigned long long)(ed.head * p.group + row - tok * p.group) * D + d;
-    if (SPLIT == 2) {
-      *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) =
-          make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-    } else {
-      uint2 w;
-      if (TYPE == APX_DTYPE_BF16) {
-        __nv_bfloat162 x = __floats2bfloat162_rn(v.x * inv, v.y * inv);
-        __nv_bfloat162 y = __floats2bfloat162_rn(v.z * inv, v.w * inv);
-        w = make_uint2(*reinterpret_cast<uint32_t *>(&x), *reinterpret_cast<uint32_t *>(&y));
-      } else {
-        w = make_uint2(h2u(__floats2half2_rn(v.x * inv, v.y * inv)),
-                       h2u(__floats2half2_rn(v.z * inv, v.w * inv)));
-      }
-      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) = w;
-    }
   };
   auto add4 = [](float4 &v, float f, const float4 x) {
     v = make_float4(fmaf(f, x.x, v.x), fmaf(f, x.y, v.y), fmaf(f, x.z, v.z), fmaf(f, x.w, v.w));
   };
-  // the edges of the warps, one a lane (the same in every warp)
-  const bool lane_used = lane < W && s_edge[lane % W][0].used;
-  const unsigned lane_begin = s_edge[lane % W][0].begin;
-  // the first part of each item in this CTA: the one that began before it, and the last items of
-  // its warps
-  unsigned starts = __ballot_sync(0xFFFFFFFFu, lane < W && s_edge[lane % W][1].used);
-  bool from_before = __shfl_sync(0xFFFFFFFFu, (int)lane_used, 0);
-  int out_of_cta = 0;  // bit 0: the item that began before this CTA; bit 1: its last item
-  Edge edge0, edge1;
-  while (from_before || starts) {
-    const int w = from_before ? 0 : __ffs(starts) - 1, e = from_before ? 0 : 1;
-    if (!from_before) starts &= starts - 1;
-    from_before = false;
-    const Edge ed = s_edge[w][e];
-    // its parts: this one and the first edges of the warps that follow
-    const unsigned same =
-        __ballot_sync(0xFFFFFFFFu, lane_used && lane > w && lane_begin == ed.begin);
-    const int n = __popc(same) + 1;
-    for (int i = tid; i < n * R; i += C::kThreads) {
-      const int k = i / R, r = i % R;
-      float top = -INFINITY;
-#pragma unroll 4
-      for (int j = 0; j < n; j++) top = fmaxf(top, part_of(w + j, j ? 0 : e)[R * D + r]);
-      const float *src = part_of(w + k, k ? 0 : e);
-      const float m = src[R * D + r], f = m == -INFINITY ? 0.0f : ex2(m - top);
-      s_f[k * R + r] = f;
-      s_l[k * R + r] = f * src[R * D + R + r];
-      if (k == 0) s_top[r] = top;
-    }
-    __syncthreads();
-    const bool whole = ed.begin >= c0 && ed.end <= c1;
-    const int at = ed.begin >= c0 ? 1 : 0;
-    float *dst = p.part + ((size_t)blockIdx.x * 2 + at) * C::kPart;
-    if (!whole) {
-      out_of_cta |= 1 << at;
-      if (at) edge1 = ed;
-      else edge0 = ed;
-    }
-    for (int i = tid; i < E; i += C::kThreads) {
-      const int r = i / (D / 4), d = i % (D / 4) * 4;
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float sum = 0.0f;
-#pragma unroll 4
-      for (int k = 0; k < n; k++) {
-        add4(v, s_f[k * R + r],
-             *reinterpret_cast<const float4 *>(part_of(w + k, k ? 0 : e) + r * D + d));
-        sum += s_l[k * R + r];
+  auto write4 = [&](const Edge &ed, int r, int d, const float4 v, float inv) {
+    const int row = ed.row0 + r;
+    if (row >= ed.rows) return;
+    const int tok = by_group(p, row);
+    store4<TYPE>(p.out,
+                 (unsigned long long)(ed.first + tok) * p.ldo +
+                     (unsigned long long)(ed.head * p.group + row - tok * p.group) * D + d,
+                 make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+  };
+  {
+    const bool used = lane < W && s_edge[lane % W][0].used;
+    const unsigned begin = s_edge[lane % W][0].begin;
+#pragma unroll 1
+    for (int e = warp ? 1 : 0; e < 2; e++) {
+      if (!s_edge[warp][e].used) continue;
+      const Edge ed = s_edge[warp][e];
+      // its parts: this one and the first edges of the warps that follow
+      const int n =
+          __popc(__ballot_sync(0xFFFFFFFFu, used && lane > warp && begin == ed.begin)) + 1;
+      const float *first = part_of(warp, e), *rest = part_of(warp, 0);
+      constexpr int S = C::kWarpSmem / 4;  // from a warp's part to the next one's
+      // the parts' factors, then the sums: lane's row is lane % R
+      float top = -INFINITY, sum = 0.0f;
+      for (int k = lane / R; k < n; k += 32 / R)
+        top = fmaxf(top, (k ? rest + k * S : first)[R * D + lane % R]);
+#pragma unroll
+      for (int o = R; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      for (int k = lane / R; k < n; k += 32 / R) {
+        const float *part = (k ? rest + k * S : first) + R * D + lane % R;
+        const float f = part[0] == -INFINITY ? 0.0f : ex2(part[0] - top);
+        sum = fmaf(f, part[R], sum);
+        s_f[warp][k * R + lane % R] = f;
       }
-      if (whole) {
-        write4(ed, r, d, v, sum);
-      } else {
-        *reinterpret_cast<float4 *>(dst + r * D + d) = v;
-        if (d == 0) {
-          dst[R * D + r] = s_top[r];
-          dst[R * D + R + r] = sum;
-        }
+#pragma unroll
+      for (int o = R; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+      __syncwarp();
+      const bool whole = ed.begin >= e0 && ed.end <= e1;
+      const float scale = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+      float *dst = p.part + ((size_t)blockIdx.x * 2 + (ed.begin >= e0 ? 1 : 0)) * C::kPart;
+      if (!whole && lane < R) {
+        dst[R * D + lane] = top;
+        dst[R * D + R + lane] = sum;
       }
+#pragma unroll 2
+      for (int i = lane; i < E; i += 32) {
+        const int r = i / Q, d = i % Q * 4;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        add4(v, s_f[warp][r], *reinterpret_cast<const float4 *>(first + r * D + d));
+#pragma unroll 4
+        for (int k = 1; k < n; k++)
+          add4(v, s_f[warp][k * R + r],
+               *reinterpret_cast<const float4 *>(rest + k * S + r * D + d));
+        const float inv = __shfl_sync(0xFFFFFFFFu, scale, r);
+        if (whole) write4(ed, r, d, v, inv);
+        else *reinterpret_cast<float4 *>(dst + r * D + d) = v;
+      }
+      __syncwarp();
     }
-    __syncthreads();
+  }
+  // ---- items that cross CTAs: the CTA that arrives last joins their parts, in their order ----
+  if (whole_items) return;
+  int out_of_cta = 0;  // bit 0: an item began before this CTA; bit 1: one goes on after it
+  Edge edge0 = s_edge[0][0], edge1;
+  if (edge0.used && edge0.begin < e0) out_of_cta = 1;
+  {
+    const unsigned any = __ballot_sync(0xFFFFFFFFu, lane < W && (s_edge[lane % W][0].used ||
+                                                                 s_edge[lane % W][1].used));
+    if (!any) return;
+    const int last = 31 - __clz(any);
+    edge1 = s_edge[last][s_edge[last][1].used ? 1 : 0];
+    if (edge1.end > e1 && edge1.begin >= e0) out_of_cta |= 2;
   }
   if (!out_of_cta) return;  // the same in every thread
-
-  // an item's CTAs: the first holds it as its last item, the others as the one from before
+  // An item's CTAs: the first holds it as its last item, the others as the one from before.
   auto cta_of = [&](unsigned step) {
     const unsigned wide = rem * (base + 1);
     return (int)((step < wide ? step / (base + 1) : rem + (step - wide) / base) / W);
@@ -784,18 +801,17 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
     const int n = s_last[e];
     if (!n) continue;
     const Edge ed = e ? edge1 : edge0;
-    const int a = cta_of(ed.begin);
-    auto src_of = [&](int k) {
-      return p.part + ((size_t)(a + k) * 2 + (k == 0 ? 1 : 0)) * C::kPart;
-    };
+    const float *first = p.part + ((size_t)cta_of(ed.begin) * 2 + 1) * C::kPart;
+    auto src_of = [&](int k) { return first + (k ? (size_t)(2 * k - 1) * C::kPart : 0); };
     // the parts' factors, then their sum by groups of threads, each a share of the parts
     float *f = reinterpret_cast<float *>(smem), *fl = f + n * R;
     float4 *red = reinterpret_cast<float4 *>(smem + ((n * R * 8 + 15) & ~15));
     for (int i = tid; i < n * R; i += C::kThreads) {
-      const float *src = src_of(i / R) + R * D + i % R;
-      f[i] = __ldcg(src);
-      fl[i] = __ldcg(src + R);
+      const float *part = src_of(i / R) + R * D + i % R;
+      f[i] = __ldcg(part);
+      fl[i] = __ldcg(part + R);
     }
+    constexpr int G = C::kThreads >= E ? C::kThreads / E : 1;
     __syncthreads();
     for (int r = warp; r < R; r += W) {
       float top = -INFINITY, sum = 0.0f;
@@ -809,17 +825,16 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-      if (lane == 0) s_l[r] = sum;
+      if (lane == 0) s_f[0][r] = sum == 0.0f ? 0.0f : 1.0f / sum;
     }
     __syncthreads();
-    constexpr int G = C::kThreads >= E ? C::kThreads / E : 1;
     for (int i = tid; i < E * G; i += C::kThreads) {
-      const int q4 = i % E, r = q4 / (D / 4), d = q4 % (D / 4) * 4;
+      const int q4 = i % E, r = q4 / Q, d = q4 % Q * 4;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
       for (int k = i / E; k < n; k += G)
         add4(v, f[k * R + r], __ldcg(reinterpret_cast<const float4 *>(src_of(k) + r * D + d)));
-      if (G == 1) write4(ed, r, d, v, s_l[r]);
+      if (G == 1) write4(ed, r, d, v, s_f[0][r]);
       else red[i] = v;
     }
     if (G > 1) {
@@ -828,7 +843,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
         float4 v = red[i];
 #pragma unroll
         for (int g = 1; g < G; g++) add4(v, 1.0f, red[g * E + i]);
-        write4(ed, i / (D / 4), i % (D / 4) * 4, v, s_l[i / (D / 4)]);
+        write4(ed, i / Q, i % Q * 4, v, s_f[0][i / Q]);
       }
     }
     __syncthreads();
@@ -895,7 +910,6 @@ cudaError_t launch_attn_kv4(const apx_attn_args &a, const apx_kv4_cache &c,
   p.window = a.window;
   p.sinks = a.window ? a.sinks : 0;
   p.type = a.type;
-  p.warps_min = 1;
   p.scale = a.scale;
   p.group_mul = (unsigned)(0x100000000ull / (unsigned)p.group + 1);
   const int grid = std::min(sms, kCountBytes / 4);

@@ -46,7 +46,7 @@ struct AttnArgs {
   float *part;      // apx_attn.cu: two partial items per CTA
   unsigned *count;  // apx_attn.cu: CTAs that have arrived at an item (zero between calls)
   int n_pages, n_seqs, max_pages, kv_heads, group, page_shift;
-  int window, sinks, type, warps_min, n_tokens;
+  int window, sinks, type, n_tokens;
   unsigned group_mul;  // 2^32 / group + 1, for by_group
   float scale;
 };
