@@ -286,6 +286,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   const uint8_t *src = nullptr;  // lane i: tile i % 2 of step u0 + batch + i / 2; null: no such
   unsigned there = 0;            // which lanes' tiles are
   int batch = -16;
+  const uint64_t policy = stream_policy();
   auto look_ahead = [&](int i, Item c) {  // c: the item of step u0 + i, or one before
     batch = i;
     src = nullptr;
@@ -312,7 +313,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
     if (lane == owner)
       mbar_expect_tx(bar + sl, (uint32_t)__popc(there >> owner & 3u) * C::kTile);
     if ((lane & ~1) == owner && src != nullptr)
-      bulk_g2s(ring + sl * C::kSlot + (lane & 1) * C::kTile, src, C::kTile, bar + sl);
+      bulk_g2s_policy(ring + sl * C::kSlot + (lane & 1) * C::kTile, src, C::kTile, bar + sl,
+                      policy);
   };
   const int mine = (int)(u1 - u0);  // steps of this warp
   int at = 0;                       // of them, done

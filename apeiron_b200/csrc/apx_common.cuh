@@ -184,6 +184,22 @@ __device__ __forceinline__ void bulk_g2s(void *dst, const void *src, uint32_t by
       : "memory");
 }
 
+// The same with an L2 policy.  stream_policy: data read once, the first to make room for other
+// data (weights, activations, instructions).
+__device__ __forceinline__ uint64_t stream_policy() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ void bulk_g2s_policy(void *dst, const void *src, uint32_t bytes,
+                                                uint64_t *bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], "
+      "[%1], %2, [%3], %4;" ::"r"(smem_addr(dst)),
+      "l"(src), "r"(bytes), "r"(smem_addr(bar)), "l"(policy)
+      : "memory");
+}
+
 // Wait for phase `parity` of the barrier; false if the bounded wait gave up (after
 // kWaitLimit polls or about one second of %globaltimer, whichever comes first).  A poll
 // that finds the phase open backs off with a short sleep, so that waiting warps leave the
