@@ -47,6 +47,10 @@ cudaError_t launch_attn_tc(const AttnArgs &p, int dim, int max_q, cudaStream_t s
 namespace {
 
 constexpr int kStepKeys = 32;
+// What a warp loses at an item's end (its rows to keep or write, the next one's to read), in steps:
+// items of single tokens carry as many steps without keys, so that warps with a boundary get fewer
+// keys (64 ragged requests: 53.2 -> 51.4 us; prompts' many short items lose by it).
+constexpr int kItemCost = 2;
 // Probabilities are held at 2^13 e^(s - m), where m is a stale maximum: it moves when a score
 // outgrows it by more than 2^2.
 constexpr float kTopExp = 13.0f, kStale = 2.0f;
@@ -95,7 +99,7 @@ __device__ __forceinline__ void store_out(void *o, unsigned long long i, float v
 }
 
 // A sequence's steps.  Its blocks of rows pair first with last: a pair has `pair` steps, the
-// first block's, then the second's, then none.  ONE: every sequence has one block at most.
+// first block's, then the second's, then filling, steps without keys.  ONE: every sequence has one block at most.
 template <int R, bool ONE>
 struct SeqShape : SeqRows<R, kStepKeys> {
   using Base = SeqRows<R, kStepKeys>;
@@ -105,7 +109,7 @@ struct SeqShape : SeqRows<R, kStepKeys> {
     Base::load(p, s);
     const int n = this->nblk;
     if (n <= 0) pair = 0;
-    else if (ONE || n == 1) pair = steps(p, 0);
+    else if (ONE || n == 1) pair = steps(p, 0) + kItemCost;
     else if (!p.window) pair = steps(p, 0) + steps(p, n - 1) + 2;
     else {
       // a window's keys: what the block's positions span, in whole steps
@@ -184,7 +188,7 @@ __device__ __noinline__ Item find_item(const AttnArgs &p, const unsigned *pre, i
   int blk = ONE ? 0 : (int)(nth - it.head * n);
   it.i0 = seq0 + nth * q.pair;
   const unsigned end = it.i0 + q.pair;
-  it.i1 = ONE ? end : it.i0 + q.steps(p, blk);
+  it.i1 = it.i0 + q.steps(p, blk);
   if (!ONE && g >= it.i1 && blk != q.nblk - 1 - blk) {
     blk = q.nblk - 1 - blk;
     it.i0 = it.i1;
@@ -212,7 +216,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   __shared__ __align__(8) uint64_t s_bar[W * C::kSlots];
   __shared__ Edge s_edge[W][2];
   __shared__ int s_last[2], s_most[W];
-  __shared__ float s_f[W][W * R];
+  __shared__ float s_inv[R];
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, gid = lane / 4, tig = lane % 4;
   pdl_launch_dependents();
@@ -267,7 +271,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   // CTAs for all items and the longest costs a warp four steps at most: an item per CTA, which
   // saves the join through the workspace (0.5B shape, 777 keys: 13.5 -> 8.6 us).
   const int items = ONE ? p.n_seqs * p.kv_heads : 0;
-  const bool whole_items = ONE && items <= (int)gridDim.x && longest <= 4 * W;
+  const bool whole_items = ONE && items <= (int)gridDim.x && longest <= 4 * W + kItemCost;
   const unsigned nwarps = whole_items ? W : min(gridDim.x * W, max(total, 1u));
   unsigned c0 = 0, c1 = total;
   if (whole_items) {
@@ -275,7 +279,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
     const int s = blockIdx.x / p.kv_heads, h = blockIdx.x - s * p.kv_heads;
     const unsigned s0 = s ? s_pre[s - 1] : 0, n = (s_pre[s] - s0) / (unsigned)p.kv_heads;
     c0 = s0 + h * n;
-    c1 = c0 + n;
+    c1 = c0 + (n ? n - kItemCost : 0);
   }
   const unsigned base = (c1 - c0) / nwarps, rem = c1 - c0 - base * nwarps;
   auto bound = [&](unsigned w) { return c0 + min(w, nwarps) * base + min(w, rem); };
@@ -440,7 +444,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
     for (; at < stop; at++) {
       arrived(at);
       uint8_t *tile = ring + (at & (C::kSlots - 1)) * C::kSlot;
-      if (ONE || it.real) {  // not a pair's filling, which has no keys
+      if (it.real) {  // not filling, which has no keys
       const int key = it.key_of(u0 + at);
       if (key + kStepKeys > end) {
         // tokens past the last key may hold anything: V's scales there count as zero (K's are
@@ -713,53 +717,59 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
                  make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
   };
   {
+    // a bit per warp: whose first edge, whose last edge is used
     const bool used = lane < W && s_edge[lane % W][0].used;
     const unsigned begin = s_edge[lane % W][0].begin;
+    const unsigned firsts = __ballot_sync(0xFFFFFFFFu, used);
+    unsigned starts = __ballot_sync(0xFFFFFFFFu, lane < W && s_edge[lane % W][1].used);
+    // items here: the one that began before this CTA or at its first warp's first step, and each
+    // warp's last; their rows go round the warps
+    const int items_here = (int)(firsts & 1) + __popc(starts);
+    int item = 0;
 #pragma unroll 1
-    for (int e = warp ? 1 : 0; e < 2; e++) {
-      if (!s_edge[warp][e].used) continue;
-      const Edge ed = s_edge[warp][e];
+    for (int j = warp; j < items_here * R; j += W) {
+      while (item < j / R - (int)(firsts & 1)) {
+        starts &= starts - 1;
+        item++;
+      }
+      const bool head = (firsts & 1) && j < R;
+      const int w = head ? 0 : __ffs(starts) - 1, r = j % R;
+      const Edge &ed = s_edge[w][head ? 0 : 1];
       // its parts: this one and the first edges of the warps that follow
       const int n =
-          __popc(__ballot_sync(0xFFFFFFFFu, used && lane > warp && begin == ed.begin)) + 1;
-      const float *first = part_of(warp, e), *rest = part_of(warp, 0);
+          __popc(__ballot_sync(0xFFFFFFFFu, used && lane > w && begin == ed.begin)) + 1;
+      const float *first = part_of(w, head ? 0 : 1), *rest = part_of(w, 0);
       constexpr int S = C::kWarpSmem / 4;  // from a warp's part to the next one's
-      // the parts' factors, then the sums: lane's row is lane % R
-      float top = -INFINITY, sum = 0.0f;
-      for (int k = lane / R; k < n; k += 32 / R)
-        top = fmaxf(top, (k ? rest + k * S : first)[R * D + lane % R]);
+      const float *mine = (lane ? rest + min(lane, n - 1) * S : first) + R * D + r;
+      const float m = lane < n ? mine[0] : -INFINITY, l = lane < n ? mine[R] : 0.0f;
+      float top = m;
 #pragma unroll
-      for (int o = R; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-      for (int k = lane / R; k < n; k += 32 / R) {
-        const float *part = (k ? rest + k * S : first) + R * D + lane % R;
-        const float f = part[0] == -INFINITY ? 0.0f : ex2(part[0] - top);
-        sum = fmaf(f, part[R], sum);
-        s_f[warp][k * R + lane % R] = f;
-      }
+      for (int o = W / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      const float f = m == -INFINITY ? 0.0f : ex2(m - top);
+      float sum = f * l;
 #pragma unroll
-      for (int o = R; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-      __syncwarp();
-      const bool whole = ed.begin >= e0 && ed.end <= e1;
-      const float scale = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
-      float *dst = p.part + ((size_t)blockIdx.x * 2 + (ed.begin >= e0 ? 1 : 0)) * C::kPart;
-      if (!whole && lane < R) {
-        dst[R * D + lane] = top;
-        dst[R * D + R + lane] = sum;
-      }
-#pragma unroll 2
-      for (int i = lane; i < E; i += 32) {
-        const int r = i / Q, d = i % Q * 4;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        add4(v, s_f[warp][r], *reinterpret_cast<const float4 *>(first + r * D + d));
+      for (int o = W / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+      top = __shfl_sync(0xFFFFFFFFu, top, 0);
+      sum = __shfl_sync(0xFFFFFFFFu, sum, 0);
+      const int d = 4 * (lane % Q);  // half the warp idles at D = 64
+      const float f0 = __shfl_sync(0xFFFFFFFFu, f, 0);
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      add4(v, f0, *reinterpret_cast<const float4 *>(first + r * D + d));
 #pragma unroll 4
-        for (int k = 1; k < n; k++)
-          add4(v, s_f[warp][k * R + r],
-               *reinterpret_cast<const float4 *>(rest + k * S + r * D + d));
-        const float inv = __shfl_sync(0xFFFFFFFFu, scale, r);
-        if (whole) write4(ed, r, d, v, inv);
-        else *reinterpret_cast<float4 *>(dst + r * D + d) = v;
+      for (int k = 1; k < n; k++)
+        add4(v, __shfl_sync(0xFFFFFFFFu, f, k),
+             *reinterpret_cast<const float4 *>(rest + k * S + r * D + d));
+      if (lane >= Q) continue;
+      if (ed.begin >= e0 && ed.end <= e1) {
+        write4(ed, r, d, v, sum == 0.0f ? 0.0f : 1.0f / sum);
+      } else {
+        float *dst = p.part + ((size_t)blockIdx.x * 2 + (ed.begin >= e0 ? 1 : 0)) * C::kPart;
+        *reinterpret_cast<float4 *>(dst + r * D + d) = v;
+        if (lane == 0) {
+          dst[R * D + r] = top;
+          dst[R * D + R + r] = sum;
+        }
       }
-      __syncwarp();
     }
   }
   // ---- items that cross CTAs: the CTA that arrives last joins their parts, in their order ----
@@ -805,15 +815,26 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
     const Edge ed = e ? edge1 : edge0;
     const float *first = p.part + ((size_t)cta_of(ed.begin) * 2 + 1) * C::kPart;
     auto src_of = [&](int k) { return first + (k ? (size_t)(2 * k - 1) * C::kPart : 0); };
-    // the parts' factors, then their sum by groups of threads, each a share of the parts
+    // the parts' factors, then their sum by groups of threads, each a share of the parts; a
+    // thread's first eight quads are on their way meanwhile
+    constexpr int G = C::kThreads >= E ? C::kThreads / E : 1;
+    constexpr int PER = E * G / C::kThreads;  // quads of the rows a thread has
     float *f = reinterpret_cast<float *>(smem), *fl = f + n * R;
     float4 *red = reinterpret_cast<float4 *>(smem + ((n * R * 8 + 15) & ~15));
+    float4 x[PER][8 / PER];
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      const int i = tid + j * C::kThreads, q4 = i % E;
+#pragma unroll
+      for (int k = 0; k < 8 / PER; k++)
+        if (i / E + k * G < n)
+          x[j][k] = __ldcg(reinterpret_cast<const float4 *>(src_of(i / E + k * G) + 4 * q4));
+    }
     for (int i = tid; i < n * R; i += C::kThreads) {
       const float *part = src_of(i / R) + R * D + i % R;
       f[i] = __ldcg(part);
       fl[i] = __ldcg(part + R);
     }
-    constexpr int G = C::kThreads >= E ? C::kThreads / E : 1;
     __syncthreads();
     for (int r = warp; r < R; r += W) {
       float top = -INFINITY, sum = 0.0f;
@@ -821,22 +842,26 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
       for (int k = lane; k < n; k += 32) {
-        const float m = f[k * R + r], x = m == -INFINITY ? 0.0f : ex2(m - top);
-        f[k * R + r] = x;
-        sum += x * fl[k * R + r];
+        const float m = f[k * R + r], g = m == -INFINITY ? 0.0f : ex2(m - top);
+        f[k * R + r] = g;
+        sum += g * fl[k * R + r];
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-      if (lane == 0) s_f[0][r] = sum == 0.0f ? 0.0f : 1.0f / sum;
+      if (lane == 0) s_inv[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
     }
     __syncthreads();
-    for (int i = tid; i < E * G; i += C::kThreads) {
-      const int q4 = i % E, r = q4 / Q, d = q4 % Q * 4;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      const int i = tid + j * C::kThreads, q4 = i % E, r = q4 / Q;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int k = 0; k < 8 / PER; k++)
+        if (i / E + k * G < n) add4(v, f[(i / E + k * G) * R + r], x[j][k]);
 #pragma unroll 4
-      for (int k = i / E; k < n; k += G)
-        add4(v, f[k * R + r], __ldcg(reinterpret_cast<const float4 *>(src_of(k) + r * D + d)));
-      if (G == 1) write4(ed, r, d, v, s_f[0][r]);
+      for (int k = i / E + 8 / PER * G; k < n; k += G)
+        add4(v, f[k * R + r], __ldcg(reinterpret_cast<const float4 *>(src_of(k) + 4 * q4)));
+      if (G == 1) write4(ed, r, q4 % Q * 4, v, s_inv[r]);
       else red[i] = v;
     }
     if (G > 1) {
@@ -845,7 +870,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
         float4 v = red[i];
 #pragma unroll
         for (int g = 1; g < G; g++) add4(v, 1.0f, red[g * E + i]);
-        write4(ed, i / Q, i % Q * 4, v, s_f[0][i / Q]);
+        write4(ed, i / Q, i % Q * 4, v, s_inv[i / Q]);
       }
     }
     __syncthreads();
