@@ -1,16 +1,17 @@
-// apx_attn_tc.cu — attention over the paged 4-bit cache for prompts: 128 query rows at a time on
+// apx_attn_tc.cu — attention over the paged 4-bit cache for prompts: query rows 128 at a time on
 // the tensor cores (apx_attn.cu serves few rows, and f32).
 //
-// A CTA holds 128 query rows of one KV head (a token's group of heads are neighbouring rows) and
-// takes its keys 128 at a time: S = Q K^T into TMEM, the softmax warps turn S into probabilities
-// in place (f16), O += P V with P read from TMEM.  Warps 4-7 unpack the next keys and values from
-// the cache's pages to f16 operands in shared memory (exact: d (c - 8) fits f16), registers
-// holding the bytes in flight.  Two CTAs share an SM, so that one's products run under the
-// other's softmax.
+// A CTA holds two tiles of 128 query rows of one KV head (a token's group of heads are neighbouring
+// rows) and takes its keys 128 at a time: S = Q K^T into TMEM, four softmax warps a tile turn S
+// into probabilities in place (f16), O += P V with P read from TMEM.  A tile's first softmax thread
+// issues its products.  The second tile starts a softmax later: while one is in its softmax the
+// other's products run.  Both read the same keys and values, which eight warps unpack from the
+// cache's pages to f16 operands in shared memory (exact: d (c - 8) fits f16), two buffers each,
+// registers holding the bytes in flight.
 //
-// What bounds it, per 128 x 128 step at D = 128: the products 1024 cycles, the exponentials 1024
-// (16 a cycle), shared memory 1280 (S reads both operands, P V one, the unpacked keys and values
-// go in once).
+// What bounds it, per 128 x 128 step of a tile at D = 128: the products 1024 cycles, the
+// exponentials 1024 (16 a cycle), shared memory 1024 (S reads both operands, P V one, the unpacked
+// keys and values go in for both tiles).
 //
 // The running maximum is a stale one: O (in TMEM) and the row sum turn only when a row's maximum
 // has grown by more than 2^8 since the last turn; probabilities are held at 2^6 e^(s - m), at most
@@ -19,6 +20,8 @@
 // K's dims are stored in the order the unpacking yields them (0 4 1 5 2 6 3 7 of every eight), Q's
 // the same.
 #include <cuda_bf16.h>
+
+#include <type_traits>
 
 #include "apx_common.cuh"
 #include "apx_kernels.h"
@@ -30,47 +33,81 @@ namespace apx {
 
 namespace {
 
-constexpr int kRows = 128, kKeys = 128;
-constexpr int kThreads = 288;       // 4 softmax warps, 4 unpacking warps, 1 that issues products
-constexpr float kStale = 8.0f;      // log2 of how far a row's maximum may outgrow the stale one
-constexpr float kOffset = 6.0f;     // probabilities are held at 2^6 e^(s - m)
-constexpr int kTmemCols = 256;      // S (then P) in columns 0-127, O from 128 on
-constexpr int kOCol = 128;
+constexpr int kTile = 128, kRows = 2 * kTile, kKeys = 128;
+constexpr int kThreads = 512;     // 8 softmax warps, 8 unpacking warps
+constexpr int kUnpack = 256;      // unpacking threads
+constexpr float kStale = 8.0f;    // log2 of how far a row's maximum may outgrow the stale one
+constexpr float kOffset = 6.0f;   // probabilities are held at 2^6 e^(s - m)
+constexpr int kTmemCols = 512;    // S (then P) of the tiles in columns 0-255, O from 256 on
 
 // K-major operands in the 128-byte swizzle: rows of 64 f16, 8-row groups 1024 bytes apart.
 constexpr uint64_t kDesc = ((uint64_t)(16 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
                            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 // kind::f16: D f32 (1) at bits 4-5, A and B f16 (0), N >> 3 at bits 17-22, M >> 4 at bits 24-28.
 __host__ __device__ constexpr uint32_t idesc_f16(int n) {
-  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
 
 template <int D>
 struct Smem {
-  // operands in panels of 64 columns: Q and K by dims, V^T by keys
+  // operands in panels of 64 columns: Q (both tiles) and K by dims, V^T by keys
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + kRows * D * 2;
-  static constexpr int kV = kK + kKeys * D * 2;
-  static constexpr int kCq = kV + kKeys * D * 2;
+  static constexpr int kOne = kKeys * D * 2;  // a buffer of K or V
+  static constexpr int kV = kK + 2 * kOne;
+  static constexpr int kCq = kV + 2 * kOne;
   static constexpr int kBars = kCq + kRows * 4;
-  static constexpr int kBytes = kBars + 64 + 1024;  // and the base's alignment
+  static constexpr int kBytes = kBars + 128 + 1024;  // and the base's alignment
 };
 
 // 16-byte chunk c (of 8) of row r in a panel of 128-byte rows.
 __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
+// Two f32 at a time.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+__device__ __forceinline__ float as_f(uint32_t x) { return __uint_as_float(x); }
+__device__ __forceinline__ float as_f(float x) { return x; }
+template <typename A, typename B, typename C>
+__device__ __forceinline__ float max3(A a, B b, C c) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(as_f(a)), "f"(as_f(b)), "f"(as_f(c)));
+  return m;
+}
+
 template <int D>
-__global__ void __launch_bounds__(kThreads, 2) attn_tc_kernel(AttnArgs p) {
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_tc_kernel(const __grid_constant__ AttnArgs p) {
   using L = Smem<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
-  uint64_t *k_full = bars, *v_full = bars + 1, *s_full = bars + 2, *p_full = bars + 3,
-           *o_full = bars + 4;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 5);
+  uint64_t *k_full = bars, *v_full = bars + 2, *k_free = bars + 4, *v_free = bars + 6;
+  uint64_t *s_full = bars + 8, *o_full = bars + 10;  // per tile
+  uint64_t *second = bars + 12;                      // the second tile may start
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 13);
   float *s_cq = reinterpret_cast<float *>(smem + L::kCq);
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int tid = threadIdx.x, warp = tid / 32;
   const int seq = blockIdx.x / p.kv_heads, head = blockIdx.x % p.kv_heads;
 
   pdl_launch_dependents();
@@ -84,22 +121,28 @@ __global__ void __launch_bounds__(kThreads, 2) attn_tc_kernel(AttnArgs p) {
   int end, sink, from;
   q.range(p, blk, end, sink, from);
   const int n = sink + max(q.steps_to(end) - from, 0);
+  const int tiles = q.rows - blk * kRows > kTile ? 2 : 1;
   auto key_of = [&](int j) { return (j < sink ? j : j - sink + from) * kKeys; };
 
-  if (warp == 8) {
+  if (warp == 15) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_addr(tmem_slot)),
                  "r"(kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    if (lane == 0) {
-      mbar_init(k_full, 128);
-      mbar_init(v_full, 128);
-      mbar_init(s_full, 1);
-      mbar_init(p_full, 128);
-      mbar_init(o_full, 1);
+  }
+  if (tid == 0) {
+    for (int i = 0; i < 2; i++) {
+      mbar_init(k_full + i, kUnpack);
+      mbar_init(v_full + i, kUnpack);
+      mbar_init(k_free + i, tiles);
+      mbar_init(v_free + i, tiles);
+      mbar_init(s_full + i, 1);
+      mbar_init(o_full + i, 1);
     }
-  } else {
+    mbar_init(second, 1);
+  }
+  {
     // ---- Q: two threads a row ----
     const int row = tid / 2, half = tid % 2;
     const int r = blk * kRows + row;
@@ -108,9 +151,10 @@ __global__ void __launch_bounds__(kThreads, 2) attn_tc_kernel(AttnArgs p) {
 #pragma unroll
     for (int i = 0; i < D / 16; i++) x[i] = make_uint4(0, 0, 0, 0);
     if (r < q.rows) {
+      const int tok = by_group(p, r);
       const uint4 *src = reinterpret_cast<const uint4 *>(
-          static_cast<const uint16_t *>(p.q) + (unsigned long long)(q.first + r / p.group) * p.ldq +
-          (unsigned long long)(head * p.group + r % p.group) * D + half * (D / 2));
+          static_cast<const uint16_t *>(p.q) + (unsigned long long)(q.first + tok) * p.ldq +
+          (unsigned long long)(head * p.group + r - tok * p.group) * D + half * (D / 2));
 #pragma unroll
       for (int i = 0; i < D / 16; i++) x[i] = src[i];
     }
@@ -132,13 +176,14 @@ __global__ void __launch_bounds__(kThreads, 2) attn_tc_kernel(AttnArgs p) {
     const int e = row_exponent(top);
     const float up = p.scale < 0.0f ? -pow2(9 - e) : pow2(9 - e);  // so that scores grow with S
     if (half == 0) s_cq[row] = fabsf(p.scale) * 1.44269504088896341f * pow2(e - 9);
+    uint8_t *dst = smem + L::kQ + row / kTile * (kTile * D * 2);
 #pragma unroll
     for (int i = 0; i < D / 16; i++) {
       const float2 a = pair(x[i].x), b = pair(x[i].y), c = pair(x[i].z), d = pair(x[i].w);
       auto two = [&](float u, float v) { return h2u(__floats2half2_rn(u * up, v * up)); };
       const int chunk = half * (D / 16) + i;
-      *reinterpret_cast<uint4 *>(smem + L::kQ + chunk / 8 * (kRows * 128) +
-                                 swizzled(row, chunk % 8)) =
+      *reinterpret_cast<uint4 *>(dst + chunk / 8 * (kTile * 128) +
+                                 swizzled(row % kTile, chunk % 8)) =
           make_uint4(two(a.x, c.x), two(a.y, c.y), two(b.x, d.x), two(b.y, d.y));
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -149,107 +194,162 @@ __global__ void __launch_bounds__(kThreads, 2) attn_tc_kernel(AttnArgs p) {
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
 
-  if (warp < 4) {
+  if (warp < 8) {
     // ---- softmax: one row a thread ----
-    const int row = tid, r = blk * kRows + row;
+    const int tile = warp / 4, row = tid, r = blk * kRows + row;
     const bool live = r < q.rows;
-    const int pos = q.p0 + r / p.group;
+    const int tok = by_group(p, live ? r : 0), pos = q.p0 + tok;
     const int hi = live ? min(pos, end - 1) : -1, lo = p.window ? pos - p.window + 1 : 0;
-    // keys that every live row of the block sees
-    const int all_hi = min(q.p0 + blk * kRows / p.group, end - 1);
+    // keys that every live row of the tile sees
+    const int r0 = blk * kRows + tile * kTile;
+    const int all_hi = min(q.p0 + by_group(p, r0), end - 1);
     const int all_lo =
-        p.window ? q.p0 + min((blk + 1) * kRows - 1, q.rows - 1) / p.group - p.window + 1 : 0;
+        p.window ? q.p0 + by_group(p, min(r0 + kTile, q.rows) - 1) - p.window + 1 : 0;
     const float cq = s_cq[row];
-    const uint32_t trow = tmem + ((uint32_t)(32 * warp) << 16);
-    float m = -INFINITY, l = 0.0f;
-    for (int j = 0; j < n; j++) {
+    const uint32_t lanes = (uint32_t)(32 * (warp % 4)) << 16;
+    const uint32_t ts = tmem + lanes + tile * 128, to = tmem + lanes + 256 + tile * D;
+    float m = -INFINITY;
+    uint64_t l2[2] = {0, 0};  // the row's sum in four parts
+    const int steps = tile < tiles ? n : 0;
+    const bool issues = tid % kTile == 0;  // this thread issues the tile's products
+    auto scores = [&](int j) {
+      ok = ok && mbar_wait(k_full + (j & 1), j >> 1 & 1);
+      if (!ok) return;
+      tc_fence_after();
+      const uint64_t qd = (kDesc | (smem_addr(smem + L::kQ) >> 4)) +
+                          (uint64_t)(tile * (kTile * D * 2 >> 4));
+      const uint64_t kd = (kDesc | (smem_addr(smem + L::kK) >> 4)) +
+                          (uint64_t)((j & 1) * (L::kOne >> 4));
+#pragma unroll
+      for (int k = 0; k < D / 16; k++) {
+        const uint64_t at = (uint64_t)(k / 4 * (kTile * 128 >> 4) + k % 4 * 2);
+        mma_f16_ss(tmem + tile * 128, qd + at, kd + at, idesc_f16(kKeys), k > 0);
+      }
+      mma_commit(s_full + tile);
+      mma_commit(k_free + (j & 1));
+    };
+    auto outputs = [&](int j) {
+      ok = ok && mbar_wait(v_full + (j & 1), j >> 1 & 1);
+      if (!ok) return;
+      tc_fence_after();
+      const uint64_t vd = (kDesc | (smem_addr(smem + L::kV) >> 4)) +
+                          (uint64_t)((j & 1) * (L::kOne >> 4));
+#pragma unroll
+      for (int k = 0; k < kKeys / 16; k++)
+        mma_f16_ts(tmem + 256 + tile * D, tmem + tile * 128 + 8 * k,
+                   vd + (uint64_t)(k / 4 * (D * 128 >> 4) + k % 4 * 2), idesc_f16(D),
+                   j > 0 || k > 0);
+      mma_commit(v_free + (j & 1));
+    };
+    if (issues && steps > 0) {
+      if (tile == 1) ok = ok && mbar_wait(second, 0);
+      scores(0);
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int j = 0; j < steps; j++) {
       const int key = key_of(j);
-      ok = ok && mbar_wait(s_full, j & 1);
-      // the product before it was complete by then: this keeps the parity of the last wait right
-      if (j > 0) ok = ok && mbar_wait(o_full, (j - 1) & 1);
+      ok = ok && mbar_wait(s_full + tile, j & 1);
       __syncwarp();
       tc_fence_after();
       const bool masked = key + kKeys - 1 > all_hi || (key < all_lo && key + kKeys > p.sinks);
       auto seen = [&](int i) { return i <= hi && (i >= lo || i < p.sinks); };
       float top = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 4; c += 2) {
-        uint32_t s0[32], s1[32];
-        tmem_ld32_nowait(trow + 32 * c, s0);
-        tmem_ld32_nowait(trow + 32 * c + 32, s1);
+      uint32_t s[2][16];  // 16 columns ahead of those in work
+      tmem_ld16_nowait(ts, s[0]);
+#pragma unroll 2
+      for (int c = 0; c < 8; c++) {
         tmem_wait_ld();
+        tmem_ld16_nowait(ts + 16 * ((c + 1) & 7), s[(c + 1) & 1]);
         if (masked) {
 #pragma unroll
-          for (int i = 0; i < 32; i++) {
-            if (seen(key + 32 * c + i)) top = fmaxf(top, __uint_as_float(s0[i]));
-            if (seen(key + 32 * c + 32 + i)) top = fmaxf(top, __uint_as_float(s1[i]));
-          }
+          for (int i = 0; i < 16; i++)
+            if (seen(key + 16 * c + i)) top = fmaxf(top, __uint_as_float(s[c & 1][i]));
         } else {
-#pragma unroll
-          for (int i = 0; i < 32; i++)
-            top = fmaxf(top, fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i])));
+          const uint32_t(&x)[16] = s[c & 1];
+          const float a = max3(max3(x[0], x[1], x[2]), x[3], x[4]);
+          const float b = max3(max3(x[5], x[6], x[7]), x[8], x[9]);
+          const float d = max3(max3(x[10], x[11], x[12]), x[13], x[14]);
+          top = max3(max3(top, a, b), d, x[15]);
         }
       }
+      tmem_wait_ld();  // s[0] has the first columns again
       const float now = top == -INFINITY ? -INFINITY : top * cq;
       const bool grew = now > m + kStale || (m == -INFINITY && now > -INFINITY);
       if (__any_sync(0xFFFFFFFFu, grew)) {
-        // every product so far is complete: O may be read and written
+        // the tile's products so far are complete: O may be read and written
         float f = 1.0f;
         if (grew) {
           f = m == -INFINITY ? 0.0f : ex2(m - now);
           m = now;
-          l *= f;
+          const float2 a = unpack2(l2[0]), b = unpack2(l2[1]);
+          l2[0] = pack2(a.x * f, a.y * f);
+          l2[1] = pack2(b.x * f, b.y * f);
         }
         if (j > 0) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
             uint32_t o[16];
-            tmem_ld16_nowait(trow + kOCol + c, o);
+            tmem_ld16_nowait(to + c, o);
             tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st16(trow + kOCol + c, o);
+            tmem_st16(to + c, o);
           }
         }
       }
       const float base = kOffset - (m == -INFINITY ? 0.0f : m);
+      const uint64_t cq2 = pack2(cq, cq), base2 = pack2(base, base);
+      auto probabilities = [&](auto cut) {  // cut: some keys of the step are not seen by some row
+#pragma unroll 2
+        for (int c = 0; c < 8; c++) {
+          if (c > 0) tmem_wait_ld();
+          if (c < 7) tmem_ld16_nowait(ts + 16 * c + 16, s[(c + 1) & 1]);
+          uint32_t h[8];
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        uint32_t s[32], h[16];
-        tmem_ld32_nowait(trow + 32 * c, s);
-        tmem_wait_ld();
-        float e[32];
-#pragma unroll
-        for (int i = 0; i < 32; i++) e[i] = ex2(fmaf(__uint_as_float(s[i]), cq, base));
-        if (masked) {
-#pragma unroll
-          for (int i = 0; i < 32; i++)
-            if (!seen(key + 32 * c + i)) e[i] = 0.0f;
+          for (int i = 0; i < 8; i++) {
+            const float2 x = unpack2(fma2(pack2(__uint_as_float(s[c & 1][2 * i]),
+                                                __uint_as_float(s[c & 1][2 * i + 1])),
+                                          cq2, base2));
+            float e0 = ex2(x.x), e1 = ex2(x.y);
+            if (decltype(cut)::value) {
+              if (!seen(key + 16 * c + 2 * i)) e0 = 0.0f;
+              if (!seen(key + 16 * c + 2 * i + 1)) e1 = 0.0f;
+            }
+            l2[i & 1] = add2(l2[i & 1], pack2(e0, e1));
+            h[i] = h2u(__floats2half2_rn(e0, e1));
+          }
+          tmem_st8(ts + 8 * c, h);
         }
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          l += e[2 * i] + e[2 * i + 1];
-          h[i] = h2u(__floats2half2_rn(e[2 * i], e[2 * i + 1]));
-        }
-        tmem_st16(trow + 16 * c, h);
-      }
+      };
+      if (masked) probabilities(std::true_type{});
+      else probabilities(std::false_type{});
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(p_full);
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + tile), "n"(kTile) : "memory");  // the tile's threads
+      if (issues) {
+        if (j == 0 && tile == 0) mbar_arrive(second);
+        outputs(j);
+        if (j + 1 < steps) scores(j + 1);
+        else if (ok) mma_commit(o_full + tile);
+      }
+      __syncwarp();
     }
     // ---- the output rows ----
-    if (n > 0) ok = ok && mbar_wait(o_full, (n - 1) & 1);
+    if (steps > 0) ok = ok && mbar_wait(o_full + tile, 0);
     __syncwarp();
     tc_fence_after();
+    const float2 la = unpack2(l2[0]), lb = unpack2(l2[1]);
+    const float l = (la.x + la.y) + (lb.x + lb.y);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     uint16_t *dst = static_cast<uint16_t *>(p.out) +
-                    (unsigned long long)(q.first + r / p.group) * p.ldo +
-                    (unsigned long long)(head * p.group + r % p.group) * D;
+                    (unsigned long long)(q.first + tok) * p.ldo +
+                    (unsigned long long)(head * p.group + (live ? r : 0) - tok * p.group) * D;
 #pragma unroll 1
     for (int c = 0; c < D; c += 16) {
       uint32_t o[16];
-      if (n > 0) {
-        tmem_ld16_nowait(trow + kOCol + c, o);
+      if (steps > 0) {
+        tmem_ld16_nowait(to + c, o);
         tmem_wait_ld();
       } else {
 #pragma unroll
@@ -272,16 +372,18 @@ __global__ void __launch_bounds__(kThreads, 2) attn_tc_kernel(AttnArgs p) {
       }
       __syncwarp();
     }
-  } else if (warp < 8) {
-    // ---- unpacking: thread t has token t of K, and of tile t / 16 of V the dims 64 mq + 16 i + g
-    // and + 8 (four i) with all 16 tokens ----
-    const int t = tid - 128, tile = t / kKvTile, g = t % 8, mq = t / 8 % 2;
+  } else {
+    // ---- unpacking: thread t has half `part` of token t / 2 of K; and of V, in tile t / 32, dims
+    // 64 mq + 32 part + 16 i + g and + 8 (i < 2) of all 16 tokens ----
+    const int t = tid - 256, tile = t / 32;
+    const int part = t % 2, tok = t / 2 % kKvTile, g = t / 2 % 8, mq = t / 16 % 2;
     const bool has_v = D == 128 || mq == 0;
     const Unpack un;
-    constexpr int K16 = D / 32;  // 16-byte loads of a token's K
-    uint4 kraw[K16], vraw[4], vsc[4];
-    __half ksc[D / 32];
-    int page = -1, page_next = -1;
+    constexpr int K16 = D / 64;  // 16-byte loads of half a token's K
+    uint4 kraw[K16], vsc[2];
+    uint2 vraw[4];
+    __half ksc[K16];
+    int page = -1;
     const int *table = p.table + (size_t)seq * p.max_pages;
     auto find = [&](int j) {  // the page of this thread's tile at step j
       const int key = key_of(j) + tile * kKvTile;
@@ -300,66 +402,69 @@ __global__ void __launch_bounds__(kThreads, 2) attn_tc_kernel(AttnArgs p) {
       if (page < 0) return;
       const uint8_t *src = source(j, page);
 #pragma unroll
-      for (int i = 0; i < K16; i++)
-        kraw[i] = __ldg(reinterpret_cast<const uint4 *>(src + t % kKvTile * (D / 2)) + i);
-#pragma unroll
-      for (int i = 0; i < D / 32; i++)
-        ksc[i] = __ldg(reinterpret_cast<const __half *>(src + kv4_ks_off(D)) + i * kKvTile +
-                       t % kKvTile);
+      for (int i = 0; i < K16; i++) {
+        kraw[i] = __ldg(reinterpret_cast<const uint4 *>(src + tok * (D / 2) + part * (D / 4)) + i);
+        ksc[i] = __ldg(reinterpret_cast<const __half *>(src + kv4_ks_off(D)) +
+                       (part * K16 + i) * kKvTile + tok);
+      }
     };
     auto load_v = [&](int j) {
       if (page < 0 || !has_v) return;
       const uint8_t *src = source(j, page);
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        vraw[i] = __ldg(reinterpret_cast<const uint4 *>(src + kv4_v_off(D)) + mq * 32 + g * 4 + i);
+        vraw[i] = __ldg(reinterpret_cast<const uint2 *>(src + kv4_v_off(D)) +
+                        (mq * 32 + g * 4 + i) * 2 + part);
 #pragma unroll
-      for (int i = 0; i < 4; i++)  // two groups of 32 dims, 16 tokens each
-        vsc[i] = __ldg(reinterpret_cast<const uint4 *>(src + kv4_vs_off(D)) + mq * 4 + i);
+      for (int i = 0; i < 2; i++)  // a group of 32 dims, 16 tokens
+        vsc[i] = __ldg(reinterpret_cast<const uint4 *>(src + kv4_vs_off(D)) +
+                       (mq * 2 + part) * 2 + i);
     };
     page = find(0);
     load_k(0);
     load_v(0);
+#pragma unroll 1
     for (int j = 0; j < n; j++) {
-      const int key = key_of(j);
-      page_next = find(j + 1);
-      if (j > 0) ok = ok && mbar_wait(s_full, (j - 1) & 1);  // K's last readers are done
+      const int key = key_of(j), buf = j & 1;
+      const int page_now = page, page_next = find(j + 1);
+      if (j > 1) ok = ok && mbar_wait(k_free + buf, ((j >> 1) - 1) & 1);
       {
-        const bool have = page >= 0 && key + t < end;
+        const bool have = page_now >= 0 && key + tile * kKvTile + tok < end;
+        uint8_t *dst = smem + L::kK + buf * L::kOne;
+        const int row = tile * kKvTile + tok;
 #pragma unroll
         for (int i = 0; i < K16; i++) {
           const uint32_t w[4] = {kraw[i].x, kraw[i].y, kraw[i].z, kraw[i].w};
           const __half2 sc = __half2half2(ksc[i]);  // 32 dims: one group
 #pragma unroll
           for (int c = 0; c < 4; c++) {
-            const int chunk = 4 * i + c;
+            const int chunk = part * (D / 16) + 4 * i + c;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (have)
               v = make_uint4(un.low2(w[c], sc), un.high2(w[c], sc), un.low2(w[c] >> 8, sc),
                              un.high2(w[c] >> 8, sc));
-            *reinterpret_cast<uint4 *>(smem + L::kK + chunk / 8 * (kKeys * 128) +
-                                       swizzled(t, chunk % 8)) = v;
+            *reinterpret_cast<uint4 *>(dst + chunk / 8 * (kKeys * 128) +
+                                       swizzled(row, chunk % 8)) = v;
           }
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(k_full);
-      const int page_now = page;
+      mbar_arrive(k_full + buf);
       page = page_next;
       load_k(j + 1);
-      if (j > 0) ok = ok && mbar_wait(o_full, (j - 1) & 1);  // V's last readers are done
+      if (j > 1) ok = ok && mbar_wait(v_free + buf, ((j >> 1) - 1) & 1);
       if (has_v) {
         const int first = key + tile * kKvTile;
         const bool have = page_now >= 0;
+        uint8_t *dst = smem + L::kV + buf * L::kOne;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {  // dims 64 mq + 16 i + g and + 8
+        for (int i = 0; i < 2; i++) {  // dims 64 mq + 32 part + 16 i + g and + 8
           uint32_t a[2][8];            // dim; tokens 2 k and 2 k + 1
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            const uint32_t w = i == 0 ? vraw[k].x : i == 1 ? vraw[k].y : i == 2 ? vraw[k].z : vraw[k].w;
-            const uint4 lo4 = vsc[i / 2 * 2], hi4 = vsc[i / 2 * 2 + 1];
-            const uint32_t s0 = k == 0 ? lo4.x : k == 1 ? lo4.y : k == 2 ? lo4.z : lo4.w;
-            const uint32_t s1 = k == 0 ? hi4.x : k == 1 ? hi4.y : k == 2 ? hi4.z : hi4.w;
+            const uint32_t w = i == 0 ? vraw[k].x : vraw[k].y;
+            const uint32_t s0 = k == 0 ? vsc[0].x : k == 1 ? vsc[0].y : k == 2 ? vsc[0].z : vsc[0].w;
+            const uint32_t s1 = k == 0 ? vsc[1].x : k == 1 ? vsc[1].y : k == 2 ? vsc[1].z : vsc[1].w;
             a[0][k] = un.low2(w, u2h(s0));
             a[1][k] = un.high2(w, u2h(s0));
             a[0][4 + k] = un.low2(w >> 8, u2h(s1));
@@ -376,50 +481,25 @@ __global__ void __launch_bounds__(kThreads, 2) attn_tc_kernel(AttnArgs p) {
           }
 #pragma unroll
           for (int h = 0; h < 2; h++) {
-            const int d = 64 * mq + 16 * i + g + 8 * h;
+            const int d = 64 * mq + 32 * part + 16 * i + g + 8 * h;
 #pragma unroll
             for (int k = 0; k < 2; k++) {  // tokens 8 k .. 8 k + 7 of the tile
               const int chunk = tile * 2 + k;
-              *reinterpret_cast<uint4 *>(smem + L::kV + chunk / 8 * (D * 128) +
-                                         swizzled(d, chunk % 8)) =
+              *reinterpret_cast<uint4 *>(dst + chunk / 8 * (D * 128) + swizzled(d, chunk % 8)) =
                   make_uint4(a[h][4 * k], a[h][4 * k + 1], a[h][4 * k + 2], a[h][4 * k + 3]);
             }
           }
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(v_full);
+      mbar_arrive(v_full + buf);
       load_v(j + 1);
-    }
-  } else if (lane == 0) {
-    // ---- the products ----
-    const uint64_t qd = kDesc | (smem_addr(smem + L::kQ) >> 4);
-    const uint64_t kd = kDesc | (smem_addr(smem + L::kK) >> 4);
-    const uint64_t vd = kDesc | (smem_addr(smem + L::kV) >> 4);
-    for (int j = 0; ok && j < n; j++) {
-      ok = ok && mbar_wait(k_full, j & 1);
-      if (!ok) break;
-      tc_fence_after();
-#pragma unroll
-      for (int k = 0; k < D / 16; k++) {
-        const uint64_t at = (uint64_t)(k / 4 * (kRows * 128 >> 4) + k % 4 * 2);
-        mma_f16_ss(tmem, qd + at, kd + at, idesc_f16(kKeys), k > 0);
-      }
-      mma_commit(s_full);
-      ok = ok && mbar_wait(v_full, j & 1) && mbar_wait(p_full, j & 1);
-      if (!ok) break;
-      tc_fence_after();
-#pragma unroll
-      for (int k = 0; k < kKeys / 16; k++)
-        mma_f16_ts(tmem + kOCol, tmem + 8 * k, vd + (uint64_t)(k / 4 * (D * 128 >> 4) + k % 4 * 2),
-                   idesc_f16(D), j > 0 || k > 0);
-      mma_commit(o_full);
     }
   }
   if (!ok) attn_refuse(p, seq, APX_ERR_DEVICE_TIMEOUT);
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 15) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(kTmemCols)
