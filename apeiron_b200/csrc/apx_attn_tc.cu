@@ -3,7 +3,7 @@
 //
 // A CTA holds two tiles of 128 query rows of one KV head (a token's group of heads are neighbouring
 // rows) and takes its keys 128 at a time: S = Q K^T into TMEM, four softmax warps a tile turn S
-// into probabilities in place (f16), O += P V with P read from TMEM.  A tile's first softmax thread
+// into probabilities in place (f16), O += P V with P read from TMEM.  A tile's first softmax warp
 // issues its products.  The second tile starts a softmax later: while one is in its softmax the
 // other's products run.  Both read the same keys and values, which eight warps unpack from the
 // cache's pages to f16 operands in shared memory (exact: d (c - 8) fits f16), two buffers each,
@@ -21,8 +21,6 @@
 // the same.
 #include <cuda_bf16.h>
 
-#include <type_traits>
-
 #include "apx_common.cuh"
 #include "apx_kernels.h"
 #include "apx_kv4.cuh"
@@ -36,7 +34,12 @@ namespace {
 constexpr int kTile = 128, kRows = 2 * kTile, kKeys = 128;
 constexpr int kThreads = 512;     // 8 softmax warps, 8 unpacking warps
 constexpr int kUnpack = 256;      // unpacking threads
+// Registers of a softmax and of an unpacking thread: together what the CTA is launched with (128 a
+// thread, the launch bounds' limit, which the build's resource table shows).
+constexpr int kSoftmaxRegs = 176, kUnpackRegs = 80;
+static_assert((kSoftmaxRegs + kUnpackRegs) * 256 <= 128 * kThreads, "the launch's registers");
 constexpr float kStale = 8.0f;    // log2 of how far a row's maximum may outgrow the stale one
+constexpr float kUnseen = -1e30f;  // an unseen key's score
 constexpr float kOffset = 6.0f;   // probabilities are held at 2^6 e^(s - m)
 constexpr int kTmemCols = 512;    // S (then P) of the tiles in columns 0-255, O from 256 on
 
@@ -107,7 +110,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t *second = bars + 12;                      // the second tile may start
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 13);
   float *s_cq = reinterpret_cast<float *>(smem + L::kCq);
-  const int tid = threadIdx.x, warp = tid / 32;
+  const int tid = threadIdx.x;
+  const int warp = __shfl_sync(0xFFFFFFFFu, tid / 32, 0);  // the same in every lane, and known to be
   const int seq = blockIdx.x / p.kv_heads, head = blockIdx.x % p.kv_heads;
 
   pdl_launch_dependents();
@@ -195,7 +199,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool ok = true;
 
   if (warp < 8) {
-    // ---- softmax: one row a thread ----
+    // ---- softmax: one row a thread, its 128 scores in registers ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int tile = warp / 4, row = tid, r = blk * kRows + row;
     const bool live = r < q.rows;
     const int tok = by_group(p, live ? r : 0), pos = q.p0 + tok;
@@ -205,16 +210,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int all_hi = min(q.p0 + by_group(p, r0), end - 1);
     const int all_lo =
         p.window ? q.p0 + by_group(p, min(r0 + kTile, q.rows) - 1) - p.window + 1 : 0;
-    const float cq = s_cq[row];
+    // below 1e-20 no score (they stay below 2^34) tells; at it an unseen one still counts as none
+    const float cq = fmaxf(s_cq[row], 1e-20f);
     const uint32_t lanes = (uint32_t)(32 * (warp % 4)) << 16;
     const uint32_t ts = tmem + lanes + tile * 128, to = tmem + lanes + 256 + tile * D;
     float m = -INFINITY;
     uint64_t l2[2] = {0, 0};  // the row's sum in four parts
     const int steps = tile < tiles ? n : 0;
-    const bool issues = tid % kTile == 0;  // this thread issues the tile's products
+    const bool issues = warp % 4 == 0;  // this warp issues the tile's products
+    const uint32_t leader = elect_leader();
     auto scores = [&](int j) {
       ok = ok && mbar_wait(k_full + (j & 1), j >> 1 & 1);
-      if (!ok) return;
+      if (!__all_sync(0xFFFFFFFFu, ok)) return;
       tc_fence_after();
       const uint64_t qd = (kDesc | (smem_addr(smem + L::kQ) >> 4)) +
                           (uint64_t)(tile * (kTile * D * 2 >> 4));
@@ -223,23 +230,27 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int k = 0; k < D / 16; k++) {
         const uint64_t at = (uint64_t)(k / 4 * (kTile * 128 >> 4) + k % 4 * 2);
-        mma_f16_ss(tmem + tile * 128, qd + at, kd + at, idesc_f16(kKeys), k > 0);
+        mma_f16_ss(leader, tmem + tile * 128, qd + at, kd + at, idesc_f16(kKeys), k > 0);
       }
-      mma_commit(s_full + tile);
-      mma_commit(k_free + (j & 1));
+      if (leader) {
+        mma_commit(s_full + tile);
+        mma_commit(k_free + (j & 1));
+      }
+      __syncwarp();
     };
     auto outputs = [&](int j) {
       ok = ok && mbar_wait(v_full + (j & 1), j >> 1 & 1);
-      if (!ok) return;
+      if (!__all_sync(0xFFFFFFFFu, ok)) return;
       tc_fence_after();
       const uint64_t vd = (kDesc | (smem_addr(smem + L::kV) >> 4)) +
                           (uint64_t)((j & 1) * (L::kOne >> 4));
 #pragma unroll
       for (int k = 0; k < kKeys / 16; k++)
-        mma_f16_ts(tmem + 256 + tile * D, tmem + tile * 128 + 8 * k,
+        mma_f16_ts(leader, tmem + 256 + tile * D, tmem + tile * 128 + 8 * k,
                    vd + (uint64_t)(k / 4 * (D * 128 >> 4) + k % 4 * 2), idesc_f16(D),
                    j > 0 || k > 0);
-      mma_commit(v_free + (j & 1));
+      if (leader) mma_commit(v_free + (j & 1));
+      __syncwarp();
     };
     if (issues && steps > 0) {
       if (tile == 1) ok = ok && mbar_wait(second, 0);
@@ -253,28 +264,31 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       tc_fence_after();
       const bool masked = key + kKeys - 1 > all_hi || (key < all_lo && key + kKeys > p.sinks);
-      auto seen = [&](int i) { return i <= hi && (i >= lo || i < p.sinks); };
-      float top = -INFINITY;
-      uint32_t s[2][16];  // 16 columns ahead of those in work
-      tmem_ld16_nowait(ts, s[0]);
-#pragma unroll 2
-      for (int c = 0; c < 8; c++) {
-        tmem_wait_ld();
-        tmem_ld16_nowait(ts + 16 * ((c + 1) & 7), s[(c + 1) & 1]);
-        if (masked) {
+      uint32_t s[4][32];  // the row's scores
 #pragma unroll
-          for (int i = 0; i < 16; i++)
-            if (seen(key + 16 * c + i)) top = fmaxf(top, __uint_as_float(s[c & 1][i]));
-        } else {
-          const uint32_t(&x)[16] = s[c & 1];
-          const float a = max3(max3(x[0], x[1], x[2]), x[3], x[4]);
-          const float b = max3(max3(x[5], x[6], x[7]), x[8], x[9]);
-          const float d = max3(max3(x[10], x[11], x[12]), x[13], x[14]);
-          top = max3(max3(top, a, b), d, x[15]);
+      for (int c = 0; c < 4; c++) tmem_ld32_nowait(ts + 32 * c, s[c]);
+      tmem_wait_ld();
+      if (masked) {  // unseen keys' scores to where they cost the exponential nothing
+        auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const int k0 = key + 32 * c;
+          const uint32_t bits = below(hi + 1 - k0) & (~below(lo - k0) | below(p.sinks - k0));
+#pragma unroll
+          for (int i = 0; i < 32; i++)
+            if (!(bits >> i & 1)) s[c][i] = __float_as_uint(kUnseen);
         }
       }
-      tmem_wait_ld();  // s[0] has the first columns again
-      const float now = top == -INFINITY ? -INFINITY : top * cq;
+      float t4[4];
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        t4[c] = max3(s[c][0], s[c][1], s[c][2]);
+#pragma unroll
+        for (int i = 3; i < 31; i += 2) t4[c] = max3(t4[c], s[c][i], s[c][i + 1]);
+        t4[c] = fmaxf(t4[c], __uint_as_float(s[c][31]));
+      }
+      const float top = fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]);
+      const float now = top <= kUnseen ? -INFINITY : top * cq;
       const bool grew = now > m + kStale || (m == -INFINITY && now > -INFINITY);
       if (__any_sync(0xFFFFFFFFu, grew)) {
         // the tile's products so far are complete: O may be read and written
@@ -300,38 +314,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float base = kOffset - (m == -INFINITY ? 0.0f : m);
       const uint64_t cq2 = pack2(cq, cq), base2 = pack2(base, base);
-      auto probabilities = [&](auto cut) {  // cut: some keys of the step are not seen by some row
-#pragma unroll 2
-        for (int c = 0; c < 8; c++) {
-          if (c > 0) tmem_wait_ld();
-          if (c < 7) tmem_ld16_nowait(ts + 16 * c + 16, s[(c + 1) & 1]);
-          uint32_t h[8];
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const float2 x = unpack2(fma2(pack2(__uint_as_float(s[c & 1][2 * i]),
-                                                __uint_as_float(s[c & 1][2 * i + 1])),
-                                          cq2, base2));
-            float e0 = ex2(x.x), e1 = ex2(x.y);
-            if (decltype(cut)::value) {
-              if (!seen(key + 16 * c + 2 * i)) e0 = 0.0f;
-              if (!seen(key + 16 * c + 2 * i + 1)) e1 = 0.0f;
-            }
-            l2[i & 1] = add2(l2[i & 1], pack2(e0, e1));
-            h[i] = h2u(__floats2half2_rn(e0, e1));
-          }
-          tmem_st8(ts + 8 * c, h);
+      for (int c = 0; c < 4; c++) {
+        uint32_t h[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float2 x = unpack2(fma2(pack2(__uint_as_float(s[c][2 * i]),
+                                              __uint_as_float(s[c][2 * i + 1])),
+                                        cq2, base2));
+          const float e0 = ex2(x.x), e1 = ex2(x.y);
+          l2[i & 1] = add2(l2[i & 1], pack2(e0, e1));
+          h[i] = h2u(__floats2half2_rn(e0, e1));
         }
-      };
-      if (masked) probabilities(std::true_type{});
-      else probabilities(std::false_type{});
+        tmem_st16(ts + 16 * c, h);
+      }
       tmem_wait_st();
       tc_fence_before();
       asm volatile("bar.sync %0, %1;" ::"r"(1 + tile), "n"(kTile) : "memory");  // the tile's threads
       if (issues) {
-        if (j == 0 && tile == 0) mbar_arrive(second);
+        if (j == 0 && tile == 0 && leader) mbar_arrive(second);
         outputs(j);
         if (j + 1 < steps) scores(j + 1);
-        else if (ok) mma_commit(o_full + tile);
+        else if (leader && ok) mma_commit(o_full + tile);
       }
       __syncwarp();
     }
@@ -373,10 +377,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
     }
   } else {
-    // ---- unpacking: thread t has half `part` of token t / 2 of K; and of V, in tile t / 32, dims
-    // 64 mq + 32 part + 16 i + g and + 8 (i < 2) of all 16 tokens ----
+    // ---- unpacking: a warp has 16 keys, a thread half `part` of one's K; and of V dims
+    // 64 mq + 32 part + 16 i + g and + 8 (i < 2) of all 16.  Neighbours have rows of different
+    // swizzle: their stores meet no bank twice ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnpackRegs));
     const int t = tid - 256, tile = t / 32;
-    const int part = t % 2, tok = t / 2 % kKvTile, g = t / 2 % 8, mq = t / 16 % 2;
+    const int tok = t % kKvTile, g = t % 8, mq = t / 8 % 2, part = t / 16 % 2;
     const bool has_v = D == 128 || mq == 0;
     const Unpack un;
     constexpr int K16 = D / 64;  // 16-byte loads of half a token's K
