@@ -2,87 +2,177 @@
 // output and the next projection's 8-bit activation, in one pass over the row.
 //
 // h = x + add; r = 1 / sqrt(sum h^2 / n + eps); y = h r w; then quant_act of y per 32 lanes
-// (apx_quant.cuh: the same codes as apx_quant_f32_cols_async of y).  The square sum and the
-// product h r w are carried in f64 and rounded once: a code changes only where y itself lies
-// within half an f32 rounding of a code's boundary.
+// (apx_quant.cuh: the same codes as apx_quant_f32_cols_async of y).  A code is one step off where y
+// is off by less than its last bit, so y is formed from more bits than it has: the squares' sum and
+// the products carry a second f32 with the roundings' rest, r is f64, and y is rounded once.
+//
+// A CTA has a row, each thread four lanes (a quad) of every turn of the CTA over it; the row stays
+// in registers between its sum and its quantization; rows past 16384 are read again.
+//
+// What bounds it: for many rows the bytes, 4 n read (8 n and 4 n written with a residual) and
+// 1 + 1/32 n written; for one row the chain load, sum over the CTA, root, quantize, store.
 #include <cuda_bf16.h>
+
+#include <algorithm>
 
 #include "apx_common.cuh"
 #include "apx_kernels.h"
+#include "apx_pack.cuh"
 #include "apx_quant.cuh"
 #include "apx_step.h"
 
 namespace apx {
 
-struct NormDesc {
+namespace {
+
+struct Stat {
+  double sum;
   int emin, emax, status;
   unsigned nz;
 };
 
-// One CTA per row, a quad of lanes per thread and turn.
-__global__ void __launch_bounds__(256) norm_quant_kernel(apx_norm_args a, size_t padded) {
-  __shared__ double s_sum[8];
-  __shared__ NormDesc s_d;
+__device__ __forceinline__ float4 load4(const float *p, size_t j, size_t n, bool quads) {
+  if (quads && j + 4 <= n) return *reinterpret_cast<const float4 *>(p + j);
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (j < n) v.x = p[j];
+  if (j + 1 < n) v.y = p[j + 1];
+  if (j + 2 < n) v.z = p[j + 2];
+  if (j + 3 < n) v.w = p[j + 3];
+  return v;
+}
+
+__device__ __forceinline__ void store4f(float *p, size_t j, size_t n, bool quads, const float4 v) {
+  if (quads && j + 4 <= n) {
+    *reinterpret_cast<float4 *>(p + j) = v;
+    return;
+  }
+  if (j < n) p[j] = v.x;
+  if (j + 1 < n) p[j + 1] = v.y;
+  if (j + 2 < n) p[j + 2] = v.z;
+  if (j + 3 < n) p[j + 3] = v.w;
+}
+
+// (s, c) += h^2, c the rest of every rounding.
+__device__ __forceinline__ void add_square(float &s, float &c, float h) {
+  const float p = __fmul_rn(h, h), e = __fmaf_rn(h, h, -p);
+  const float t = __fadd_rn(s, p), b = __fsub_rn(t, s);
+  c += (__fsub_rn(s, __fsub_rn(t, b)) + __fsub_rn(p, b)) + e;
+  s = t;
+}
+
+// h w r rounded once, r = rh + rl.  Where a rest would underflow the plain product is as near.
+__device__ __forceinline__ float scaled(float h, float w, float rh, float rl) {
+  const float p = __fmul_rn(h, w), e = __fmaf_rn(h, w, -p);
+  const float t = __fmul_rn(p, rh), f = __fmaf_rn(p, rh, -t);
+  const float y = __fadd_rn(t, __fmaf_rn(e, rh, __fmaf_rn(p, rl, f)));
+  return fabsf(t) < 1e38f ? y : t;  // an infinite product has no rest
+}
+
+// QUADS: quads of the row in registers; 0 reads it twice.
+template <int QUADS, int THREADS>
+__global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_constant__ apx_norm_args a,
+                                                             size_t padded, int vec) {
+  constexpr int W = THREADS / 32;
+  __shared__ double s_sum[W];
+  __shared__ Stat s_stat[W];
   const size_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const float *x = a.d_x + row * a.ldx;
   const float *add = a.d_add ? a.d_add + row * a.ld_add : nullptr;
-  if (tid == 0) s_d = NormDesc{1 << 30, -1, APX_OK, 0u};
+  const bool vx = vec & 1, va = vec & 2, vr = vec & 4, vy = vec & 8, vw = vec & 16, vd = vec & 32;
+  pdl_launch_dependents();
+  // the weights do not depend on the kernel before
+  constexpr int N = QUADS ? QUADS : 1;
+  float4 h[N], w[N];
+  const float4 one = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+#pragma unroll
+  for (int i = 0; i < N; i++)
+    if (QUADS) w[i] = a.d_weight ? load4(a.d_weight, 4 * (size_t)(i * THREADS + tid), a.n, vw) : one;
+  pdl_wait();
   auto value = [&](size_t j) {
-    return j < a.n ? (add ? __fadd_rn(x[j], add[j]) : x[j]) : 0.0f;
+    float4 v = load4(x, j, a.n, vx);
+    if (add) {
+      const float4 b = load4(add, j, a.n, va);
+      v = make_float4(__fadd_rn(v.x, b.x), __fadd_rn(v.y, b.y), __fadd_rn(v.z, b.z),
+                      __fadd_rn(v.w, b.w));
+    }
+    return v;
   };
-  double sum = 0.0;
-  for (size_t j = tid; j < a.n; j += blockDim.x) {
-    const double h = value(j);
-    sum += h * h;
+  float s = 0.0f, c = 0.0f;
+  auto square = [&](const float4 v) {
+    add_square(s, c, v.x);
+    add_square(s, c, v.y);
+    add_square(s, c, v.z);
+    add_square(s, c, v.w);
+  };
+  if (QUADS) {
+#pragma unroll
+    for (int i = 0; i < N; i++) h[i] = value(4 * (size_t)(i * THREADS + tid));
+#pragma unroll
+    for (int i = 0; i < N; i++) square(h[i]);
+  } else {
+    for (size_t j = 4 * (size_t)tid; j < a.n; j += 4 * THREADS) square(value(j));
   }
+  // squares near f32's ends (or a value that is not finite) leave no rest: the sum in f64
+  double sum = (double)s + (double)c;
+  if (!(s > 1e-25f && s < 3e38f)) {
+    sum = 0.0;
+    for (size_t j = 4 * (size_t)tid; j < a.n; j += 4 * THREADS) {
+      const float4 v = value(j);
+      sum += (double)v.x * v.x + (double)v.y * v.y + (double)v.z * v.z + (double)v.w * v.w;
+    }
+  }
+#pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  if (lane == 0) s_sum[warp] = sum;
-  __syncthreads();
-  sum = 0.0;
-  for (int i = 0; i < 8; i++) sum += s_sum[i];
+  if (W > 1) {
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    sum = lane < W ? s_sum[lane] : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  }
   const double r = 1.0 / sqrt(sum / (double)a.n + (double)a.eps);
+  const float rh = (float)r, rl = fabsf(rh) < 3e38f ? (float)(r - (double)rh) : 0.0f;
+
   int emin = 1 << 30, emax = -1, status = APX_OK;
   unsigned nz = 0;
-  const size_t end = (padded + 1023) / 1024 * 1024;
-  for (size_t j = 4 * (size_t)tid; j < end; j += 4 * blockDim.x) {
-    float h[4], y[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      h[i] = value(j + i);
-      const double w = a.d_weight && j + i < a.n ? (double)a.d_weight[j + i] : 1.0;
-      y[i] = (float)((double)h[i] * w * r);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (j + i < a.n) {
-        if (a.d_resid) a.d_resid[row * a.ld_resid + j + i] = h[i];
-        if (a.d_y) a.d_y[row * a.ldy + j + i] = y[i];
-      }
+  auto quad = [&](size_t j, const float4 v, const float4 g) {
+    const float4 y = make_float4(scaled(v.x, g.x, rh, rl), scaled(v.y, g.y, rh, rl),
+                                 scaled(v.z, g.z, rh, rl), scaled(v.w, g.w, rh, rl));
+    if (a.d_resid) store4f(a.d_resid + row * a.ld_resid, j, a.n, vr, v);
+    if (a.d_y) store4f(a.d_y + row * a.ldy, j, a.n, vy, y);
+    if (!a.d_codes && !a.d_deq) return;
     uint32_t packed;
     int e;
     bool ok;
-    quant_quad(make_float4(y[0], y[1], y[2], y[3]), packed, e, ok);
+    quant_quad(y, packed, e, ok);
     if (!ok || e < 0) packed = 0;
-    if (a.d_codes) {
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (j + i < padded) a.d_codes[row * padded + j + i] = (int8_t)(packed >> (8 * i));
-    }
+    if (a.d_codes && j < padded)
+      *reinterpret_cast<uint32_t *>(a.d_codes + row * padded + j) = packed;
     if (a.d_deq) {
-      const float s = ok && e >= 0 ? __int_as_float((127 + e - 32) << 23) : 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (j + i < a.n) {
-          const float v = s * (float)(int8_t)(packed >> (8 * i));
-          if (a.deq_type == APX_DTYPE_F32)
-            static_cast<float *>(a.d_deq)[row * a.ld_deq + j + i] = v;
-          else
-            static_cast<__nv_bfloat16 *>(a.d_deq)[row * a.ld_deq + j + i] = __float2bfloat16(v);
+      const float q = ok && e >= 0 ? __int_as_float((127 + e - 32) << 23) : 0.0f;
+      const float4 d = make_float4(q * (float)(int8_t)packed, q * (float)(int8_t)(packed >> 8),
+                                   q * (float)(int8_t)(packed >> 16),
+                                   q * (float)(int8_t)(packed >> 24));
+      if (a.deq_type == APX_DTYPE_F32) {
+        store4f(static_cast<float *>(a.d_deq) + row * a.ld_deq, j, a.n, vd, d);
+      } else {
+        __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.d_deq) + row * a.ld_deq + j;
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(d.x, d.y), hi = __floats2bfloat162_rn(d.z, d.w);
+        if (vd && j + 4 <= a.n) {
+          *reinterpret_cast<uint2 *>(dst) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo),
+                                                       *reinterpret_cast<const uint32_t *>(&hi));
+        } else {
+          if (j < a.n) dst[0] = lo.x;
+          if (j + 1 < a.n) dst[1] = lo.y;
+          if (j + 2 < a.n) dst[2] = hi.x;
+          if (j + 3 < a.n) dst[3] = hi.y;
         }
+      }
     }
     if ((lane & 7) == 0 && j < padded) {
-      if (a.d_exps) a.d_exps[(row * padded + j) / 32] = e < 0 || !ok ? APX_EXP_ZERO : (uint8_t)e;
+      if (a.d_exps)
+        a.d_exps[(row * padded + j) / 32] = e < 0 || !ok ? (uint8_t)APX_EXP_ZERO : (uint8_t)e;
       if (j < a.n) {
         if (!ok) {
           status = APX_ERR_QUANT_REFUSED;
@@ -93,29 +183,83 @@ __global__ void __launch_bounds__(256) norm_quant_kernel(apx_norm_args a, size_t
         }
       }
     }
+  };
+  if (QUADS) {
+#pragma unroll
+    for (int i = 0; i < N; i++) quad(4 * (size_t)(i * THREADS + tid), h[i], w[i]);
+  } else {
+    // whole warps: quant_quad's shuffles take every lane
+    const size_t end = (padded + 4 * THREADS - 1) / (4 * THREADS) * (4 * THREADS);
+    for (size_t j = 4 * (size_t)tid; j < end; j += 4 * THREADS)
+      quad(j, value(j), a.d_weight ? load4(a.d_weight, j, a.n, vw) : one);
   }
   if (!a.d_descs) return;
-  if (status != APX_OK) atomicMax(&s_d.status, status);
-  if (nz) {
-    atomicMin(&s_d.emin, emin);
-    atomicMax(&s_d.emax, emax);
-    atomicAdd(&s_d.nz, nz);
+  emin = __reduce_min_sync(0xFFFFFFFFu, emin);
+  emax = __reduce_max_sync(0xFFFFFFFFu, emax);
+  status = __reduce_max_sync(0xFFFFFFFFu, status);
+  nz = __reduce_add_sync(0xFFFFFFFFu, nz);
+  if (W > 1) {
+    if (lane == 0) s_stat[warp] = Stat{0.0, emin, emax, status, nz};
+    __syncthreads();
+    if (warp == 0) {
+      const Stat t = s_stat[lane % W];
+      emin = __reduce_min_sync(0xFFFFFFFFu, t.emin);
+      emax = __reduce_max_sync(0xFFFFFFFFu, t.emax);
+      status = __reduce_max_sync(0xFFFFFFFFu, t.status);
+      nz = __reduce_add_sync(0xFFFFFFFFu, lane < W ? t.nz : 0u);
+    }
   }
-  __syncthreads();
   if (tid == 0) {
     ActDesc d = {};
-    d.status = s_d.status;
-    d.emin = s_d.emax >= 0 ? s_d.emin : 0;
-    d.emax = s_d.emax;
+    d.status = status;
+    d.emin = emax >= 0 ? emin : 0;
+    d.emax = emax;
     d.n_in = (int32_t)a.n;
-    d.nz = s_d.nz;
+    d.nz = nz;
     reinterpret_cast<ActDesc *>(a.d_descs)[row] = d;
   }
 }
 
+template <int QUADS, int THREADS>
+cudaError_t launch(const apx_norm_args &a, size_t padded, int vec, cudaStream_t stream) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.k);
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_allowed() ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, norm_quant_kernel<QUADS, THREADS>, a, padded, vec);
+}
+
+}  // namespace
+
 cudaError_t launch_add_rms_norm_quant(const apx_norm_args &a, cudaStream_t stream) {
-  norm_quant_kernel<<<(unsigned)a.k, 256, 0, stream>>>(a, apx_act_padded_len(a.n));
-  return cudaGetLastError();
+  const size_t padded = apx_act_padded_len(a.n);
+  // which arrays have 16-byte (the 16-bit values: 8-byte) aligned rows
+  auto whole = [](const void *p, size_t ld, size_t bytes) {
+    return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0 && ld % 4 == 0;
+  };
+  int vec = 0;
+  if (whole(a.d_x, a.ldx, 16)) vec |= 1;
+  if (whole(a.d_add, a.ld_add, 16)) vec |= 2;
+  if (whole(a.d_resid, a.ld_resid, 16)) vec |= 4;
+  if (whole(a.d_y, a.ldy, 16)) vec |= 8;
+  if (whole(a.d_weight, 0, 16)) vec |= 16;
+  if (whole(a.d_deq, a.ld_deq, a.deq_type == APX_DTYPE_F32 ? 16 : 8)) vec |= 32;
+  const size_t quads = padded / 4;  // padded is what has to be written
+  // Few rows: as many threads as the row has quads, the loads of a row one round trip.  Many rows
+  // fill the GPU with smaller CTAs of more quads a thread.
+  if (quads <= 256) return launch<1, 256>(a, padded, vec, stream);
+  if (a.k <= 148 && quads <= 1024) return launch<1, 1024>(a, padded, vec, stream);
+  if (a.k <= 148 && quads <= 2048) return launch<2, 1024>(a, padded, vec, stream);
+  if (quads <= 512) return launch<2, 256>(a, padded, vec, stream);
+  if (quads <= 1024) return launch<4, 256>(a, padded, vec, stream);
+  if (quads <= 2048) return launch<4, 512>(a, padded, vec, stream);
+  if (quads <= 4096) return launch<4, 1024>(a, padded, vec, stream);
+  return launch<0, 1024>(a, padded, vec, stream);
 }
 
 }  // namespace apx

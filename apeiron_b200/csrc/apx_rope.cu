@@ -8,7 +8,9 @@
 #include <cuda_fp16.h>
 
 #include "apx_common.cuh"
+#include "apx_kernels.h"
 #include "apx_kv4.cuh"
+#include "apx_pack.cuh"
 #include "apx_step.h"
 
 namespace apx {
@@ -112,9 +114,11 @@ __device__ __forceinline__ uint2 pack4(const float4 v, bool bf16) {
 }
 
 // One token per CTA; dim / 4 threads take a head (query heads, then K heads, then V heads).
-__global__ void __launch_bounds__(256) rope_append_kernel(RopeArgs r) {
+__global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant__ RopeArgs r) {
   const apx_rope_args &a = r.a;
   const int t = blockIdx.x, per = r.dim / 4;
+  pdl_launch_dependents();
+  pdl_wait();
   const int seq = find_seq(r.cu, r.n_seqs, t);
   const int pos = r.kv_len[seq] - r.cu[seq + 1] + t;
   const int slot = pos / r.page_tokens;
@@ -220,8 +224,16 @@ cudaError_t launch_rope_kv4_append(const apx_rope_args &a, const apx_kv4_cache &
   r.kv_heads = c.n_kv_heads;
   r.dim = c.head_dim;
   r.page_tokens = c.page_tokens;
-  rope_append_kernel<<<(unsigned)b.n_tokens, 256, 0, stream>>>(r);
-  return cudaGetLastError();
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)b.n_tokens);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_allowed() ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, rope_append_kernel, r);
 }
 
 }  // namespace apx

@@ -48,7 +48,8 @@ int apx_add_rms_norm_quant_async(apx_ctx *ctx, const apx_norm_args *a, void *str
       (a->d_resid && a->ld_resid < a->n) || (a->d_y && a->ldy < a->n) ||
       (a->d_deq && (a->ld_deq < a->n || (a->deq_type != APX_DTYPE_F32 &&
                                          a->deq_type != APX_DTYPE_BF16))) ||
-      (any && !(a->d_codes && a->d_exps && a->d_descs)) || !(a->eps >= 0.0f))
+      (any && !(a->d_codes && a->d_exps && a->d_descs)) || !aligned(a->d_codes, 4) ||
+      !aligned(a->d_descs, 16) || !(a->eps >= 0.0f))
     return APX_ERR_INVALID_ARGUMENT;
   return apx::launch_add_rms_norm_quant(*a, (cudaStream_t)stream) == cudaSuccess ? APX_OK
                                                                                  : APX_ERR_CUDA;

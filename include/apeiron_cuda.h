@@ -514,7 +514,7 @@ APX_API int apx_gather_publish_async(apx_ctx *ctx, const apx_gather_desc *gd, vo
  *   layout, rounding and refusals; codes past n are set to zero here).
  * Optional outputs: d_resid = h (may be d_x itself), d_y = y, d_deq = the activation that the
  * codes stand for (S * code / 2^32, exact in f32 and bf16), and the codes / exponents /
- * descriptors (all three or none). */
+ * descriptors (all three or none; codes 4-byte, descriptors 16-byte aligned). */
 typedef struct apx_norm_args {
   const float *d_x, *d_add, *d_weight;
   float *d_resid, *d_y;
