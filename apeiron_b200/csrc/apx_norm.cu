@@ -70,7 +70,8 @@ __device__ __forceinline__ float scaled(float h, float w, float rh, float rl) {
 
 // QUADS: quads of the row in registers; 0 reads it twice.
 template <int QUADS, int THREADS>
-__global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_constant__ apx_norm_args a,
+__global__ void __launch_bounds__(THREADS, QUADS == 8 ? 4 : 1)
+    norm_quant_kernel(const __grid_constant__ apx_norm_args a,
                                                              size_t padded, int vec) {
   constexpr int W = THREADS / 32;
   __shared__ double s_sum[W];
@@ -83,11 +84,13 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
   pdl_launch_dependents();
   // the weights do not depend on the kernel before
   constexpr int N = QUADS ? QUADS : 1;
-  float4 h[N], w[N];
+  constexpr bool kWeightsFirst = QUADS > 0 && QUADS <= 2;  // few rows: on their way before the wait
+  float4 h[N], w[kWeightsFirst ? N : 1];
   const float4 one = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
 #pragma unroll
   for (int i = 0; i < N; i++)
-    if (QUADS) w[i] = a.d_weight ? load4(a.d_weight, 4 * (size_t)(i * THREADS + tid), a.n, vw) : one;
+    if (kWeightsFirst)
+      w[i] = a.d_weight ? load4(a.d_weight, 4 * (size_t)(i * THREADS + tid), a.n, vw) : one;
   pdl_wait();
   auto value = [&](size_t j) {
     float4 v = load4(x, j, a.n, vx);
@@ -186,7 +189,12 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
   };
   if (QUADS) {
 #pragma unroll
-    for (int i = 0; i < N; i++) quad(4 * (size_t)(i * THREADS + tid), h[i], w[i]);
+    for (int i = 0; i < N; i++) {
+      const size_t j = 4 * (size_t)(i * THREADS + tid);
+      quad(j, h[i], kWeightsFirst ? w[kWeightsFirst ? i : 0]
+                    : a.d_weight  ? load4(a.d_weight, j, a.n, vw)
+                                  : one);
+    }
   } else {
     // whole warps: quant_quad's shuffles take every lane
     const size_t end = (padded + 4 * THREADS - 1) / (4 * THREADS) * (4 * THREADS);
@@ -257,7 +265,7 @@ cudaError_t launch_add_rms_norm_quant(const apx_norm_args &a, cudaStream_t strea
   if (a.k <= 148 && quads <= 2048) return launch<2, 1024>(a, padded, vec, stream);
   if (quads <= 512) return launch<2, 256>(a, padded, vec, stream);
   if (quads <= 1024) return launch<4, 256>(a, padded, vec, stream);
-  if (quads <= 2048) return launch<4, 512>(a, padded, vec, stream);
+  if (quads <= 2048) return launch<8, 256>(a, padded, vec, stream);  // four CTAs to an SM
   if (quads <= 4096) return launch<4, 1024>(a, padded, vec, stream);
   return launch<0, 1024>(a, padded, vec, stream);
 }

@@ -113,7 +113,8 @@ __device__ __forceinline__ uint2 pack4(const float4 v, bool bf16) {
   return make_uint2(*reinterpret_cast<uint32_t *>(&p), *reinterpret_cast<uint32_t *>(&q));
 }
 
-// One token per CTA; dim / 4 threads take a head (query heads, then K heads, then V heads).
+// A token per blockIdx.x; dim / 4 threads take a head (query heads, then K heads, then V heads),
+// the heads shared by the CTAs of blockIdx.y.
 __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant__ RopeArgs r) {
   const apx_rope_args &a = r.a;
   const int t = blockIdx.x, per = r.dim / 4;
@@ -129,7 +130,7 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
     ok = page >= 0 && (size_t)page < r.n_pages;
   }
   if (!ok) {
-    if (threadIdx.x == 0 && a.d_status)
+    if (threadIdx.x == 0 && blockIdx.y == 0 && a.d_status)
       atomicMin(&a.d_status->first,
                 (unsigned long long)t << 24 | (unsigned long long)APX_ERR_INVALID_ARGUMENT << 16);
     return;
@@ -137,7 +138,8 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
   const float2 *cs = reinterpret_cast<const float2 *>(a.d_table) + (size_t)pos * (a.rot_dim / 2);
   const int row = pos % kKvTile, tile = pos % r.page_tokens / kKvTile;
   const int nq = a.d_q ? a.n_heads : 0, heads = nq + 2 * r.kv_heads;
-  for (int w = threadIdx.x; w < heads * per; w += blockDim.x) {  // whole groups of 8 lanes
+  for (int w = blockIdx.y * blockDim.x + threadIdx.x; w < heads * per;
+       w += gridDim.y * blockDim.x) {  // whole groups of 8 lanes
     const int head = w / per, i = w % per * 4;
     if (head < nq) {
       const float4 v = turn4(a.d_q + (size_t)t * a.ldq + (size_t)head * r.dim, i, a.rot_dim,
@@ -228,7 +230,9 @@ cudaError_t launch_rope_kv4_append(const apx_rope_args &a, const apx_kv4_cache &
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)b.n_tokens);
+  // two heads' worth a thread: more CTAs hide the chain position, page, values of each
+  const unsigned work = (unsigned)((a.d_q ? a.n_heads : 0) + 2 * c.n_kv_heads) * (c.head_dim / 4);
+  cfg.gridDim = dim3((unsigned)b.n_tokens, (work + 511) / 512);
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cfg.attrs = attr;

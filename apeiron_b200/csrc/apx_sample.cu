@@ -12,8 +12,12 @@
 // own shared memory and adds its bins to the first CTA's, which scans them from the top and
 // publishes the bin that crosses the target.  The first level's histogram serves both filters.
 //
-// What bounds it: 4 bytes a logit for many rows; for one row the chain of levels, two cluster
-// barriers each.
+// Where that bin and those above it hold 1024 tokens at most (any top-k in the hundreds, most
+// nuclei), they go to the first CTA, which sorts them, a token a thread: ranks and running sums
+// decide every filter at once, and a second sort, by index, the token.  It takes two cluster
+// barriers instead of two for each of up to five more levels.
+//
+// What bounds it: 4 bytes a logit for many rows; for one row the chain of barriers and scans.
 #include <algorithm>
 #include <climits>
 
@@ -67,6 +71,7 @@ struct Shared {
   unsigned warp_cnt[kWarps];
   Found found[2];  // by turns: one is read while the next is written
   u64 total;       // the weights of the level scanned last
+  unsigned floor_bin, floor_count, n_local, n_list;  // the candidates' lowest bin, their number
   u64 part[kMaxCluster][3];  // of each CTA: the weights above the cut, their number, the ties
   float top[kMaxCluster];
   int first[kMaxCluster];
@@ -89,6 +94,43 @@ __device__ u64 cta_sum(u64 v, Shared &s) {
   return v;
 }
 
+// Descending sort of v over the first n threads (a power of two from 32 to 1024; all threads call).
+__device__ u64 cta_sort(u64 v, int n, u64 *buf) {
+  const int tid = threadIdx.x;
+  for (int size = 2; size <= n; size <<= 1)
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      u64 other;
+      if (stride >= 32) {
+        __syncthreads();
+        buf[tid] = v;
+        __syncthreads();
+        other = buf[tid ^ stride];
+      } else {
+        other = __shfl_xor_sync(0xFFFFFFFFu, v, stride);
+      }
+      const bool larger = ((tid & stride) == 0) == ((tid & size) == 0);
+      v = larger == (v > other) ? v : other;
+    }
+  return v;
+}
+
+// Inclusive sum of v over the threads.
+__device__ u64 cta_scan(u64 v, Shared &s) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 t = __shfl_up_sync(0xFFFFFFFFu, v, o);
+    if (lane >= o) v += t;
+  }
+  __syncthreads();
+  if (lane == 31) s.warp_sum[warp] = v;
+  __syncthreads();
+  u64 b = lane < warp ? s.warp_sum[lane] : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
+  return v + b;
+}
+
 // A cluster per row; IPT tokens per thread, in quads: quad j of thread t is 4 (j 1024 + t).
 template <int IPT>
 __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, int ctas) {
@@ -101,6 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
   const unsigned v0 = min(per * rank, vocab), v1 = min(v0 + per, vocab);
   pdl_launch_dependents();
   s.cnt[tid] = s.lo[tid] = s.hi[tid] = s.mcnt[tid] = s.mlo[tid] = s.mhi[tid] = 0;
+  if (tid == 0) s.n_local = s.n_list = 0;
   pdl_wait();
   const float *x = a.d_logits + row * a.ld;
   const float temp = a.d_temperature ? a.d_temperature[row] : 1.0f;
@@ -186,6 +229,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
   }
 
   const bool by_k = k > 0 && (unsigned)k < vocab, by_p = top_p < 1.0f;
+  const double min_w = (double)min_p * (double)kWeightOne;
+  // (double)w < min_w for whole w: w below the next whole number
+  const unsigned least = min_w > 0.0 ? (unsigned)fmin(ceil(min_w), 4294967295.0) : 0u;
   // tokens with key > cut stay, and the first `ties` of those with key == cut
   unsigned cut = 0;
   u64 ties = ULLONG_MAX;
@@ -263,9 +309,97 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
   auto level_total = [&] { return ld_cluster(cluster_map(&s.total, 0)); };
 
   if (by_k || by_p) {
-    level(20, 0, 0, by_k, by_p, 0, 0);
+    level(20, 0, 0, true, by_p, 0, 0);
     // the first level, kept for top-p
     const u64 sum1 = sum, own1 = own_sum;
+    {
+      // the lowest bin that can hold a token that stays, and the tokens from it up
+      if (rank == 0) {
+        if (tid == kThreads - 1) s.floor_bin = 0;
+        __syncthreads();
+        const double limit = (double)top_p * (double)s.total;
+        const bool crosses = by_k ? count < (u64)k && count + own_count >= (u64)k
+                                  : (double)sum < limit && (double)(sum + own_sum) >= limit;
+        if (crosses) s.floor_bin = kBins - 1 - tid;
+        if (!by_k && limit <= 0.0 && tid == 0) s.floor_bin = kTopKey >> 20;
+        __syncthreads();
+        // tokens below min-p stay out, unless top-p's total needs those that top-k keeps
+        unsigned f = s.floor_bin;
+        if (!(by_k && by_p) && least > 1)
+          f = max(f, __float_as_uint((float)(least - 1) / kWeightOne * 0.999999f) >> 20);
+        f = min(f, kTopKey >> 20);
+        __syncthreads();
+        if (kBins - 1 - tid == (int)f) {
+          s.floor_bin = f;
+          s.floor_count = (unsigned)(count + own_count);
+        }
+        __syncthreads();
+      }
+      const Found c = publish(tid == 0, rank ? 0 : s.floor_bin, rank ? 0 : s.floor_count, 0);
+      if (c.count <= kThreads) {
+        // to a list here, then to the first CTA's
+        u64 *local = reinterpret_cast<u64 *>(s.cnt), *list = reinterpret_cast<u64 *>(s.mcnt);
+#pragma unroll
+        for (int i = 0; i < IPT; i++)
+          if (key[i] && key[i] >> 20 >= (unsigned)c.bin)
+            local[atomicAdd(&s.n_local, 1u)] =
+                (u64)key[i] << 32 | (0xFFFFFFFFu - (v0 + 4 * (i / 4 * kThreads + tid) + i % 4));
+        __syncthreads();
+        const unsigned mine = s.n_local;
+        if (tid == 0 && mine) {
+          unsigned at;
+          asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;"
+                       : "=r"(at)
+                       : "r"(cluster_map(&s.n_list, 0)), "r"(mine)
+                       : "memory");
+          s.floor_count = at;
+        }
+        __syncthreads();
+        if ((unsigned)tid < mine) st_cluster(cluster_map(list + s.floor_count + tid, 0), local[tid]);
+        cluster_sync();
+        if (rank) return;
+        const int nc = (int)c.count;
+        int n = 32;
+        while (n < nc) n <<= 1;
+        u64 v = cta_sort(tid < nc ? list[tid] : 0, n, local);
+        const unsigned w = tid < nc ? weight_of((unsigned)(v >> 32)) : 0u;
+        u64 run = cta_scan(w, s);
+        // the weights that top-p counts: of the first k, or of all
+        u64 all = s.total;
+        if (by_k && by_p && nc >= k) {
+          if (tid == k - 1) s.pick[0] = run;
+          __syncthreads();
+          all = s.pick[0];
+        }
+        const bool stays = tid < nc && (!by_k || tid < k) && w >= least && w > 0 &&
+                           (!by_p || tid == 0 ||
+                            (double)(run - w) < (double)top_p * (double)all);
+        const int kept = __syncthreads_count(stays);
+        if (kept == 0) {
+          if (tid == 0) {
+            a.d_token[row] = -1;
+            if (a.d_prob) a.d_prob[row] = 0.0f;
+            if (a.d_kept) a.d_kept[row] = 0;
+          }
+          return;
+        }
+        // in the vocabulary's order: the lowest index is the largest of the complements
+        v = cta_sort(stays ? (v & 0xFFFFFFFFull) << 32 | w : 0, n, local);
+        const u64 mine_w = v & 0xFFFFFFFFull;
+        run = cta_scan(mine_w, s);
+        if (tid == kThreads - 1) s.pick[1] = run;
+        __syncthreads();
+        const u64 total = s.pick[1];
+        u64 aim = u > 0.0f ? (u64)((double)u * (double)total) : 0;
+        if (aim >= total) aim = total - 1;
+        if (mine_w && run - mine_w <= aim && aim < run) {
+          a.d_token[row] = (int)(0xFFFFFFFFu - (unsigned)(v >> 32));
+          if (a.d_prob) a.d_prob[row] = (float)((double)mine_w / (double)total);
+          if (a.d_kept) a.d_kept[row] = kept;
+        }
+        return;
+      }
+    }
     u64 all = 0;         // the weights of all tokens that stay
     unsigned bin_k = 0;  // the first ten bits of the cut
     Found f;
@@ -342,9 +476,6 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
   }
 
   // ---- the weights that stay, of each CTA to every CTA ----
-  const double min_w = (double)min_p * (double)kWeightOne;
-  // (double)w < min_w for whole w: w below the next whole number
-  const unsigned least = min_w > 0.0 ? (unsigned)fmin(ceil(min_w), 4294967295.0) : 0u;
   const unsigned cut_w = cut ? weight_of(cut) : 0u, tie_w = cut_w >= least ? cut_w : 0u;
   auto above = [&](unsigned v) {  // its weight if it stays for being above the cut
     const unsigned w = v > cut ? weight_of(v) : 0u;
