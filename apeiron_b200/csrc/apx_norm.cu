@@ -52,11 +52,10 @@ __device__ __forceinline__ void store4f(float *p, size_t j, size_t n, bool quads
   if (j + 3 < n) p[j + 3] = v.w;
 }
 
-// (s, c) += h^2, c the rest of every rounding.
+// (s, c) += h^2, c the rest of the roundings: s - t is exact once s is half its end.
 __device__ __forceinline__ void add_square(float &s, float &c, float h) {
-  const float p = __fmul_rn(h, h), e = __fmaf_rn(h, h, -p);
-  const float t = __fadd_rn(s, p), b = __fsub_rn(t, s);
-  c += (__fsub_rn(s, __fsub_rn(t, b)) + __fsub_rn(p, b)) + e;
+  const float t = __fmaf_rn(h, h, s);
+  c += __fmaf_rn(h, h, __fsub_rn(s, t));
   s = t;
 }
 
@@ -70,8 +69,7 @@ __device__ __forceinline__ float scaled(float h, float w, float rh, float rl) {
 
 // QUADS: quads of the row in registers; 0 reads it twice.
 template <int QUADS, int THREADS>
-__global__ void __launch_bounds__(THREADS, QUADS == 8 ? 4 : 1)
-    norm_quant_kernel(const __grid_constant__ apx_norm_args a,
+__global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_constant__ apx_norm_args a,
                                                              size_t padded, int vec) {
   constexpr int W = THREADS / 32;
   __shared__ double s_sum[W];
@@ -265,7 +263,7 @@ cudaError_t launch_add_rms_norm_quant(const apx_norm_args &a, cudaStream_t strea
   if (a.k <= 148 && quads <= 2048) return launch<2, 1024>(a, padded, vec, stream);
   if (quads <= 512) return launch<2, 256>(a, padded, vec, stream);
   if (quads <= 1024) return launch<4, 256>(a, padded, vec, stream);
-  if (quads <= 2048) return launch<8, 256>(a, padded, vec, stream);  // four CTAs to an SM
+  if (quads <= 2048) return launch<4, 512>(a, padded, vec, stream);
   if (quads <= 4096) return launch<4, 1024>(a, padded, vec, stream);
   return launch<0, 1024>(a, padded, vec, stream);
 }

@@ -25,7 +25,6 @@
 #include "apx_kernels.h"
 #include "apx_pack.cuh"
 #include "apx_step.h"
-#include "apx_swiglu.cuh"
 
 namespace apx {
 
@@ -40,6 +39,25 @@ typedef unsigned long long u64;
 
 __device__ __forceinline__ unsigned weight_of(unsigned key) {
   return __float2uint_rn(__uint_as_float(key) * kWeightOne);
+}
+
+// exp_ref (apx_swiglu.cuh) bit for bit where e rounds to a weight above 0, -22.2 < x <= 0; there
+// n = rint(x log2 e) comes from an addition that rounds at the unit, and the scaling by 2^n, n >=
+// -33, is exact.  Below, 0: no weight, and no tie that could tell.
+__device__ __forceinline__ unsigned exp_key(float x) {
+  if (!(x > -22.2f)) return 0u;
+  const float t = __fadd_rn(__fmul_rn(x, __int_as_float(0x3fb8aa3b)), 12582912.0f);
+  const float n = __fsub_rn(t, 12582912.0f);
+  const float r = __fsub_rn(__fsub_rn(x, __fmul_rn(n, __int_as_float(0x3f318000))),
+                            __fmul_rn(n, __int_as_float((int)0xb95e8083u)));
+  float p = __int_as_float(0x39506967);
+  p = __fadd_rn(__fmul_rn(p, r), __int_as_float(0x3ab743ce));
+  p = __fadd_rn(__fmul_rn(p, r), __int_as_float(0x3c088908));
+  p = __fadd_rn(__fmul_rn(p, r), __int_as_float(0x3d2aa9c1));
+  p = __fadd_rn(__fmul_rn(p, r), __int_as_float(0x3e2aaaaa));
+  p = __fadd_rn(__fmul_rn(p, r), __int_as_float(0x3f000000));
+  const float y = __fadd_rn(__fadd_rn(1.0f, r), __fmul_rn(__fmul_rn(r, r), p));
+  return __float_as_uint(y) + (__float_as_uint(t) << 23);
 }
 
 __device__ __forceinline__ void cluster_sync() {
@@ -94,16 +112,19 @@ __device__ u64 cta_sum(u64 v, Shared &s) {
   return v;
 }
 
-// Descending sort of v over the first n threads (a power of two from 32 to 1024; all threads call).
+// Descending sort of v over the first n threads, which alone call it (a power of two from 32 to
+// 1024).
 __device__ u64 cta_sort(u64 v, int n, u64 *buf) {
   const int tid = threadIdx.x;
+#pragma unroll 1
   for (int size = 2; size <= n; size <<= 1)
+#pragma unroll 1
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
       u64 other;
       if (stride >= 32) {
-        __syncthreads();
+        asm volatile("bar.sync 1, %0;" ::"r"(n) : "memory");
         buf[tid] = v;
-        __syncthreads();
+        asm volatile("bar.sync 1, %0;" ::"r"(n) : "memory");
         other = buf[tid ^ stride];
       } else {
         other = __shfl_xor_sync(0xFFFFFFFFu, v, stride);
@@ -144,6 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
   pdl_launch_dependents();
   s.cnt[tid] = s.lo[tid] = s.hi[tid] = s.mcnt[tid] = s.mlo[tid] = s.mhi[tid] = 0;
   if (tid == 0) s.n_local = s.n_list = 0;
+  cluster_arrive_release();  // this CTA runs, its bins are zero
   pdl_wait();
   const float *x = a.d_logits + row * a.ld;
   const float temp = a.d_temperature ? a.d_temperature[row] : 1.0f;
@@ -179,8 +201,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
   top = s.wtop[lane];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  // every CTA's maximum to every CTA (the first barrier also says that all of them run)
-  cluster_sync();
+  // every CTA's maximum to every CTA
+  cluster_wait_acquire();
   if (tid < ctas)
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_map(&s.top[rank], tid)), "f"(top)
                  : "memory");
@@ -225,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
     const float l = __uint_as_float(key[i]);
     key[i] = !(l > -INFINITY) ? 0u  // NaN and -inf
              : l == top       ? kTopKey
-                              : __float_as_uint(exp_ref(__fmul_rn(__fsub_rn(l, top), inv)));
+                              : exp_key(__fmul_rn(__fsub_rn(l, top), inv));
   }
 
   const bool by_k = k > 0 && (unsigned)k < vocab, by_p = top_p < 1.0f;
@@ -239,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
   // One level's histogram over the keys in (floor, ..) whose bits above shift + 10 are `prefix`,
   // scanned by the first CTA from the top; thread t there holds bin 1023 - t: `count` and `sum`
   // of the bins above it, `own_count` and `own_sum` its own.
-  u64 count = 0, sum = 0, own_count = 0, own_sum = 0;
+  u64 count = 0, sum = 0, own_count = 0, own_sum = 0, kept1 = 0, kept_own1 = 0;
   auto level = [&](int shift, unsigned prefix, unsigned floor, bool counts, bool sums, u64 lump,
                    unsigned lump_key) {
 #pragma unroll
@@ -309,18 +331,16 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
   auto level_total = [&] { return ld_cluster(cluster_map(&s.total, 0)); };
 
   if (by_k || by_p) {
-    level(20, 0, 0, true, by_p, 0, 0);
-    // the first level, kept for top-p
-    const u64 sum1 = sum, own1 = own_sum;
+    level(20, 0, 0, true, !by_k, 0, 0);  // with top-k the sums can wait: a list has its own
     {
       // the lowest bin that can hold a token that stays, and the tokens from it up
       if (rank == 0) {
-        if (tid == kThreads - 1) s.floor_bin = 0;
+        if (tid == kThreads - 1) s.floor_bin = 0, s.pick[2] = 0;
         __syncthreads();
         const double limit = (double)top_p * (double)s.total;
         const bool crosses = by_k ? count < (u64)k && count + own_count >= (u64)k
                                   : (double)sum < limit && (double)(sum + own_sum) >= limit;
-        if (crosses) s.floor_bin = kBins - 1 - tid;
+        if (crosses) s.floor_bin = kBins - 1 - tid, s.pick[2] = by_k;
         if (!by_k && limit <= 0.0 && tid == 0) s.floor_bin = kTopKey >> 20;
         __syncthreads();
         // tokens below min-p stay out, unless top-p's total needs those that top-k keeps
@@ -330,18 +350,32 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
         f = min(f, kTopKey >> 20);
         __syncthreads();
         if (kBins - 1 - tid == (int)f) {
+          if (s.floor_bin != f) s.pick[2] = 0;  // the bin is not where top-k cuts
           s.floor_bin = f;
           s.floor_count = (unsigned)(count + own_count);
+          s.pick[0] = count;
         }
         __syncthreads();
       }
-      const Found c = publish(tid == 0, rank ? 0 : s.floor_bin, rank ? 0 : s.floor_count, 0);
+      Found c = publish(tid == 0, rank ? 0 : s.floor_bin, rank ? 0 : s.floor_count,
+                        rank ? 0 : s.pick[2]);
+      unsigned low = (unsigned)c.bin << 20;  // the lowest key of the candidates
+      if (c.count > kThreads && c.sum) {
+        // too many, most of them often in the bin where top-k cuts: ten bits more of those
+        const u64 over = s.pick[0];
+        kept1 = count, kept_own1 = own_count;
+        level(10, (unsigned)c.bin, 0, true, false, 0, 0);
+        const bool crosses = over + count < (u64)k && over + count + own_count >= (u64)k;
+        c = publish(crosses, kBins - 1 - tid, over + count + own_count, 0);
+        low |= (unsigned)c.bin << 10;
+        count = kept1, own_count = kept_own1;
+      }
       if (c.count <= kThreads) {
         // to a list here, then to the first CTA's
         u64 *local = reinterpret_cast<u64 *>(s.cnt), *list = reinterpret_cast<u64 *>(s.mcnt);
 #pragma unroll
         for (int i = 0; i < IPT; i++)
-          if (key[i] && key[i] >> 20 >= (unsigned)c.bin)
+          if (key[i] && key[i] >= low)
             local[atomicAdd(&s.n_local, 1u)] =
                 (u64)key[i] << 32 | (0xFFFFFFFFu - (v0 + 4 * (i / 4 * kThreads + tid) + i % 4));
         __syncthreads();
@@ -361,13 +395,14 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
         const int nc = (int)c.count;
         int n = 32;
         while (n < nc) n <<= 1;
-        u64 v = cta_sort(tid < nc ? list[tid] : 0, n, local);
+        u64 v = tid < nc ? list[tid] : 0;
+        if (tid < n) v = cta_sort(v, n, local);
         const unsigned w = tid < nc ? weight_of((unsigned)(v >> 32)) : 0u;
         u64 run = cta_scan(w, s);
         // the weights that top-p counts: of the first k, or of all
         u64 all = s.total;
-        if (by_k && by_p && nc >= k) {
-          if (tid == k - 1) s.pick[0] = run;
+        if (by_k && by_p) {  // fewer than k have weight: all of them are in the list
+          if (tid == min(k, nc) - 1) s.pick[0] = run;
           __syncthreads();
           all = s.pick[0];
         }
@@ -384,7 +419,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
           return;
         }
         // in the vocabulary's order: the lowest index is the largest of the complements
-        v = cta_sort(stays ? (v & 0xFFFFFFFFull) << 32 | w : 0, n, local);
+        v = stays ? (v & 0xFFFFFFFFull) << 32 | w : 0;
+        if (tid < n) v = cta_sort(v, n, local);
         const u64 mine_w = v & 0xFFFFFFFFull;
         run = cta_scan(mine_w, s);
         if (tid == kThreads - 1) s.pick[1] = run;
@@ -400,6 +436,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
         return;
       }
     }
+    if (by_k && by_p) level(20, 0, 0, true, true, 0, 0);
+    const u64 sum1 = sum, own1 = own_sum;  // kept for top-p
     u64 all = 0;         // the weights of all tokens that stay
     unsigned bin_k = 0;  // the first ten bits of the cut
     Found f;
@@ -640,9 +678,11 @@ cudaError_t launch(const apx_sample_args &a, int ctas, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_sample(const apx_sample_args &a, cudaStream_t stream) {
-  // the fewest CTAs whose registers hold the row in 20 tokens a thread, in 32 past 16 x 20
+  // the fewest CTAs whose registers hold the row in 20 tokens a thread, in 32 past 16 x 20; twice
+  // as many while all rows still run at once (one row of 151936: 16 CTAs 13.3 us)
   int ctas = 1;
   while (ctas < kMaxCluster && (size_t)ctas * kThreads * 20 < a.vocab) ctas *= 2;
+  if (ctas < kMaxCluster && a.rows * ctas * 2 <= 64 && a.vocab > 8192 * (size_t)ctas) ctas *= 2;
   const size_t per = ((a.vocab + 4 * ctas - 1) / (4 * ctas) * 4 + kThreads - 1) / kThreads;
   if (per <= 4) return launch<4>(a, ctas, stream);
   if (per <= 12) return launch<12>(a, ctas, stream);

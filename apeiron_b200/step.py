@@ -52,8 +52,8 @@ def _vector(t, n, dtype, name):
 def _rows(t, shape, name, dtype):
     """The elements between rows of a tensor of `shape` (2 or 3 dims, rows first) whose rows are
     each contiguous."""
-    st = t.stride()
     if t.dtype is dtype and t.is_cuda and t.shape == shape:
+        st = t.stride()
         if len(st) == 2:
             width = shape[1]
             if st[1] == 1 or width == 1:
