@@ -31,7 +31,10 @@ struct Stat {
   unsigned nz;
 };
 
+template <bool FULL>
 __device__ __forceinline__ float4 load4(const float *p, size_t j, size_t n, bool quads) {
+  if (FULL)
+    return j < n ? *reinterpret_cast<const float4 *>(p + j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (quads && j + 4 <= n) return *reinterpret_cast<const float4 *>(p + j);
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (j < n) v.x = p[j];
@@ -41,7 +44,12 @@ __device__ __forceinline__ float4 load4(const float *p, size_t j, size_t n, bool
   return v;
 }
 
+template <bool FULL>
 __device__ __forceinline__ void store4f(float *p, size_t j, size_t n, bool quads, const float4 v) {
+  if (FULL) {
+    if (j < n) *reinterpret_cast<float4 *>(p + j) = v;
+    return;
+  }
   if (quads && j + 4 <= n) {
     *reinterpret_cast<float4 *>(p + j) = v;
     return;
@@ -67,8 +75,36 @@ __device__ __forceinline__ float scaled(float h, float w, float rh, float rl) {
   return fabsf(t) < 1e38f ? y : t;  // an infinite product has no rest
 }
 
-// QUADS: quads of the row in registers; 0 reads it twice.
-template <int QUADS, int THREADS>
+// quant_quad (apx_quant.cuh) in f32 arithmetic, for blocks whose S is 2^-7 or more (e >= 25: their
+// largest value above 0.49, and below kFastAbsMax).  There a value that round(|y| 2^32) changes at
+// all lies below every code's boundary, so one rounding is left: |y| / S is exact, and additions
+// that round toward zero add the half and cut at the unit.  False, for the whole warp, where some
+// block is another; `code` are the codes as f32.
+__device__ __forceinline__ bool quant_quad_f32(const float4 y, uint32_t &packed, int &e, float4 &code) {
+  const float m = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
+  unsigned top = __float_as_uint(m);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  const int exp = (int)(top >> 23) - 101;
+  e = exp + ((top & 0x7FFFFFu) > 0x7E0000u ? 1 : 0);  // fast_scale_exp for E >= 118
+  const bool nan = !(y.x + y.y + y.z + y.w == y.x + y.y + y.z + y.w);
+  if (!__all_sync(0xFFFFFFFFu, exp >= 25 && top <= kFastAbsMax && !nan)) return false;
+  const float inv = __int_as_float((127 + 32 - e) << 23);  // 1 / S
+  auto one = [inv](float v, float &c) {
+    const float cut = __fadd_rz(__fadd_rz(fabsf(v) * inv, 0.5f), 8388608.0f);
+    c = copysignf(cut - 8388608.0f, v);
+    const int mag = (int)(__float_as_uint(cut) & 0xFFu);
+    return (unsigned)(v < 0.0f ? -mag : mag);
+  };
+  const unsigned a = one(y.x, code.x), b = one(y.y, code.y), c = one(y.z, code.z),
+                 d = one(y.w, code.w);
+  packed = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+  return true;
+}
+
+// QUADS: quads of the row in registers; 0 reads it twice.  FULL: quads are whole (n a multiple of
+// 4) and every array's rows aligned.
+template <int QUADS, int THREADS, bool FULL>
 __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_constant__ apx_norm_args a,
                                                              size_t padded, int vec) {
   constexpr int W = THREADS / 32;
@@ -88,12 +124,12 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
 #pragma unroll
   for (int i = 0; i < N; i++)
     if (kWeightsFirst)
-      w[i] = a.d_weight ? load4(a.d_weight, 4 * (size_t)(i * THREADS + tid), a.n, vw) : one;
+      w[i] = a.d_weight ? load4<FULL>(a.d_weight, 4 * (size_t)(i * THREADS + tid), a.n, vw) : one;
   pdl_wait();
   auto value = [&](size_t j) {
-    float4 v = load4(x, j, a.n, vx);
+    float4 v = load4<FULL>(x, j, a.n, vx);
     if (add) {
-      const float4 b = load4(add, j, a.n, va);
+      const float4 b = load4<FULL>(add, j, a.n, va);
       v = make_float4(__fadd_rn(v.x, b.x), __fadd_rn(v.y, b.y), __fadd_rn(v.z, b.z),
                       __fadd_rn(v.w, b.w));
     }
@@ -140,30 +176,33 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
   auto quad = [&](size_t j, const float4 v, const float4 g) {
     const float4 y = make_float4(scaled(v.x, g.x, rh, rl), scaled(v.y, g.y, rh, rl),
                                  scaled(v.z, g.z, rh, rl), scaled(v.w, g.w, rh, rl));
-    if (a.d_resid) store4f(a.d_resid + row * a.ld_resid, j, a.n, vr, v);
-    if (a.d_y) store4f(a.d_y + row * a.ldy, j, a.n, vy, y);
+    if (a.d_resid) store4f<FULL>(a.d_resid + row * a.ld_resid, j, a.n, vr, v);
+    if (a.d_y) store4f<FULL>(a.d_y + row * a.ldy, j, a.n, vy, y);
     if (!a.d_codes && !a.d_deq) return;
     uint32_t packed;
     int e;
-    bool ok;
-    quant_quad(y, packed, e, ok);
-    if (!ok || e < 0) packed = 0;
+    bool ok = true;
+    float4 code;
+    if (!quant_quad_f32(y, packed, e, code)) {
+      quant_quad(y, packed, e, ok);
+      if (!ok || e < 0) packed = 0;
+      code = make_float4((float)(int8_t)packed, (float)(int8_t)(packed >> 8),
+                         (float)(int8_t)(packed >> 16), (float)(int8_t)(packed >> 24));
+    }
     if (a.d_codes && j < padded)
       *reinterpret_cast<uint32_t *>(a.d_codes + row * padded + j) = packed;
     if (a.d_deq) {
       const float q = ok && e >= 0 ? __int_as_float((127 + e - 32) << 23) : 0.0f;
-      const float4 d = make_float4(q * (float)(int8_t)packed, q * (float)(int8_t)(packed >> 8),
-                                   q * (float)(int8_t)(packed >> 16),
-                                   q * (float)(int8_t)(packed >> 24));
+      const float4 d = make_float4(q * code.x, q * code.y, q * code.z, q * code.w);
       if (a.deq_type == APX_DTYPE_F32) {
-        store4f(static_cast<float *>(a.d_deq) + row * a.ld_deq, j, a.n, vd, d);
+        store4f<FULL>(static_cast<float *>(a.d_deq) + row * a.ld_deq, j, a.n, vd, d);
       } else {
         __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.d_deq) + row * a.ld_deq + j;
         const __nv_bfloat162 lo = __floats2bfloat162_rn(d.x, d.y), hi = __floats2bfloat162_rn(d.z, d.w);
-        if (vd && j + 4 <= a.n) {
+        if (FULL ? j < a.n : vd && j + 4 <= a.n) {
           *reinterpret_cast<uint2 *>(dst) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo),
                                                        *reinterpret_cast<const uint32_t *>(&hi));
-        } else {
+        } else if (!FULL) {
           if (j < a.n) dst[0] = lo.x;
           if (j + 1 < a.n) dst[1] = lo.y;
           if (j + 2 < a.n) dst[2] = hi.x;
@@ -190,14 +229,14 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
     for (int i = 0; i < N; i++) {
       const size_t j = 4 * (size_t)(i * THREADS + tid);
       quad(j, h[i], kWeightsFirst ? w[kWeightsFirst ? i : 0]
-                    : a.d_weight  ? load4(a.d_weight, j, a.n, vw)
+                    : a.d_weight  ? load4<FULL>(a.d_weight, j, a.n, vw)
                                   : one);
     }
   } else {
     // whole warps: quant_quad's shuffles take every lane
     const size_t end = (padded + 4 * THREADS - 1) / (4 * THREADS) * (4 * THREADS);
     for (size_t j = 4 * (size_t)tid; j < end; j += 4 * THREADS)
-      quad(j, value(j), a.d_weight ? load4(a.d_weight, j, a.n, vw) : one);
+      quad(j, value(j), a.d_weight ? load4<FULL>(a.d_weight, j, a.n, vw) : one);
   }
   if (!a.d_descs) return;
   emin = __reduce_min_sync(0xFFFFFFFFu, emin);
@@ -226,8 +265,8 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
   }
 }
 
-template <int QUADS, int THREADS>
-cudaError_t launch(const apx_norm_args &a, size_t padded, int vec, cudaStream_t stream) {
+template <int QUADS, int THREADS, bool FULL>
+cudaError_t launch_full(const apx_norm_args &a, size_t padded, int vec, cudaStream_t stream) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -237,7 +276,13 @@ cudaError_t launch(const apx_norm_args &a, size_t padded, int vec, cudaStream_t 
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_allowed() ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, norm_quant_kernel<QUADS, THREADS>, a, padded, vec);
+  return cudaLaunchKernelEx(&cfg, norm_quant_kernel<QUADS, THREADS, FULL>, a, padded, vec);
+}
+
+template <int QUADS, int THREADS>
+cudaError_t launch(const apx_norm_args &a, size_t padded, int vec, cudaStream_t stream) {
+  return a.n % 4 == 0 && vec == 63 ? launch_full<QUADS, THREADS, true>(a, padded, vec, stream)
+                                   : launch_full<QUADS, THREADS, false>(a, padded, vec, stream);
 }
 
 }  // namespace
