@@ -49,8 +49,8 @@ namespace {
 constexpr int kStepKeys = 32;
 // What a warp loses at an item's end (its rows to keep or write, the next one's to read), in steps:
 // items of single tokens carry as many steps without keys, so that warps with a boundary get fewer
-// keys (64 ragged requests: 53.2 -> 51.4 us; prompts' many short items lose by it).
-constexpr int kItemCost = 2;
+// keys (64 ragged requests: 53.2 us without, 51.4 at 2, 48.7 at 5; prompts lose by it).
+constexpr int kItemCost = 5;
 // Probabilities are held at 2^13 e^(s - m), where m is a stale maximum: it moves when a score
 // outgrows it by more than 2^2.
 constexpr float kTopExp = 13.0f, kStale = 2.0f;

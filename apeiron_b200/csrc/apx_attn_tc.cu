@@ -4,8 +4,8 @@
 // A CTA holds two tiles of 128 query rows of one KV head (a token's group of heads are neighbouring
 // rows) and takes its keys 128 at a time: S = Q K^T into TMEM, four softmax warps a tile turn S
 // into probabilities in place (f16), O += P V with P read from TMEM.  A tile's first softmax warp
-// issues its products.  The second tile starts a softmax later: while one is in its softmax the
-// other's products run.  Both read the same keys and values, which eight warps unpack from the
+// issues its products.  The tiles' softmaxes take turns: while one is in its softmax the other's
+// products run (left to themselves they fall into step and both wait for their products).  Both read the same keys and values, which eight warps unpack from the
 // cache's pages to f16 operands in shared memory (exact: d (c - 8) fits f16), two buffers each,
 // registers holding the bytes in flight.
 //
@@ -88,6 +88,14 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return d;
 }
 
+// Named barriers over n threads, those that wait and those that only arrive.
+__device__ __forceinline__ void bar_sync_n(int id, int n) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_arrive_n(int id, int n) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory");
+}
+
 __device__ __forceinline__ float as_f(uint32_t x) { return __uint_as_float(x); }
 __device__ __forceinline__ float as_f(float x) { return x; }
 template <typename A, typename B, typename C>
@@ -107,8 +115,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
   uint64_t *k_full = bars, *v_full = bars + 2, *k_free = bars + 4, *v_free = bars + 6;
   uint64_t *s_full = bars + 8, *o_full = bars + 10;  // per tile
-  uint64_t *second = bars + 12;                      // the second tile may start
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 13);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 12);
   float *s_cq = reinterpret_cast<float *>(smem + L::kCq);
   const int tid = threadIdx.x;
   const int warp = __shfl_sync(0xFFFFFFFFu, tid / 32, 0);  // the same in every lane, and known to be
@@ -144,7 +151,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(s_full + i, 1);
       mbar_init(o_full + i, 1);
     }
-    mbar_init(second, 1);
   }
   {
     // ---- Q: two threads a row ----
@@ -217,6 +223,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m = -INFINITY;
     uint64_t l2[2] = {0, 0};  // the row's sum in four parts
     const int steps = tile < tiles ? n : 0;
+    const bool turns = tiles == 2;
+    if (turns && tile == 1 && steps > 0) bar_arrive_n(3, 2 * kTile);  // the first turn is tile 0's
     const bool issues = warp % 4 == 0;  // this warp issues the tile's products
     const uint32_t leader = elect_leader();
     auto scores = [&](int j) {
@@ -253,7 +261,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
     };
     if (issues && steps > 0) {
-      if (tile == 1) ok = ok && mbar_wait(second, 0);
       scores(0);
     }
     __syncwarp();
@@ -264,6 +271,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       tc_fence_after();
       const bool masked = key + kKeys - 1 > all_hi || (key < all_lo && key + kKeys > p.sinks);
+      if (turns) bar_sync_n(3 + tile, 2 * kTile);  // the other tile's softmax is over
+      tc_fence_after();
       uint32_t s[4][32];  // the row's scores
 #pragma unroll
       for (int c = 0; c < 4; c++) tmem_ld32_nowait(ts + 32 * c, s[c]);
@@ -330,9 +339,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tmem_wait_st();
       tc_fence_before();
+      if (turns && (tile == 0 || j + 1 < steps)) bar_arrive_n(3 + (tile ^ 1), 2 * kTile);
       asm volatile("bar.sync %0, %1;" ::"r"(1 + tile), "n"(kTile) : "memory");  // the tile's threads
       if (issues) {
-        if (j == 0 && tile == 0 && leader) mbar_arrive(second);
         outputs(j);
         if (j + 1 < steps) scores(j + 1);
         else if (leader && ok) mma_commit(o_full + tile);
