@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   }
   // Equal shares for every warp of the grid, the first `rem` one step more.  Or, while there are
   // CTAs for all items and the longest costs a warp four steps at most: an item per CTA, which
-  // saves the join through the workspace (0.5B shape, 777 keys: 13.5 -> 8.6 us).
+  // saves the join through the workspace (0.5B shape, 777 keys: 13.5 -> 9.3 us).
   const int items = ONE ? p.n_seqs * p.kv_heads : 0;
   const bool whole_items = ONE && items <= (int)gridDim.x && longest <= 4 * W + kItemCost;
   const unsigned nwarps = whole_items ? W : min(gridDim.x * W, max(total, 1u));

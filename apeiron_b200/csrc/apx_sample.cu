@@ -17,7 +17,10 @@
 // decide every filter at once, and a second sort, by index, the token.  It takes two cluster
 // barriers instead of two for each of up to five more levels.
 //
-// What bounds it: 4 bytes a logit for many rows; for one row the chain of barriers and scans.
+// What bounds it: 4 bytes a logit is the floor (64 rows of 151936: 5.9 us); measured 61 us, with
+// half of the issue slots of the SMs that hold a CTA in use (some 90 instructions a token: e in
+// separately rounded steps, three shared-memory additions, the comparisons) and barriers the first
+// reason to wait.  One row: the chain of barriers, scans and the list's sorts, 13.6 us.
 #include <algorithm>
 #include <climits>
 
@@ -152,9 +155,24 @@ __device__ u64 cta_scan(u64 v, Shared &s) {
   return v + b;
 }
 
-// A cluster per row; IPT tokens per thread, in quads: quad j of thread t is 4 (j 1024 + t).
+// A thread's tokens: in its registers, or (two CTAs an SM) in shared memory, its own words.
+template <int IPT, bool PAIR>
+struct Keys {
+  unsigned r[IPT];
+  __device__ __forceinline__ unsigned &operator[](int i) { return r[i]; }
+};
 template <int IPT>
-__global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, int ctas) {
+struct Keys<IPT, true> {
+  __device__ __forceinline__ unsigned &operator[](int i) {
+    extern __shared__ unsigned shared_keys[];
+    return shared_keys[i * kThreads + threadIdx.x];
+  }
+};
+
+// A cluster per row; IPT tokens per thread, in quads: quad j of thread t is 4 (j 1024 + t).
+template <int IPT, bool PAIR>
+__global__ void __launch_bounds__(kThreads, PAIR ? 2 : 1)
+    sample_kernel(apx_sample_args a, int ctas) {
   __shared__ Shared s;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int rank = blockIdx.x % ctas;
@@ -175,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
   const float u = a.d_u[row];
 
   // ---- the logits, once; tokens past the end are excluded ones ----
-  unsigned key[IPT];  // the logit's bits, then e's
+  Keys<IPT, PAIR> key;  // the logit's bits, then e's
   const bool quads = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   float top = -INFINITY;
 #pragma unroll
@@ -653,9 +671,14 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(apx_sample_args a, 
   }
 }
 
-template <int IPT>
+template <int IPT, bool PAIR>
 cudaError_t launch(const apx_sample_args &a, int ctas, cudaStream_t stream) {
-  auto kern = sample_kernel<IPT>;
+  auto kern = sample_kernel<IPT, PAIR>;
+  if (PAIR) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               IPT * kThreads * 4);
+    if (e != cudaSuccess) return e;
+  }
   if (ctas > 8) {
     const cudaError_t e =
         cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -669,6 +692,7 @@ cudaError_t launch(const apx_sample_args &a, int ctas, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * ctas));
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = PAIR ? IPT * kThreads * 4 : 0;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_allowed() ? 2 : 1;
@@ -679,15 +703,19 @@ cudaError_t launch(const apx_sample_args &a, int ctas, cudaStream_t stream) {
 
 cudaError_t launch_sample(const apx_sample_args &a, cudaStream_t stream) {
   // the fewest CTAs whose registers hold the row in 20 tokens a thread, in 32 past 16 x 20; twice
-  // as many while all rows still run at once (one row of 151936: 16 CTAs 13.3 us)
+  // as many while all rows still run at once (one row of 151936: 8 CTAs 15.5 us, 16 CTAs 13.6)
   int ctas = 1;
   while (ctas < kMaxCluster && (size_t)ctas * kThreads * 20 < a.vocab) ctas *= 2;
   if (ctas < kMaxCluster && a.rows * ctas * 2 <= 64 && a.vocab > 8192 * (size_t)ctas) ctas *= 2;
   const size_t per = ((a.vocab + 4 * ctas - 1) / (4 * ctas) * 4 + kThreads - 1) / kThreads;
-  if (per <= 4) return launch<4>(a, ctas, stream);
-  if (per <= 12) return launch<12>(a, ctas, stream);
-  if (per <= 20) return launch<20>(a, ctas, stream);
-  return launch<32>(a, ctas, stream);
+  if (per <= 4) return launch<4, false>(a, ctas, stream);
+  // more CTAs than SMs: two an SM, one's barriers behind the other's work (a nucleus, min-p: 64
+  // rows of 151936 71.5 us with one an SM, 61.0 with two; 512 rows of 32003 125 and 97)
+  if (a.rows * ctas > 148 && per <= 20)
+    return per <= 12 ? launch<12, true>(a, ctas, stream) : launch<20, true>(a, ctas, stream);
+  if (per <= 12) return launch<12, false>(a, ctas, stream);
+  if (per <= 20) return launch<20, false>(a, ctas, stream);
+  return launch<32, false>(a, ctas, stream);
 }
 
 }  // namespace apx
