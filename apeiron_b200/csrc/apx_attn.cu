@@ -99,7 +99,8 @@ __device__ __forceinline__ void store_out(void *o, unsigned long long i, float v
 }
 
 // A sequence's steps.  Its blocks of rows pair first with last: a pair has `pair` steps, the
-// first block's, then the second's, then filling, steps without keys.  ONE: every sequence has one block at most.
+// first block's, then the second's, then filling, steps without keys.  ONE: every sequence has one
+// block at most.
 template <int R, bool ONE>
 struct SeqShape : SeqRows<R, kStepKeys> {
   using Base = SeqRows<R, kStepKeys>;
@@ -723,23 +724,69 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
     const unsigned firsts = __ballot_sync(0xFFFFFFFFu, used);
     unsigned starts = __ballot_sync(0xFFFFFFFFu, lane < W && s_edge[lane % W][1].used);
     // items here: the one that began before this CTA or at its first warp's first step, and each
-    // warp's last; their rows go round the warps
+    // warp's last; their rows go round the warps, one at a time, of prompts eight
+    constexpr int U = ONE ? 1 : 8, UNITS = R / U;
     const int items_here = (int)(firsts & 1) + __popc(starts);
     int item = 0;
 #pragma unroll 1
-    for (int j = warp; j < items_here * R; j += W) {
-      while (item < j / R - (int)(firsts & 1)) {
+    for (int j = warp; j < items_here * UNITS; j += W) {
+      while (item < j / UNITS - (int)(firsts & 1)) {
         starts &= starts - 1;
         item++;
       }
-      const bool head = (firsts & 1) && j < R;
-      const int w = head ? 0 : __ffs(starts) - 1, r = j % R;
+      const bool head = (firsts & 1) && j < UNITS;
+      const int w = head ? 0 : __ffs(starts) - 1, r = j % UNITS * U;
       const Edge &ed = s_edge[w][head ? 0 : 1];
       // its parts: this one and the first edges of the warps that follow
       const int n =
           __popc(__ballot_sync(0xFFFFFFFFu, used && lane > w && begin == ed.begin)) + 1;
       const float *first = part_of(w, head ? 0 : 1), *rest = part_of(w, 0);
       constexpr int S = C::kWarpSmem / 4;  // from a warp's part to the next one's
+      if constexpr (!ONE) {
+        // lane: row r + lane % U, parts lane / U + i KG
+        constexpr int KG = 32 / U, KR = (W + KG - 1) / KG;
+        float m[KR], l[KR], f[KR], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KR; i++) {
+          const int k = lane / U + i * KG;
+          const float *mine = (k ? rest + min(k, n - 1) * S : first) + R * D + r + lane % U;
+          m[i] = k < n ? mine[0] : -INFINITY, l[i] = k < n ? mine[R] : 0.0f;
+          top = fmaxf(top, m[i]);
+        }
+#pragma unroll
+        for (int o = U; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+#pragma unroll
+        for (int i = 0; i < KR; i++) {
+          f[i] = m[i] == -INFINITY ? 0.0f : ex2(m[i] - top);
+          sum = fmaf(f[i], l[i], sum);
+        }
+#pragma unroll
+        for (int o = U; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        const bool whole = ed.begin >= e0 && ed.end <= e1;
+        const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+        float *dst = p.part + ((size_t)blockIdx.x * 2 + (ed.begin >= e0 ? 1 : 0)) * C::kPart;
+        if (!whole && lane < U) {
+          dst[R * D + r + lane] = top;
+          dst[R * D + R + r + lane] = sum;
+        }
+#pragma unroll 2
+        for (int i = lane; i < U * Q; i += 32) {
+          const int u = i / Q, d = 4 * (i % Q);
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          add4(v, __shfl_sync(0xFFFFFFFFu, f[0], u),
+               *reinterpret_cast<const float4 *>(first + (r + u) * D + d));
+#pragma unroll
+          for (int k = 1; k < W; k++) {
+            if (k >= n) break;
+            add4(v, __shfl_sync(0xFFFFFFFFu, f[k / KG], u + U * (k % KG)),
+                 *reinterpret_cast<const float4 *>(rest + k * S + (r + u) * D + d));
+          }
+          const float inv = __shfl_sync(0xFFFFFFFFu, scale, u);
+          if (whole) write4(ed, r + u, d, v, inv);
+          else *reinterpret_cast<float4 *>(dst + (r + u) * D + d) = v;
+        }
+        continue;
+      }
       const float *mine = (lane ? rest + min(lane, n - 1) * S : first) + R * D + r;
       const float m = lane < n ? mine[0] : -INFINITY, l = lane < n ? mine[R] : 0.0f;
       float top = m;
