@@ -10,7 +10,10 @@
 // in registers between its sum and its quantization; rows past 16384 are read again.
 //
 // What bounds it: for many rows the bytes, 4 n read (8 n and 4 n written with a residual) and
-// 1 + 1/32 n written; for one row the chain load, sum over the CTA, root, quantize, store.
+// 1 + 1/32 n written, and some 65 instructions an element beside them: 512 rows of 8192 with
+// residual and 16-bit values move 63 MB in 19.5 us, 3.2 TB/s, half of what a large copy reaches,
+// with half of the issue slots used.  One row: the chain load, sum over the CTA, root, quantize,
+// store (896 wide: 2.4 us).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -71,30 +74,41 @@ __device__ __forceinline__ void add_square(float &s, float &c, float h) {
 __device__ __forceinline__ float scaled(float h, float w, float rh, float rl) {
   const float p = __fmul_rn(h, w), e = __fmaf_rn(h, w, -p);
   const float t = __fmul_rn(p, rh), f = __fmaf_rn(p, rh, -t);
-  const float y = __fadd_rn(t, __fmaf_rn(e, rh, __fmaf_rn(p, rl, f)));
-  return fabsf(t) < 1e38f ? y : t;  // an infinite product has no rest
+  return __fadd_rn(t, __fmaf_rn(e, rh, __fmaf_rn(p, rl, f)));
+}
+// The same where that came out at 1e37 or above, or not a number: an infinite product has no rest.
+__device__ __forceinline__ float scaled_large(float y, float h, float w, float rh) {
+  const float t = __fmul_rn(__fmul_rn(h, w), rh);
+  return fabsf(t) < 1e38f ? y : t;
+}
+
+// The largest magnitude, NaN if any is one.
+__device__ __forceinline__ float max_abs(const float4 v) {
+  float m;
+  asm("{ .reg .f32 a; max.NaN.f32 a, %1, %2; max.NaN.f32 %0, %3, %4; max.NaN.f32 %0, %0, a; }"
+      : "=&f"(m)
+      : "f"(fabsf(v.x)), "f"(fabsf(v.y)), "f"(fabsf(v.z)), "f"(fabsf(v.w)));
+  return m;
 }
 
 // quant_quad (apx_quant.cuh) in f32 arithmetic, for blocks whose S is 2^-7 or more (e >= 25: their
 // largest value above 0.49, and below kFastAbsMax).  There a value that round(|y| 2^32) changes at
 // all lies below every code's boundary, so one rounding is left: |y| / S is exact, and additions
 // that round toward zero add the half and cut at the unit.  False, for the whole warp, where some
-// block is another; `code` are the codes as f32.
-__device__ __forceinline__ bool quant_quad_f32(const float4 y, uint32_t &packed, int &e, float4 &code) {
-  const float m = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
-  unsigned top = __float_as_uint(m);
+// block is another or holds a NaN; `m` is the quad's max_abs, `code` are the codes as f32.
+__device__ __forceinline__ bool quant_quad_f32(const float4 y, float m, uint32_t &packed, int &e,
+                                               float4 &code) {
+  unsigned top = __float_as_uint(m);  // a NaN's is above kFastAbsMax
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   const int exp = (int)(top >> 23) - 101;
   e = exp + ((top & 0x7FFFFFu) > 0x7E0000u ? 1 : 0);  // fast_scale_exp for E >= 118
-  const bool nan = !(y.x + y.y + y.z + y.w == y.x + y.y + y.z + y.w);
-  if (!__all_sync(0xFFFFFFFFu, exp >= 25 && top <= kFastAbsMax && !nan)) return false;
+  if (!__all_sync(0xFFFFFFFFu, exp >= 25 && top <= kFastAbsMax)) return false;
   const float inv = __int_as_float((127 + 32 - e) << 23);  // 1 / S
   auto one = [inv](float v, float &c) {
-    const float cut = __fadd_rz(__fadd_rz(fabsf(v) * inv, 0.5f), 8388608.0f);
+    const float cut = __fadd_rz(__fmaf_rz(fabsf(v), inv, 0.5f), 8388608.0f);
     c = copysignf(cut - 8388608.0f, v);
-    const int mag = (int)(__float_as_uint(cut) & 0xFFu);
-    return (unsigned)(v < 0.0f ? -mag : mag);
+    return __float_as_uint(c + 12582912.0f);  // its low byte: c in two's complement
   };
   const unsigned a = one(y.x, code.x), b = one(y.y, code.y), c = one(y.z, code.z),
                  d = one(y.w, code.w);
@@ -108,7 +122,7 @@ template <int QUADS, int THREADS, bool FULL>
 __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_constant__ apx_norm_args a,
                                                              size_t padded, int vec) {
   constexpr int W = THREADS / 32;
-  __shared__ double s_sum[W];
+  __shared__ double s_sum[W], s_r;
   __shared__ Stat s_stat[W];
   const size_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
@@ -164,18 +178,32 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
   if (W > 1) {
     if (lane == 0) s_sum[warp] = sum;
     __syncthreads();
-    sum = lane < W ? s_sum[lane] : 0.0;
+    if (kWeightsFirst || warp == 0) {
+      sum = lane < W ? s_sum[lane] : 0.0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    }
   }
-  const double r = 1.0 / sqrt(sum / (double)a.n + (double)a.eps);
+  double r = 0.0;
+  if (kWeightsFirst || warp == 0) r = 1.0 / sqrt(sum / (double)a.n + (double)a.eps);
+  if (!kWeightsFirst) {  // many rows: its instructions once a row
+    if (tid == 0) s_r = r;
+    __syncthreads();
+    r = s_r;
+  }
   const float rh = (float)r, rl = fabsf(rh) < 3e38f ? (float)(r - (double)rh) : 0.0f;
 
   int emin = 1 << 30, emax = -1, status = APX_OK;
   unsigned nz = 0;
   auto quad = [&](size_t j, const float4 v, const float4 g) {
-    const float4 y = make_float4(scaled(v.x, g.x, rh, rl), scaled(v.y, g.y, rh, rl),
-                                 scaled(v.z, g.z, rh, rl), scaled(v.w, g.w, rh, rl));
+    float4 y = make_float4(scaled(v.x, g.x, rh, rl), scaled(v.y, g.y, rh, rl),
+                           scaled(v.z, g.z, rh, rl), scaled(v.w, g.w, rh, rl));
+    float m = max_abs(y);
+    if (!(m < 1e37f)) {
+      y = make_float4(scaled_large(y.x, v.x, g.x, rh), scaled_large(y.y, v.y, g.y, rh),
+                      scaled_large(y.z, v.z, g.z, rh), scaled_large(y.w, v.w, g.w, rh));
+      m = max_abs(y);
+    }
     if (a.d_resid) store4f<FULL>(a.d_resid + row * a.ld_resid, j, a.n, vr, v);
     if (a.d_y) store4f<FULL>(a.d_y + row * a.ldy, j, a.n, vy, y);
     if (!a.d_codes && !a.d_deq) return;
@@ -183,7 +211,7 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
     int e;
     bool ok = true;
     float4 code;
-    if (!quant_quad_f32(y, packed, e, code)) {
+    if (!quant_quad_f32(y, m, packed, e, code)) {
       quant_quad(y, packed, e, ok);
       if (!ok || e < 0) packed = 0;
       code = make_float4((float)(int8_t)packed, (float)(int8_t)(packed >> 8),
@@ -302,13 +330,14 @@ cudaError_t launch_add_rms_norm_quant(const apx_norm_args &a, cudaStream_t strea
   if (whole(a.d_deq, a.ld_deq, a.deq_type == APX_DTYPE_F32 ? 16 : 8)) vec |= 32;
   const size_t quads = padded / 4;  // padded is what has to be written
   // Few rows: as many threads as the row has quads, the loads of a row one round trip.  Many rows
-  // fill the GPU with smaller CTAs of more quads a thread.
+  // fill the GPU with smaller CTAs of more quads a thread (512 rows of 8192: 4 quads of 512 threads
+  // 20.0 us, 8 of 256 19.5).
   if (quads <= 256) return launch<1, 256>(a, padded, vec, stream);
   if (a.k <= 148 && quads <= 1024) return launch<1, 1024>(a, padded, vec, stream);
   if (a.k <= 148 && quads <= 2048) return launch<2, 1024>(a, padded, vec, stream);
   if (quads <= 512) return launch<2, 256>(a, padded, vec, stream);
   if (quads <= 1024) return launch<4, 256>(a, padded, vec, stream);
-  if (quads <= 2048) return launch<4, 512>(a, padded, vec, stream);
+  if (quads <= 2048) return launch<8, 256>(a, padded, vec, stream);
   if (quads <= 4096) return launch<4, 1024>(a, padded, vec, stream);
   return launch<0, 1024>(a, padded, vec, stream);
 }
