@@ -617,7 +617,8 @@ APX_API int apx_rope_kv4_append_async(apx_ctx *ctx, const apx_rope_args *args,
  * j < sinks.  A query that sees no key gets zeros.  Keys past d_kv_len never take part, whatever
  * the pages hold there.  q and out share one type.  For APX_DTYPE_F32 the products carry 22 bits
  * of q and of the probabilities (one below 2^-38 of its row's largest counts as zero), the sums
- * f32; for the 16-bit types the probabilities are rounded to 11 bits before the product with v.  Uses a context workspace: calls on one context must not overlap in time.
+ * f32; for the 16-bit types the probabilities are rounded to 11 bits before the product with v.
+ * Uses a context workspace: calls on one context must not overlap in time.
  * d_status (optional, all ones on entry): APX_ERR_INVALID_ARGUMENT with the first sequence whose
  * lengths or page numbers lie outside the batch or the cache (its rows are then undefined), or
  * APX_ERR_DEVICE_TIMEOUT. */
