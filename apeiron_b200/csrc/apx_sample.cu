@@ -156,8 +156,8 @@ __device__ u64 cta_scan(u64 v, Shared &s) {
   return v + b;
 }
 
-// A thread's tokens: in its registers, or (two CTAs an SM) in shared memory, its own words.
-template <int IPT, bool PAIR>
+// A thread's tokens: in its registers, or in shared memory, its own words.
+template <int IPT, bool SHARED>
 struct Keys {
   unsigned r[IPT];
   __device__ __forceinline__ unsigned &operator[](int i) { return r[i]; }
@@ -171,8 +171,8 @@ struct Keys<IPT, true> {
 };
 
 // A cluster per row; IPT tokens per thread, in quads: quad j of thread t is 4 (j 1024 + t).
-template <int IPT, bool PAIR>
-__global__ void __launch_bounds__(kThreads, PAIR ? 2 : 1)
+template <int IPT, bool SHARED, int PER_SM>
+__global__ void __launch_bounds__(kThreads, PER_SM)
     sample_kernel(apx_sample_args a, int ctas) {
   __shared__ Shared s;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, PAIR ? 2 : 1)
   const float u = a.d_u[row];
 
   // ---- the logits, once; tokens past the end are excluded ones ----
-  Keys<IPT, PAIR> key;  // the logit's bits, then e's
+  Keys<IPT, SHARED> key;  // the logit's bits, then e's
   const bool quads = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   float top = -INFINITY;
 #pragma unroll
@@ -672,10 +672,10 @@ __global__ void __launch_bounds__(kThreads, PAIR ? 2 : 1)
   }
 }
 
-template <int IPT, bool PAIR>
+template <int IPT, bool SHARED, int PER_SM>
 cudaError_t launch(const apx_sample_args &a, int ctas, cudaStream_t stream) {
-  auto kern = sample_kernel<IPT, PAIR>;
-  if (PAIR) {
+  auto kern = sample_kernel<IPT, SHARED, PER_SM>;
+  if (SHARED) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                IPT * kThreads * 4);
     if (e != cudaSuccess) return e;
@@ -693,7 +693,7 @@ cudaError_t launch(const apx_sample_args &a, int ctas, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * ctas));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = PAIR ? IPT * kThreads * 4 : 0;
+  cfg.dynamicSmemBytes = SHARED ? IPT * kThreads * 4 : 0;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_allowed() ? 2 : 1;
@@ -703,20 +703,22 @@ cudaError_t launch(const apx_sample_args &a, int ctas, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_sample(const apx_sample_args &a, cudaStream_t stream) {
-  // the fewest CTAs whose registers hold the row in 20 tokens a thread, in 32 past 16 x 20; twice
+  // the fewest CTAs that hold the row in 20 tokens a thread, in 32 past 16 x 20; twice
   // as many while all rows still run at once (one row of 151936: 8 CTAs 15.5 us, 16 CTAs 13.6)
   int ctas = 1;
   while (ctas < kMaxCluster && (size_t)ctas * kThreads * 20 < a.vocab) ctas *= 2;
   if (ctas < kMaxCluster && a.rows * ctas * 2 <= 64 && a.vocab > 8192 * (size_t)ctas) ctas *= 2;
   const size_t per = ((a.vocab + 4 * ctas - 1) / (4 * ctas) * 4 + kThreads - 1) / kThreads;
-  if (per <= 4) return launch<4, false>(a, ctas, stream);
+  if (per <= 4) return launch<4, false, 1>(a, ctas, stream);
   // more CTAs than SMs: two an SM, one's barriers behind the other's work (a nucleus, min-p: 64
   // rows of 151936 71.5 us with one an SM, 61.0 with two; 512 rows of 32003 125 and 97)
   if (a.rows * ctas > 148 && per <= 20)
-    return per <= 12 ? launch<12, true>(a, ctas, stream) : launch<20, true>(a, ctas, stream);
-  if (per <= 12) return launch<12, false>(a, ctas, stream);
-  if (per <= 20) return launch<20, false>(a, ctas, stream);
-  return launch<32, false>(a, ctas, stream);
+    return per <= 12 ? launch<12, true, 2>(a, ctas, stream) : launch<20, true, 2>(a, ctas, stream);
+  // more than 12 tokens a thread leave the levels too few registers (16 rows of 151936, a nucleus of
+  // thousands: 60 us in registers, 54 in shared memory; one row of 524288, top-k 50: 20.0 and 21.0)
+  if (per <= 12) return launch<12, false, 1>(a, ctas, stream);
+  if (per <= 20) return launch<20, true, 1>(a, ctas, stream);
+  return launch<32, true, 1>(a, ctas, stream);
 }
 
 }  // namespace apx
