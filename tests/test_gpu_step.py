@@ -457,6 +457,18 @@ def test_sample_large_vocabulary(ops, vocab):
         check_sample(ops, logits, [0.2, 0.7, 0.97], **f)
 
 
+@pytest.mark.parametrize("rows,vocab", [(90, 32003), (45, 65535), (24, 151936), (12, 300001)])
+def test_sample_many_rows(ops, rows, vocab):
+    """More CTAs than the GPU has SMs; flat rows, whose nuclei fit no list, among peaked ones."""
+    rng = np.random.default_rng(rows)
+    logits = (rng.standard_normal((rows, vocab)) * 2).astype(np.float32)
+    logits[::2, :: vocab // 70] += 9
+    u = (np.arange(rows) + 0.5) / rows
+    for f in (dict(), dict(top_k=40, top_p=0.9), dict(top_p=0.93, min_p=0.02),
+              dict(top_k=3001, top_p=0.8)):
+        check_sample(ops, logits, u, **f)
+
+
 @pytest.mark.parametrize("f", FILTERS, ids=str)
 def test_sample_ties(ops, f):
     """Few different logits: the lower index comes first of equals, at every cut."""
