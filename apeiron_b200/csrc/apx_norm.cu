@@ -70,16 +70,11 @@ __device__ __forceinline__ void add_square(float &s, float &c, float h) {
   s = t;
 }
 
-// h w r rounded once, r = rh + rl.  Where a rest would underflow the plain product is as near.
+// h w r rounded once, r = rh + rl, where the products stay within f32.
 __device__ __forceinline__ float scaled(float h, float w, float rh, float rl) {
   const float p = __fmul_rn(h, w), e = __fmaf_rn(h, w, -p);
   const float t = __fmul_rn(p, rh), f = __fmaf_rn(p, rh, -t);
   return __fadd_rn(t, __fmaf_rn(e, rh, __fmaf_rn(p, rl, f)));
-}
-// The same where that came out at 1e37 or above, or not a number: an infinite product has no rest.
-__device__ __forceinline__ float scaled_large(float y, float h, float w, float rh) {
-  const float t = __fmul_rn(__fmul_rn(h, w), rh);
-  return fabsf(t) < 1e38f ? y : t;
 }
 
 // The largest magnitude, NaN if any is one.
@@ -192,6 +187,9 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
     r = s_r;
   }
   const float rh = (float)r, rl = fabsf(rh) < 3e38f ? (float)(r - (double)rh) : 0.0f;
+  // f64 from here up, where h w may pass f32's end; everywhere where r lifts an h w below the normal
+  // numbers by more than 2^20 (less: an error below 2^-129)
+  const float most = rh < 1048576.0f ? 1e37f : -1.0f;
 
   int emin = 1 << 30, emax = -1, status = APX_OK;
   unsigned nz = 0;
@@ -199,9 +197,9 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
     float4 y = make_float4(scaled(v.x, g.x, rh, rl), scaled(v.y, g.y, rh, rl),
                            scaled(v.z, g.z, rh, rl), scaled(v.w, g.w, rh, rl));
     float m = max_abs(y);
-    if (!(m < 1e37f)) {
-      y = make_float4(scaled_large(y.x, v.x, g.x, rh), scaled_large(y.y, v.y, g.y, rh),
-                      scaled_large(y.z, v.z, g.z, rh), scaled_large(y.w, v.w, g.w, rh));
+    if (!(m < most)) {
+      auto wide = [r](float h, float w) { return (float)((double)h * (double)w * r); };
+      y = make_float4(wide(v.x, g.x), wide(v.y, g.y), wide(v.z, g.z), wide(v.w, g.w));
       m = max_abs(y);
     }
     if (a.d_resid) store4f<FULL>(a.d_resid + row * a.ld_resid, j, a.n, vr, v);

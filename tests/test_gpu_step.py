@@ -107,6 +107,38 @@ def test_norm(ops, n, k, extra, add, weight):
     assert np.array_equal(deq.float().cpu().numpy().astype(np.float64), stands)
 
 
+@pytest.mark.parametrize("n", [31, 896, 1537, 4097, 8192, 16001])
+@pytest.mark.parametrize("k,extra,add,weight", [(149, 0, True, True), (301, 2, False, True)])
+def test_norm_many_rows(ops, n, k, extra, add, weight):
+    """More rows than the GPU has SMs."""
+    test_norm(ops, n, k, extra, add, weight)
+
+
+@pytest.mark.parametrize("k", [5, 160])
+@pytest.mark.parametrize("n", [900, 5000])
+@pytest.mark.parametrize("x_size,w_size,eps", [
+    (1e18, 1e25, 1e-5), (1e37, 10.0, 1e-5), (1.0, 1e38, 1e-5), (1e-30, 1e-12, 0.0),
+    (1e-36, 1e20, 0.0), (1e-20, 1e-30, 1e-30), (1e-3, 1e-38, 1e-12)])
+def test_norm_far_numbers(ops, n, k, x_size, w_size, eps):
+    """h w past f32's ends where y is not, and y itself past the upper one; y is rounded once, but
+    for h w under the normal numbers, which lose up to 2^-150 before r < 2^20 lifts them."""
+    import torch
+
+    rng = np.random.default_rng(n + k)
+    x = (rng.uniform(0.5, 2, (k, n)) * rng.choice([-1, 1], (k, n)) * x_size).astype(np.float32)
+    w = (rng.uniform(0.5, 2, n) * w_size).astype(np.float32)
+    y = torch.empty(k, n, device="cuda")
+    ops.add_rms_norm_quant(gpu(x), gpu(w), eps, y=y, act=None)
+    eps = np.float64(np.float32(eps))
+    want = norm_ref(x, w.astype(np.float64), eps)
+    got = y.cpu().numpy().astype(np.float64)
+    r = 1 / np.sqrt((x.astype(np.float64) ** 2).mean(1, keepdims=True) + eps)
+    bound = 2.0 ** -23 * np.abs(want) + 2.0 ** -149 * np.where(r < 2.0 ** 20, np.maximum(r, 1), 1)
+    over = np.abs(want) > 3.4028235e38
+    assert np.all(np.abs(got - want)[~over] <= bound[~over])
+    assert np.all(np.abs(got[over]) >= 3.4028234e38)
+
+
 def test_norm_in_place_and_refusals(ops):
     """resid = x; a row with NaN or Inf refuses as the quantizer does, the others do not; -1 rows
     stay apart; a row of any size, denormals among them."""
