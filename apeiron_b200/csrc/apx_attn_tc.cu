@@ -14,6 +14,11 @@
 // exponentials 1024 (16 a cycle), shared memory 1024 (S reads both operands, P V one, the unpacked
 // keys and values go in for both tiles).
 //
+// A block's keys are shared by a cluster of up to eight CTAs where the blocks are too few for the
+// GPU; each turns its part of the steps into rows of O, m and l, and every CTA joins its share of the
+// block's rows from what the others have stored into its shared memory (in the CTAs' order: the same
+// bits every time).
+//
 // The running maximum is a stale one: O (in TMEM) and the row sum turn only when a row's maximum
 // has grown by more than 2^8 since the last turn; probabilities are held at 2^6 e^(s - m), at most
 // 2^14.  A row of q is scaled by a power of two to the top of f16's range: bf16 and f16 both fit.
@@ -21,6 +26,8 @@
 // K's dims are stored in the order the unpacking yields them (0 4 1 5 2 6 3 7 of every eight), Q's
 // the same.
 #include <cuda_bf16.h>
+
+#include <atomic>
 
 #include "apx_common.cuh"
 #include "apx_kernels.h"
@@ -42,6 +49,7 @@ static_assert((kSoftmaxRegs + kUnpackRegs) * 256 <= 128 * kThreads, "the launch'
 constexpr float kStale = 8.0f;    // log2 of how far a row's maximum may outgrow the stale one
 constexpr float kUnseen = -1e30f;  // an unseen key's score
 constexpr float kOffset = 6.0f;   // probabilities are held at 2^6 e^(s - m)
+constexpr int kMaxSplit = 8;      // CTAs a block's keys are shared by at most
 constexpr int kTmemCols = 512;    // S (then P) of the tiles in columns 0-255, O from 256 on
 
 // K-major operands in the 128-byte swizzle: rows of 64 f16, 8-row groups 1024 bytes apart.
@@ -62,6 +70,7 @@ struct Smem {
   static constexpr int kCq = kV + 2 * kOne;
   static constexpr int kBars = kCq + kRows * 4;
   static constexpr int kBytes = kBars + 128 + 1024;  // and the base's alignment
+  static_assert((kMaxSplit - 1) * (kRows / kMaxSplit) * (D * 4 + 8) <= kCq, "a join's parts");
 };
 
 // 16-byte chunk c (of 8) of row r in a panel of 128-byte rows.
@@ -108,7 +117,7 @@ __device__ __forceinline__ float max3(A a, B b, C c) {
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    attn_tc_kernel(const __grid_constant__ AttnArgs p) {
+    attn_tc_kernel(const __grid_constant__ AttnArgs p, const int ctas) {
   using L = Smem<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
@@ -120,21 +129,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   float *s_cq = reinterpret_cast<float *>(smem + L::kCq);
   const int tid = threadIdx.x;
   const int warp = __shfl_sync(0xFFFFFFFFu, tid / 32, 0);  // the same in every lane, and known to be
-  const int seq = blockIdx.x / p.kv_heads, head = blockIdx.x % p.kv_heads;
+  const int rank = (int)blockIdx.x % ctas, item = (int)blockIdx.x / ctas;  // of the cluster
+  const int seq = item / p.kv_heads, head = item % p.kv_heads;
 
   pdl_launch_dependents();
   pdl_wait();
   SeqRows<kRows, kKeys> q;
   q.load(p, seq);
-  if (q.bad && blockIdx.y == 0 && head == 0 && tid == 0)
+  if (q.bad && blockIdx.y == 0 && head == 0 && rank == 0 && tid == 0)
     attn_refuse(p, seq, APX_ERR_INVALID_ARGUMENT);
   const int blk = (int)(gridDim.y - 1 - blockIdx.y);  // the longest first
-  if (blk >= q.nblk) return;
+  if (blk >= q.nblk) return;  // with its whole cluster
   int end, sink, from;
   q.range(p, blk, end, sink, from);
-  const int n = sink + max(q.steps_to(end) - from, 0);
+  // this CTA's share of the block's steps: [j0, j0 + n)
+  const int all = sink + max(q.steps_to(end) - from, 0);
+  const int split = all >= ctas ? ctas : 1;  // too few steps: all of them here
+  if (rank >= split) return;
+  const int j0 = (int)((long long)all * rank / split);
+  const int n = (int)((long long)all * (rank + 1) / split) - j0;
   const int tiles = q.rows - blk * kRows > kTile ? 2 : 1;
-  auto key_of = [&](int j) { return (j < sink ? j : j - sink + from) * kKeys; };
+  auto key_of = [&](int j) { return (j + j0 < sink ? j + j0 : j + j0 - sink + from) * kKeys; };
 
   if (warp == 15) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -354,21 +369,85 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     tc_fence_after();
     const float2 la = unpack2(l2[0]), lb = unpack2(l2[1]);
-    const float l = (la.x + la.y) + (lb.x + lb.y);
+    float l = (la.x + la.y) + (lb.x + lb.y);
+    // a row of a split block is joined where rank = row / per: its parts from the other CTAs come
+    // into what held the operands, [split - 1][per] rows of D (chunks of a row turned by its number:
+    // no bank twice), then as many (m, l)
+    const int per = kRows / split, to_rank = row / per, rl = row % per;
+    auto part = [&](int slot) { return smem + (size_t)(slot * per + rl) * (D * 4); };
+    auto part_ml = [&](int slot) {
+      return smem + (size_t)(split - 1) * per * (D * 4) + (slot * per + rl) * 8;
+    };
+    auto turned = [&](int chunk) { return (chunk ^ (rl & (D / 4 - 1))) << 4; };
+    float own = steps > 0 && m > -INFINITY ? 1.0f : 0.0f, top = m;  // this CTA's factor
+    if (split > 1) {
+      cluster_arrive_release();  // every CTA is done with its operands
+      cluster_wait_acquire();
+      if (to_rank != rank) {
+        const int slot = rank < to_rank ? rank : rank - 1;
+        const uint32_t dst = cluster_map(part(slot), to_rank);
+        if (steps > 0)
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tmem_ld16_nowait(to + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                               dst + turned(c / 4 + i)),
+                           "r"(o[4 * i]), "r"(o[4 * i + 1]), "r"(o[4 * i + 2]), "r"(o[4 * i + 3])
+                           : "memory");
+          }
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(
+                         cluster_map(part_ml(slot), to_rank)),
+                     "f"(own == 0.0f ? -INFINITY : m), "f"(l)
+                     : "memory");
+      }
+      __syncwarp();
+      cluster_arrive_release();
+      cluster_wait_acquire();
+      if (to_rank == rank) {
+        for (int i = 0; i < split - 1; i++)
+          top = fmaxf(top, *reinterpret_cast<const float *>(part_ml(i)));
+        if (own != 0.0f) own = ex2(m - top);
+        l *= own;
+        for (int i = 0; i < split - 1; i++) {
+          const float2 ml = *reinterpret_cast<const float2 *>(part_ml(i));
+          if (ml.x > -INFINITY) l = fmaf(ex2(ml.x - top), ml.y, l);
+        }
+      }
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     uint16_t *dst = static_cast<uint16_t *>(p.out) +
                     (unsigned long long)(q.first + tok) * p.ldo +
                     (unsigned long long)(head * p.group + (live ? r : 0) - tok * p.group) * D;
 #pragma unroll 1
-    for (int c = 0; c < D; c += 16) {
+    for (int c = 0; c < (to_rank == rank ? D : 0); c += 16) {
       uint32_t o[16];
       if (steps > 0) {
         tmem_ld16_nowait(to + c, o);
         tmem_wait_ld();
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[i] = 0;
       }
+      if (own != 1.0f)
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+          o[i] = own == 0.0f ? 0 : __float_as_uint(__uint_as_float(o[i]) * own);
+#pragma unroll 1
+      for (int k = 0; k < split - 1; k++) {
+        const float ms = *reinterpret_cast<const float *>(part_ml(k));
+        if (ms == -INFINITY) continue;
+        const float f = ex2(ms - top);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float4 x = *reinterpret_cast<const float4 *>(part(k) + turned(c / 4 + i));
+          o[4 * i] = __float_as_uint(fmaf(f, x.x, __uint_as_float(o[4 * i])));
+          o[4 * i + 1] = __float_as_uint(fmaf(f, x.y, __uint_as_float(o[4 * i + 1])));
+          o[4 * i + 2] = __float_as_uint(fmaf(f, x.z, __uint_as_float(o[4 * i + 2])));
+          o[4 * i + 3] = __float_as_uint(fmaf(f, x.w, __uint_as_float(o[4 * i + 3])));
+        }
+      }
+      __syncwarp();
       uint32_t w[8];
 #pragma unroll
       for (int i = 0; i < 8; i++) {
@@ -511,6 +590,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive(v_full + buf);
       load_v(j + 1);
     }
+    if (split > 1) {  // the softmax threads' two
+      __syncwarp();
+      cluster_arrive_release();
+      cluster_wait_acquire();
+      cluster_arrive_release();
+      cluster_wait_acquire();
+    }
   }
   if (!ok) attn_refuse(p, seq, APX_ERR_DEVICE_TIMEOUT);
   tc_fence_before();
@@ -523,32 +609,69 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Clusters of `split` CTAs that the current device holds at once (found once a device).
+template <int D>
+int resident(int split, cudaLaunchConfig_t cfg) {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices][4];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= kDevices) return 0;
+  std::atomic<int> &k = known[dev][split == 2 ? 1 : split == 4 ? 2 : 3];
+  n = k.load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {(unsigned)split, 1, 1};
+    cfg.gridDim = dim3((unsigned)split, 1);
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, attn_tc_kernel<D>, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    k.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 template <int D>
 cudaError_t launch(const AttnArgs &p, int max_q, cudaStream_t stream) {
   auto kern = attn_tc_kernel<D>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        Smem<D>::kBytes);
   if (e != cudaSuccess) return e;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  const long long blocks = ((long long)max_q * p.group + kRows - 1) / kRows;
+  const long long items = (long long)p.n_seqs * p.kv_heads * blocks;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.n_seqs * p.kv_heads,
-                     (unsigned)(((long long)max_q * p.group + kRows - 1) / kRows));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = Smem<D>::kBytes;
   cfg.stream = stream;
+  // A block's keys to as many CTAs as let all of them run at once (64 tokens over 60000 keys, 8 KV
+  // heads: one CTA a block 1245 us, four 345; 128 over 8000: 165 and 61; 100 over 30000, 2 KV heads:
+  // 511, with eight 80).  Past that it costs: two rounds of short CTAs are slower than one of long
+  // ones (two prompts of 2048, 192 blocks: 64 us, in pairs 95).
+  int split = 1;
+  while (split < kMaxSplit && items <= resident<D>(2 * split, cfg))
+    split *= 2;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_allowed() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)split, 1, 1};
+  cfg.gridDim = dim3((unsigned)(p.n_seqs * p.kv_heads * split), (unsigned)blocks);
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_allowed() ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kern, p);
+  cfg.numAttrs = split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, p, split);
 }
 
 }  // namespace
 
-// Prompts in 16-bit numbers: enough rows for half a block.
+// Prompts in 16-bit numbers, from three quarters of a tile's rows on: a tile costs the same however
+// many of its rows are there (one request over 30000 keys, 8 KV heads: 90 us; apx_attn.cu's kernel 60
+// us for 64 rows, 77 for 96, 98 for 128; 32 requests over up to 4000, 96 rows: 158 and 201).
 bool attn_tc_serves(const AttnArgs &p, int dim, int max_q) {
   const long long rows = (long long)max_q * p.group;
-  return p.type != APX_DTYPE_F32 && rows >= 64 && rows <= 65535ll * kRows &&
+  return p.type != APX_DTYPE_F32 && rows >= 96 && rows <= 65535ll * kRows &&
          (long long)p.n_seqs * p.kv_heads < (1ll << 31) && (dim == 64 || dim == 128);
 }
 

@@ -388,6 +388,16 @@ def test_attention_prefill(ops, kind, heads, kv_heads, dim, page, q_lens, kv_len
     check_attention(ops, q_lens, kv_lens, heads, kv_heads, dim, page, kind)
 
 
+@pytest.mark.parametrize("kind", ["float16", "bfloat16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(14, 2, 64, 16), (16, 1, 128, 128), (12, 2, 128, 64)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1100, 0), (300, 5)])
+@pytest.mark.parametrize("q_lens,kv_lens", [([14], [1025]), ([30], [4001]), ([100, 3, 20], [2500, 900, 20]),
+                                            ([130], [1300])])
+def test_attention_chunk_of_long(ops, kind, heads, kv_heads, dim, page, window, sinks, q_lens, kv_lens):
+    """Few blocks of rows over long contexts, whose keys several CTAs share."""
+    check_attention(ops, q_lens, kv_lens, heads, kv_heads, dim, page, kind, window, sinks)
+
+
 @pytest.mark.parametrize("kind", ["float32", "bfloat16"])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (17, 0), (100, 33), (5000, 4),
                                           (64, 64)])
