@@ -5,8 +5,8 @@
 // rows) and takes its keys 128 at a time: S = Q K^T into TMEM, four softmax warps a tile turn S
 // into probabilities in place (f16), O += P V with P read from TMEM.  A tile's first softmax warp
 // issues its products.  The tiles' softmaxes take turns: while one is in its softmax the other's
-// products run (left to themselves they fall into step and both wait for their products: a prompt
-// of 2048 66 us, with turns 62.6).  Both read the same keys and values, which eight warps unpack
+// products run (left to themselves they fall into step and both wait for their products: two prompts
+// of up to 2048 66 us, with turns 60.5, 570 TFLOP/s of what they see).  Both read the same keys and values, which eight warps unpack
 // from the cache's pages to f16 operands in shared memory (exact: d (c - 8) fits f16), two buffers
 // each, registers holding the bytes in flight.
 //
@@ -60,6 +60,9 @@ __host__ __device__ constexpr uint32_t idesc_f16(int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
 
+// Warps' rows that a CTA of `split` joins at most.
+__host__ __device__ constexpr int join_warps(int split) { return (8 + split - 1) / split; }
+
 template <int D>
 struct Smem {
   // operands in panels of 64 columns: Q (both tiles) and K by dims, V^T by keys
@@ -70,7 +73,10 @@ struct Smem {
   static constexpr int kCq = kV + 2 * kOne;
   static constexpr int kBars = kCq + kRows * 4;
   static constexpr int kBytes = kBars + 128 + 1024;  // and the base's alignment
-  static_assert((kMaxSplit - 1) * (kRows / kMaxSplit) * (D * 4 + 8) <= kCq, "a join's parts");
+  // the parts that a join by `split` CTAs holds fit the operands' place
+  static constexpr bool joins(int split) {
+    return (split - 1) * 32 * join_warps(split) * (D * 4 + 8) <= kCq;
+  }
 };
 
 // 16-byte chunk c (of 8) of row r in a panel of 128-byte rows.
@@ -370,10 +376,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const float2 la = unpack2(l2[0]), lb = unpack2(l2[1]);
     float l = (la.x + la.y) + (lb.x + lb.y);
-    // a row of a split block is joined where rank = row / per: its parts from the other CTAs come
-    // into what held the operands, [split - 1][per] rows of D (chunks of a row turned by its number:
-    // no bank twice), then as many (m, l)
-    const int per = kRows / split, to_rank = row / per, rl = row % per;
+    // The rows of a split block are joined by the CTAs in warps' rows, as even as they go: warp w's by
+    // CTA w split / 8, in whose shared memory the parts from the others take the operands' place,
+    // [split - 1][per] rows of D (chunks of a row turned by its number: no bank twice), then as many
+    // (m, l).
+    const int per = 32 * join_warps(split), to_rank = warp * split / 8;
+    const int rl = row - 32 * ((8 * to_rank + split - 1) / split);
     auto part = [&](int slot) { return smem + (size_t)(slot * per + rl) * (D * 4); };
     auto part_ml = [&](int slot) {
       return smem + (size_t)(split - 1) * per * (D * 4) + (slot * per + rl) * 8;
@@ -613,10 +621,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int D>
 int resident(int split, cudaLaunchConfig_t cfg) {
   constexpr int kDevices = 64;
-  static std::atomic<int> known[kDevices][4];
+  static std::atomic<int> known[kDevices][kMaxSplit + 1];
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= kDevices) return 0;
-  std::atomic<int> &k = known[dev][split == 2 ? 1 : split == 4 ? 2 : 3];
+  std::atomic<int> &k = known[dev][split];
   n = k.load(std::memory_order_relaxed);
   if (n == 0) {
     cudaLaunchAttribute attr;
@@ -647,12 +655,11 @@ cudaError_t launch(const AttnArgs &p, int max_q, cudaStream_t stream) {
   cfg.dynamicSmemBytes = Smem<D>::kBytes;
   cfg.stream = stream;
   // A block's keys to as many CTAs as let all of them run at once (64 tokens over 60000 keys, 8 KV
-  // heads: one CTA a block 1245 us, four 345; 128 over 8000: 165 and 61; 100 over 30000, 2 KV heads:
-  // 511, with eight 80).  Past that it costs: two rounds of short CTAs are slower than one of long
-  // ones (two prompts of 2048, 192 blocks: 64 us, in pairs 95).
-  int split = 1;
-  while (split < kMaxSplit && items <= resident<D>(2 * split, cfg))
-    split *= 2;
+  // heads: one CTA a block 1245 us, four 344, six 243; 128 over 8000: 165, with four 61; 100 over
+  // 30000, 2 KV heads: 511, with eight 80).  Past that it costs: two rounds of short CTAs are slower
+  // than one of long ones (two prompts of 2048, 192 blocks: 64 us, in pairs 95).
+  int split = kMaxSplit;
+  while (split > 1 && !(Smem<D>::joins(split) && items <= resident<D>(split, cfg))) split--;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_allowed() ? 1 : 0;
