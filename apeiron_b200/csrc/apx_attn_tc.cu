@@ -5,10 +5,10 @@
 // rows) and takes its keys 128 at a time: S = Q K^T into TMEM, four softmax warps a tile turn S
 // into probabilities in place (f16), O += P V with P read from TMEM.  A tile's first softmax warp
 // issues its products.  The tiles' softmaxes take turns: while one is in its softmax the other's
-// products run (left to themselves they fall into step and both wait for their products: two prompts
-// of up to 2048 66 us, with turns 60.5, 570 TFLOP/s of what they see).  Both read the same keys and values, which eight warps unpack
-// from the cache's pages to f16 operands in shared memory (exact: d (c - 8) fits f16), two buffers
-// each, registers holding the bytes in flight.
+// products run (left to themselves they fall into step and both wait for their products: two
+// prompts of up to 2048 66 us, with turns 60.5, 570 TFLOP/s of what they see).  Both read the same
+// keys and values, which eight warps unpack from the cache's pages to f16 operands in shared memory
+// (exact: d (c - 8) fits f16), two buffers each, registers holding the bytes in flight.
 //
 // What bounds it, per 128 x 128 step of a tile at D = 128: the products 1024 cycles, the
 // exponentials 1024 (16 a cycle), shared memory 1024 (S reads both operands, P V one, the unpacked
