@@ -124,17 +124,12 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
   const float *x = a.d_x + row * a.ldx;
   const float *add = a.d_add ? a.d_add + row * a.ld_add : nullptr;
   const bool vx = vec & 1, va = vec & 2, vr = vec & 4, vy = vec & 8, vw = vec & 16, vd = vec & 32;
-  pdl_launch_dependents();
-  // the weights do not depend on the kernel before
   constexpr int N = QUADS ? QUADS : 1;
-  constexpr bool kWeightsFirst = QUADS > 0 && QUADS <= 2;  // few rows: on their way before the wait
-  float4 h[N], w[kWeightsFirst ? N : 1];
+  constexpr bool kFewRows = QUADS > 0 && QUADS <= 2;  // the weights in the values' round trip
+  float4 h[N], w[kFewRows ? N : 1];
   const float4 one = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-#pragma unroll
-  for (int i = 0; i < N; i++)
-    if (kWeightsFirst)
-      w[i] = a.d_weight ? load4<FULL>(a.d_weight, 4 * (size_t)(i * THREADS + tid), a.n, vw) : one;
-  pdl_wait();
+  pdl_launch_dependents();
+  pdl_wait();  // every input may be the output of the kernel before, the weights too
   auto value = [&](size_t j) {
     float4 v = load4<FULL>(x, j, a.n, vx);
     if (add) {
@@ -153,7 +148,11 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
   };
   if (QUADS) {
 #pragma unroll
-    for (int i = 0; i < N; i++) h[i] = value(4 * (size_t)(i * THREADS + tid));
+    for (int i = 0; i < N; i++) {
+      const size_t j = 4 * (size_t)(i * THREADS + tid);
+      h[i] = value(j);
+      if (kFewRows) w[kFewRows ? i : 0] = a.d_weight ? load4<FULL>(a.d_weight, j, a.n, vw) : one;
+    }
 #pragma unroll
     for (int i = 0; i < N; i++) square(h[i]);
   } else {
@@ -173,15 +172,15 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
   if (W > 1) {
     if (lane == 0) s_sum[warp] = sum;
     __syncthreads();
-    if (kWeightsFirst || warp == 0) {
+    if (kFewRows || warp == 0) {
       sum = lane < W ? s_sum[lane] : 0.0;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     }
   }
   double r = 0.0;
-  if (kWeightsFirst || warp == 0) r = 1.0 / sqrt(sum / (double)a.n + (double)a.eps);
-  if (!kWeightsFirst) {  // many rows: its instructions once a row
+  if (kFewRows || warp == 0) r = 1.0 / sqrt(sum / (double)a.n + (double)a.eps);
+  if (!kFewRows) {  // many rows: its instructions once a row
     if (tid == 0) s_r = r;
     __syncthreads();
     r = s_r;
@@ -254,7 +253,7 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const size_t j = 4 * (size_t)(i * THREADS + tid);
-      quad(j, h[i], kWeightsFirst ? w[kWeightsFirst ? i : 0]
+      quad(j, h[i], kFewRows ? w[kFewRows ? i : 0]
                     : a.d_weight  ? load4<FULL>(a.d_weight, j, a.n, vw)
                                   : one);
     }
