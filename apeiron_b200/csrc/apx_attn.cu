@@ -114,7 +114,8 @@ struct SeqShape : SeqRows<R, kStepKeys> {
     else if (!p.window) pair = steps(p, 0) + steps(p, n - 1) + 2;
     else {
       // a window's keys: what the block's positions span, in whole steps
-      const int most = p.window + (R - 1) / p.group + 1;
+      const int most =
+          (int)min((long long)p.window + (R - 1) / p.group + 1, (long long)this->kv);
       pair = 2 * (min(most / kStepKeys + 2 + Base::steps_to(min(p.sinks, this->kv)),
                       Base::steps_to(this->kv)) + 1);
     }
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
         const int pos = it.p0 + by_group(p, col);
         const bool live = col < it.rows;
         vis_hi[n][j] = live ? min(pos, end - 1) : -1;
-        vis_lo[n][j] = p.window ? pos - p.window + 1 : 0;
+        vis_lo[n][j] = window_start(p, pos);
         if (live) {
           all_hi = min(all_hi, vis_hi[n][j]);
           all_lo = max(all_lo, vis_lo[n][j]);
@@ -981,8 +982,10 @@ cudaError_t launch_attn_kv4(const apx_attn_args &a, const apx_kv4_cache &c,
   p.group = a.n_heads / c.n_kv_heads;
   p.page_shift = 0;
   while (1 << p.page_shift < c.page_tokens) p.page_shift++;
-  p.window = a.window;
-  p.sinks = a.window ? a.sinks : 0;
+  // a window with room for all that the table can hold hides no key
+  const long long room = (long long)b.max_pages * c.page_tokens;
+  p.window = a.window < room ? a.window : 0;
+  p.sinks = p.window ? a.sinks : 0;
   p.type = a.type;
   p.scale = a.scale;
   p.group_mul = (unsigned)(0x100000000ull / (unsigned)p.group + 1);

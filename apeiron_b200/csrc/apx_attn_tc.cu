@@ -232,12 +232,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tile = warp / 4, row = tid, r = blk * kRows + row;
     const bool live = r < q.rows;
     const int tok = by_group(p, live ? r : 0), pos = q.p0 + tok;
-    const int hi = live ? min(pos, end - 1) : -1, lo = p.window ? pos - p.window + 1 : 0;
+    const int hi = live ? min(pos, end - 1) : -1, lo = window_start(p, pos);
     // keys that every live row of the tile sees
     const int r0 = blk * kRows + tile * kTile;
     const int all_hi = min(q.p0 + by_group(p, r0), end - 1);
-    const int all_lo =
-        p.window ? q.p0 + by_group(p, min(r0 + kTile, q.rows) - 1) - p.window + 1 : 0;
+    const int all_lo = window_start(p, q.p0 + by_group(p, min(r0 + kTile, q.rows) - 1));
     // below 1e-20 no score (they stay below 2^34) tells; at it an unseen one still counts as none
     const float cq = fmaxf(s_cq[row], 1e-20f);
     const uint32_t lanes = (uint32_t)(32 * (warp % 4)) << 16;

@@ -95,6 +95,11 @@ __device__ __forceinline__ int by_group(const AttnArgs &p, int r) {
   return (int)(q - (q * (unsigned)p.group > (unsigned)r ? 1u : 0u));
 }
 
+// The first key of the window of the query at `pos`, which may stand before token 0.
+__device__ __forceinline__ int window_start(const AttnArgs &p, int pos) {
+  return p.window == 0 || pos < p.window ? 0 : pos - p.window + 1;
+}
+
 // A power of two that brings a row's largest |q| to [2^9, 2^10) (exponents outside the f32
 // normals are clamped), as its exponent's distance: q 2^(9 - e).
 __device__ __forceinline__ int row_exponent(float top) {
@@ -126,7 +131,7 @@ struct SeqRows {
     end = max(min(kv, hi + 1), 0);
     sink = from = 0;
     if (p.window) {
-      from = max(lo - p.window + 1, 0) / KEYS;
+      from = window_start(p, lo) / KEYS;
       sink = min(steps_to(min(p.sinks, end)), from);
     }
   }
