@@ -977,6 +977,7 @@ cudaError_t launch_attn_kv4(const apx_attn_args &a, const apx_kv4_cache &c,
   p.n_pages = (int)c.n_pages;
   p.n_seqs = b.n_seqs;
   p.n_tokens = (int)b.n_tokens;
+  p.max_q = b.max_q;
   p.max_pages = b.max_pages;
   p.kv_heads = c.n_kv_heads;
   p.group = a.n_heads / c.n_kv_heads;

@@ -46,7 +46,7 @@ struct AttnArgs {
   float *part;      // apx_attn.cu: two partial items per CTA
   unsigned *count;  // apx_attn.cu: CTAs that have arrived at an item (zero between calls)
   int n_pages, n_seqs, max_pages, kv_heads, group, page_shift;
-  int window, sinks, type, n_tokens;
+  int window, sinks, type, n_tokens, max_q;
   unsigned group_mul;  // 2^32 / group + 1, for by_group
   float scale;
 };
@@ -112,12 +112,12 @@ __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) <
 template <int R, int KEYS>
 struct SeqRows {
   int first, rows, kv, p0, nblk;  // first query token, rows, usable keys, position of row 0
-  bool bad;                       // lengths outside the batch or the cache
+  bool bad;  // lengths outside the batch or the cache, or more query tokens than the launch is for
 
   __device__ void load(const AttnArgs &p, int s) {
     const int a = p.cu[s], b = p.cu[s + 1], n = p.kv_len[s];
     const long long room = (long long)p.max_pages << p.page_shift;
-    bad = a < 0 || b < a || b > p.n_tokens || n < 0 || n > room;
+    bad = a < 0 || b < a || b > p.n_tokens || b - a > p.max_q || n < 0 || n > room;
     first = a;
     rows = bad ? 0 : (b - a) * p.group;
     kv = bad ? 0 : n;

@@ -38,3 +38,35 @@ def test_attention_wide_windows(ops, kind, window, sinks, q_lens, kv_lens):
 def test_attention_window_before_the_first_key(ops, kind, window, sinks, q_lens, kv_lens):
     """Queries that stand before token 0 under a window: zeros."""
     check_attention(ops, q_lens, kv_lens, 8, 2, 64, 16, kind, window, sinks)
+
+
+# ---- lengths and bounds that do not fit ------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+@pytest.mark.parametrize("q_lens,max_q", [([1, 3, 1], 2), ([8, 9, 1], 8), ([20, 41, 2], 40),
+                                          ([256, 257, 9], 256), ([600, 700, 128], 128)])
+def test_attention_more_queries_than_max_q(ops, kind, q_lens, max_q):
+    """A sequence with more query tokens than the batch says is refused with its number; the others
+    get what a batch whose bound fits gives them, to the roundings of another split."""
+    import torch
+    from apeiron_b200.step import KV4Cache, SeqBatch
+
+    rng = np.random.default_rng(max_q)
+    kv_lens = [n + 30 for n in q_lens]
+    good, table, n_pages = batch_of(q_lens, kv_lens, 16, rng)
+    cache = KV4Cache(gpu(random_pages(n_pages, 2, 64, 16, rng)), 2, 64, 16)
+    q = torch.randn(sum(q_lens), 2, 64, device="cuda").to(getattr(torch, kind))
+    stale = SeqBatch(good.cu, good.kv_len, good.table, good.n_tokens, max_q)
+    status = ops.new_status()
+    ops.attn_kv4(q, cache, stale, 0.1, status=status)
+    first = [i for i, n in enumerate(q_lens) if n > max_q][0]
+    assert ops.check_status(status) == (first, 20)
+    status = ops.new_status()
+    out = ops.attn_kv4(q, cache, stale, 0.1)
+    want = ops.attn_kv4(q, cache, good, 0.1, status=status)
+    assert ops.check_status(status) is None
+    cu = np.r_[0, np.cumsum(q_lens)]
+    for i, n in enumerate(q_lens):
+        if n <= max_q:
+            a, b = (t[cu[i]: cu[i + 1]].double() for t in (out, want))
+            assert (a - b).abs().max() <= 2.0 ** -7 * b.abs().max()
