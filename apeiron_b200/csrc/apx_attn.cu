@@ -32,6 +32,7 @@
 
 #include <algorithm>
 
+#include "apx_attn_items.cuh"
 #include "apx_common.cuh"
 #include "apx_kv4.cuh"
 #include "apx_pack.cuh"
@@ -46,11 +47,6 @@ cudaError_t launch_attn_tc(const AttnArgs &p, int dim, int max_q, cudaStream_t s
 
 namespace {
 
-constexpr int kStepKeys = 32;
-// What a warp loses at an item's end (its rows to keep or write, the next one's to read), in steps:
-// items of single tokens carry as many steps without keys, so that warps with a boundary get fewer
-// keys (64 ragged requests: 53.2 us without, 51.4 at 2, 48.7 at 5; prompts lose by it).
-constexpr int kItemCost = 5;
 // Probabilities are held at 2^13 e^(s - m), where m is a stale maximum: it moves when a score
 // outgrows it by more than 2^2.
 constexpr float kTopExp = 13.0f, kStale = 2.0f;
@@ -98,38 +94,6 @@ __device__ __forceinline__ void store_out(void *o, unsigned long long i, float v
   else static_cast<__nv_bfloat16 *>(o)[i] = __float2bfloat16_rn(v);
 }
 
-// A sequence's steps.  Its blocks of rows pair first with last: a pair has `pair` steps, the
-// first block's, then the second's, then filling, steps without keys.  ONE: every sequence has one
-// block at most.
-template <int R, bool ONE>
-struct SeqShape : SeqRows<R, kStepKeys> {
-  using Base = SeqRows<R, kStepKeys>;
-  int pair;
-
-  __device__ __forceinline__ void load(const AttnArgs &p, int s) {
-    Base::load(p, s);
-    const int n = this->nblk;
-    if (n <= 0) pair = 0;
-    else if (ONE || n == 1) pair = steps(p, 0) + kItemCost;
-    else if (!p.window) pair = steps(p, 0) + steps(p, n - 1) + 2;
-    else {
-      // a window's keys: what the block's positions span, in whole steps
-      const int most =
-          (int)min((long long)p.window + (R - 1) / p.group + 1, (long long)this->kv);
-      pair = 2 * (min(most / kStepKeys + 2 + Base::steps_to(min(p.sinks, this->kv)),
-                      Base::steps_to(this->kv)) + 1);
-    }
-  }
-  __device__ __forceinline__ int steps(const AttnArgs &p, int b) const {
-    int end, sink, from;
-    this->range(p, b, end, sink, from);
-    return max(sink + max(Base::steps_to(end) - from, 0), 1);  // one writes unseeing rows' zeros
-  }
-  __device__ __forceinline__ int pairs() const {
-    return ONE ? (this->nblk > 0 ? 1 : 0) : (this->nblk + 1) / 2;
-  }
-};
-
 template <int D, int NT>
 struct Cfg {
   static constexpr int kWarps = NT == 1 ? 16 : 8;
@@ -147,27 +111,6 @@ struct Cfg {
   static_assert(kSmem <= 227 * 1024 - 13 * 1024, "shared memory");
 };
 
-// One item that crosses a warp's boundary, kept for the join at the end of the CTA.
-struct Edge {
-  unsigned begin, end;          // the item's steps, numbered over the whole call
-  int first, rows, head, row0;  // its sequence's first token and rows, its KV head and first row
-  int used;
-};
-
-// One item: the steps [i0, i1) of a block of query rows of a KV head.  `real` is false for a pair's
-// filling, steps without keys.
-struct Item {
-  unsigned i0, i1;
-  int seq, first, rows, p0;  // of its sequence: first query token, rows, position of row 0
-  int head, row0;            // its KV head and first row
-  int end, sink, from;       // its keys (SeqRows::range)
-  bool real;
-  __device__ __forceinline__ int key_of(unsigned step) const {
-    const int st = (int)(step - i0);
-    return (st < sink ? st : st - sink + from) * kStepKeys;
-  }
-};
-
 // The item of step g, the same g in every lane.  pre: the steps of the call up to the end of each
 // thread's `per` sequences.
 template <int R, bool ONE, int THREADS>
@@ -176,34 +119,24 @@ __device__ __noinline__ Item find_item(const AttnArgs &p, const unsigned *pre, i
   const int lane = threadIdx.x % 32;
   int at = __ffs(__ballot_sync(0xFFFFFFFFu, pre[lane * N + N - 1] > g)) - 1;
   at = at * N + __ffs(__ballot_sync(0xFFFFFFFFu, lane < N && pre[at * N + lane % N] > g)) - 1;
-  unsigned seq0, seq1 = at ? pre[at - 1] : 0;
-  SeqShape<R, ONE> q;
-  Item it;
-  it.seq = at * per - 1;
-  do {
-    seq0 = seq1;
-    q.load(p, ++it.seq);
-    seq1 = seq0 + (unsigned)q.pairs() * q.pair * p.kv_heads;
-  } while (g >= seq1);
-  const unsigned nth = (g - seq0) / (unsigned)q.pair, n = q.pairs();
-  it.head = (int)(ONE ? nth : nth / n);
-  int blk = ONE ? 0 : (int)(nth - it.head * n);
-  it.i0 = seq0 + nth * q.pair;
-  const unsigned end = it.i0 + q.pair;
-  it.i1 = it.i0 + q.steps(p, blk);
-  if (!ONE && g >= it.i1 && blk != q.nblk - 1 - blk) {
-    blk = q.nblk - 1 - blk;
-    it.i0 = it.i1;
-    it.i1 = it.i0 + q.steps(p, blk);
-  }
-  it.real = g < it.i1;
-  if (!it.real) it.i1 = end;
-  it.first = q.first;
-  it.rows = q.rows;
-  it.p0 = q.p0;
-  it.row0 = blk * R;
-  q.range(p, blk, it.end, it.sink, it.from);
-  return it;
+  return item_from<R, ONE>(p, at * per, at ? pre[at - 1] : 0, g);
+}
+
+// Where a wait has given up, a CTA has no parts to give, yet each item that crosses its ends counts it:
+// these stand for what its warps would have kept (the parts behind them may hold anything: the
+// status has the call as refused), so that the counters are zero again at the end of the call.
+template <int R, bool ONE, int W>
+__device__ __noinline__ void keep_owed(const AttnArgs &p, unsigned e0, unsigned e1, Edge (*edge)[2]) {
+  for (int w = 0; w < W; w++) edge[w][0].used = edge[w][1].used = 0;
+  Edge from_before, goes_on;
+  const int owes = owed<R, ONE>(p, e0, e1, from_before, goes_on);
+  if (owes & 1) edge[0][0] = from_before;
+  if (owes & 2) edge[W - 1][1] = goes_on;
+}
+
+// After a wait has given up: copies [from, to) may still be on their way into shared memory.
+__device__ __noinline__ void drain(uint64_t *bar, int slots, int from, int to) {
+  for (int i = from; i < to; i++) mbar_wait(bar + i % slots, i / slots & 1);
 }
 
 template <int D, int NT, int TYPE>
@@ -283,10 +216,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
     c0 = s0 + h * n;
     c1 = c0 + (n ? n - kItemCost : 0);
   }
-  const unsigned base = (c1 - c0) / nwarps, rem = c1 - c0 - base * nwarps;
-  auto bound = [&](unsigned w) { return c0 + min(w, nwarps) * base + min(w, rem); };
+  const Shares<W> share(c0, c1, nwarps);
   const unsigned w0 = whole_items ? 0 : blockIdx.x * W;  // this CTA's first warp
-  const unsigned u0 = bound(w0 + warp), u1 = bound(w0 + warp + 1);
+  const unsigned u0 = share.bound(w0 + warp), u1 = share.bound(w0 + warp + 1);
 
   // ---- copies: step u0 + i into slot i of the ring, through every item of this warp ----
   const uint8_t *src = nullptr;  // lane i: tile i % 2 of step u0 + batch + i / 2; null: no such
@@ -324,11 +256,11 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   };
   const int mine = (int)(u1 - u0);  // steps of this warp
   int at = 0;                       // of them, done
-  bool alive = true;                // no wait has given up
+  bool alive = true;                // no wait has given up; between steps the same in every lane
   auto arrived = [&](int i) {
     const int sl = i & (C::kSlots - 1);
     const unsigned parity = (unsigned)i / C::kSlots & 1;
-    if (!mbar_try(bar + sl, parity)) alive = alive && mbar_wait_more(bar + sl, parity);
+    if (!mbar_try(bar + sl, parity)) alive = mbar_wait_more(bar + sl, parity);
   };
 
   // ---- this warp's steps, item by item ----
@@ -443,7 +375,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
     const bool from_start = u0 + at == it.i0;
 
 #pragma unroll 1
-    for (; at < stop; at++) {
+    for (; at < stop && alive; at++) {
       arrived(at);
       uint8_t *tile = ring + (at & (C::kSlots - 1)) * C::kSlot;
       if (it.real) {  // not filling, which has no keys
@@ -640,13 +572,13 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
         }
       }
       }
-      __syncwarp();  // every lane has read the slot
-      if (at + C::kSlots < mine) {
+      alive = __all_sync(0xFFFFFFFFu, alive);  // and every lane has read the slot
+      if (alive && at + C::kSlots < mine) {
         if (at + C::kSlots - batch >= 16) look_ahead(at + C::kSlots, it);
         start(at + C::kSlots);
       }
     }
-    if (!it.real) continue;
+    if (!it.real || !alive) continue;
 
     // ---- the item's rows of this warp ----
 #pragma unroll
@@ -694,14 +626,21 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
             part[R * D + R + r] = l[n][j];
           }
         }
-      if (lane == 0) s_edge[warp][e] = Edge{it.i0, it.i1, it.first, it.rows, it.head, it.row0, 1};
+      if (lane == 0) s_edge[warp][e] = edge_of(it);
     }
   }
-  if (!alive && lane == 0) attn_refuse(p, 0, APX_ERR_DEVICE_TIMEOUT);
+  if (!alive) {
+    if (lane == 0) attn_refuse(p, 0, APX_ERR_DEVICE_TIMEOUT);
+    drain(bar, C::kSlots, at - 1, min(at - 1 + C::kSlots, mine));
+  }
 
   // ---- the join: items that cross warps, each by the warp that has its first part ----
-  __syncthreads();
-  const unsigned e0 = bound(w0), e1 = bound(w0 + W);  // this CTA's steps
+  const unsigned e0 = share.bound(w0), e1 = share.bound(w0 + W);  // this CTA's steps
+  if (__syncthreads_or(!alive)) {
+    if (whole_items) return;
+    if (tid == 0) keep_owed<R, ONE, W>(p, e0, e1, s_edge);
+    __syncthreads();
+  }
   constexpr int E = R * D / 4, Q = D / 4;             // quads of an item's rows, of a row
   auto part_of = [&](int w, int e) {
     return reinterpret_cast<const float *>(smem + w * C::kWarpSmem + (e ? 0 : C::kRing));
@@ -835,10 +774,6 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   }
   if (!out_of_cta) return;  // the same in every thread
   // An item's CTAs: the first holds it as its last item, the others as the one from before.
-  auto cta_of = [&](unsigned step) {
-    const unsigned wide = rem * (base + 1);
-    return (int)((step < wide ? step / (base + 1) : rem + (step - wide) / base) / W);
-  };
   fence_acq_rel_gpu();
   __syncthreads();
   if (tid < 2) {
@@ -846,7 +781,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
     if (out_of_cta >> tid & 1) {
       const unsigned begin = tid ? edge1.begin : edge0.begin;
       const unsigned end = tid ? edge1.end : edge0.end;
-      const int a = cta_of(begin), all = cta_of(end - 1) - a + 1;
+      const int a = share.cta_of(begin), all = share.cta_of(end - 1) - a + 1;
       if (atomicAdd(p.count + a, 1u) == (unsigned)all - 1) {
         n = all;
         p.count[a] = 0;  // for the next call
@@ -861,7 +796,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
     const int n = s_last[e];
     if (!n) continue;
     const Edge ed = e ? edge1 : edge0;
-    const float *first = p.part + ((size_t)cta_of(ed.begin) * 2 + 1) * C::kPart;
+    const float *first = p.part + ((size_t)share.cta_of(ed.begin) * 2 + 1) * C::kPart;
     auto src_of = [&](int k) { return first + (k ? (size_t)(2 * k - 1) * C::kPart : 0); };
     // the parts' factors, then their sum by groups of threads, each a share of the parts; a
     // thread's first eight quads are on their way meanwhile

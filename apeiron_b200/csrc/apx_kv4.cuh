@@ -89,14 +89,14 @@ __device__ __forceinline__ void attn_refuse(const AttnArgs &p, int seq, int code
 }
 
 // r / group for 0 <= r < 2^31: the product's high word is the quotient or one more.
-__device__ __forceinline__ int by_group(const AttnArgs &p, int r) {
+__host__ __device__ __forceinline__ int by_group(const AttnArgs &p, int r) {
   if (p.group == 1) return r;
-  const unsigned q = __umulhi((unsigned)r, p.group_mul);
+  const unsigned q = (unsigned)((unsigned long long)(unsigned)r * p.group_mul >> 32);
   return (int)(q - (q * (unsigned)p.group > (unsigned)r ? 1u : 0u));
 }
 
 // The first key of the window of the query at `pos`, which may stand before token 0.
-__device__ __forceinline__ int window_start(const AttnArgs &p, int pos) {
+__host__ __device__ __forceinline__ int window_start(const AttnArgs &p, int pos) {
   return p.window == 0 || pos < p.window ? 0 : pos - p.window + 1;
 }
 
@@ -114,7 +114,7 @@ struct SeqRows {
   int first, rows, kv, p0, nblk;  // first query token, rows, usable keys, position of row 0
   bool bad;  // lengths outside the batch or the cache, or more query tokens than the launch is for
 
-  __device__ void load(const AttnArgs &p, int s) {
+  __host__ __device__ void load(const AttnArgs &p, int s) {
     const int a = p.cu[s], b = p.cu[s + 1], n = p.kv_len[s];
     const long long room = (long long)p.max_pages << p.page_shift;
     bad = a < 0 || b < a || b > p.n_tokens || b - a > p.max_q || n < 0 || n > room;
@@ -124,9 +124,9 @@ struct SeqRows {
     p0 = n - (b - a);
     nblk = (rows + R - 1) / R;
   }
-  __device__ static int steps_to(int n) { return (max(n, 0) + KEYS - 1) / KEYS; }
+  __host__ __device__ static int steps_to(int n) { return (max(n, 0) + KEYS - 1) / KEYS; }
   // Block b sees keys below `end`: those of the sinks' steps [0, sink) and of steps `from` on.
-  __device__ void range(const AttnArgs &p, int b, int &end, int &sink, int &from) const {
+  __host__ __device__ void range(const AttnArgs &p, int b, int &end, int &sink, int &from) const {
     const int lo = p0 + by_group(p, b * R), hi = p0 + by_group(p, min((b + 1) * R - 1, rows - 1));
     end = max(min(kv, hi + 1), 0);
     sink = from = 0;
