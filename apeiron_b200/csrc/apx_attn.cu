@@ -113,23 +113,23 @@ struct Cfg {
 
 // The item of step g, the same g in every lane.  pre: the steps of the call up to the end of each
 // thread's `per` sequences.
-template <int R, bool ONE, int THREADS>
-__device__ __noinline__ Item find_item(const AttnArgs &p, const unsigned *pre, int per, unsigned g) {
+template <int R, bool ONE, int THREADS, typename S>
+__device__ __noinline__ Item<S> find_item(const AttnArgs &p, const S *pre, int per, S g) {
   constexpr int N = THREADS / 32;
   const int lane = threadIdx.x % 32;
   int at = __ffs(__ballot_sync(0xFFFFFFFFu, pre[lane * N + N - 1] > g)) - 1;
   at = at * N + __ffs(__ballot_sync(0xFFFFFFFFu, lane < N && pre[at * N + lane % N] > g)) - 1;
-  return item_from<R, ONE>(p, at * per, at ? pre[at - 1] : 0, g);
+  return item_from<R, ONE, S>(p, at * per, at ? pre[at - 1] : 0, g);
 }
 
 // Where a wait has given up, a CTA has no parts to give, yet each item that crosses its ends counts it:
 // these stand for what its warps would have kept (the parts behind them may hold anything: the
 // status has the call as refused), so that the counters are zero again at the end of the call.
-template <int R, bool ONE, int W>
-__device__ __noinline__ void keep_owed(const AttnArgs &p, unsigned e0, unsigned e1, Edge (*edge)[2]) {
+template <int R, bool ONE, int W, typename S>
+__device__ __noinline__ void keep_owed(const AttnArgs &p, S e0, S e1, Edge<S> (*edge)[2]) {
   for (int w = 0; w < W; w++) edge[w][0].used = edge[w][1].used = 0;
-  Edge from_before, goes_on;
-  const int owes = owed<R, ONE>(p, e0, e1, from_before, goes_on);
+  Edge<S> from_before, goes_on;
+  const int owes = owed<R, ONE, S>(p, e0, e1, from_before, goes_on);
   if (owes & 1) edge[0][0] = from_before;
   if (owes & 2) edge[W - 1][1] = goes_on;
 }
@@ -139,17 +139,16 @@ __device__ __noinline__ void drain(uint64_t *bar, int slots, int from, int to) {
   for (int i = from; i < to; i++) mbar_wait(bar + i % slots, i / slots & 1);
 }
 
-template <int D, int NT, int TYPE>
+template <int D, int NT, int TYPE, typename S>
 __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(const __grid_constant__ AttnArgs p) {
   using C = Cfg<D, NT>;
   constexpr int SPLIT = TYPE == APX_DTYPE_F32 ? 2 : 1;
   constexpr int W = C::kWarps, R = C::kRows, K4 = D / 32;  // words of K per thread and row
   constexpr bool ONE = NT == 1;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ unsigned s_pre[C::kThreads];
-  __shared__ unsigned long long s_warp[W];
+  __shared__ S s_pre[C::kThreads], s_warp[W];
   __shared__ __align__(8) uint64_t s_bar[W * C::kSlots];
-  __shared__ Edge s_edge[W][2];
+  __shared__ Edge<S> s_edge[W][2];
   __shared__ int s_last[2], s_most[W];
   __shared__ float s_inv[R];
 
@@ -164,10 +163,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
 
   // ---- the call's steps, summed over the sequences before each thread's share of them ----
   const int per = (p.n_seqs + C::kThreads - 1) / C::kThreads;
-  unsigned total;
+  S total;
   int longest = 0;
   {
-    unsigned long long run = 0;
+    S run = 0;
     int most = 0;
 #pragma unroll 1
     for (int i = 0; i < per; i++) {
@@ -177,29 +176,25 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
       q.load(p, s);
       if (q.bad && blockIdx.x == 0) attn_refuse(p, s, APX_ERR_INVALID_ARGUMENT);
       most = max(most, q.pair);
-      run += (unsigned long long)q.pairs() * q.pair * p.kv_heads;
+      run += q.template all<S>(p);
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long u = __shfl_up_sync(0xFFFFFFFFu, run, o);
+      const S u = __shfl_up_sync(0xFFFFFFFFu, run, o);
       if (lane >= o) run += u;
     }
     if (ONE) most = __reduce_max_sync(0xFFFFFFFFu, most);
     if (lane == 31) s_warp[warp] = run, s_most[warp] = most;
     __syncthreads();
-    unsigned long long before = 0, all = 0;
+    S before = 0, all = 0;
 #pragma unroll
     for (int i = 0; i < W; i++) {
       all += s_warp[i];
       longest = max(longest, s_most[i]);
       if (i < warp) before += s_warp[i];
     }
-    s_pre[tid] = (unsigned)(before + run);  // inclusive
-    if (all >> 32) {  // 2^37 keys: past any cache
-      if (tid == 0) attn_refuse(p, 0, APX_ERR_TOO_LARGE);
-      return;
-    }
-    total = (unsigned)all;
+    s_pre[tid] = before + run;  // inclusive
+    total = all;
     __syncthreads();
   }
   // Equal shares for every warp of the grid, the first `rem` one step more.  Or, while there are
@@ -207,31 +202,32 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   // saves the join through the workspace (0.5B shape, 777 keys: 13.5 -> 9.3 us).
   const int items = ONE ? p.n_seqs * p.kv_heads : 0;
   const bool whole_items = ONE && items <= (int)gridDim.x && longest <= 4 * W + kItemCost;
-  const unsigned nwarps = whole_items ? W : min(gridDim.x * W, max(total, 1u));
-  unsigned c0 = 0, c1 = total;
+  const unsigned nwarps =
+      whole_items ? W : (unsigned)min((S)(gridDim.x * W), max(total, (S)1));
+  S c0 = 0, c1 = total;
   if (whole_items) {
     if ((int)blockIdx.x >= items) return;
     const int s = blockIdx.x / p.kv_heads, h = blockIdx.x - s * p.kv_heads;
-    const unsigned s0 = s ? s_pre[s - 1] : 0, n = (s_pre[s] - s0) / (unsigned)p.kv_heads;
+    const S s0 = s ? s_pre[s - 1] : 0, n = (s_pre[s] - s0) / (unsigned)p.kv_heads;
     c0 = s0 + h * n;
     c1 = c0 + (n ? n - kItemCost : 0);
   }
-  const Shares<W> share(c0, c1, nwarps);
+  const Shares<W, S> share(c0, c1, nwarps);
   const unsigned w0 = whole_items ? 0 : blockIdx.x * W;  // this CTA's first warp
-  const unsigned u0 = share.bound(w0 + warp), u1 = share.bound(w0 + warp + 1);
+  const S u0 = share.bound(w0 + warp), u1 = share.bound(w0 + warp + 1);
 
   // ---- copies: step u0 + i into slot i of the ring, through every item of this warp ----
   const uint8_t *src = nullptr;  // lane i: tile i % 2 of step u0 + batch + i / 2; null: no such
   unsigned there = 0;            // which lanes' tiles are
   int batch = -16;
   const uint64_t policy = stream_policy();
-  auto look_ahead = [&](int i, Item c) {  // c: the item of step u0 + i, or one before
+  auto look_ahead = [&](int i, Item<S> c) {  // c: the item of step u0 + i, or one before
     batch = i;
     src = nullptr;
-    const unsigned g0 = u0 + i, g = g0 + lane / 2;
+    const S g0 = u0 + i, g = g0 + lane / 2;
     while (true) {
       if (c.real && g >= c.i0 && g < min(c.i1, u1)) {
-        const int key = c.key_of(g) + lane % 2 * kKvTile;
+        const int key = c.key_of((int)(g - c.i0)) + lane % 2 * kKvTile;
         if (key < c.end) {
           const int page = p.table[(size_t)c.seq * p.max_pages + (key >> p.page_shift)];
           if (page >= 0 && page < p.n_pages)
@@ -242,7 +238,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
         }
       }
       if (c.i1 >= min(g0 + 16, u1)) break;
-      c = find_item<R, ONE, C::kThreads>(p, s_pre, per, c.i1);
+      c = find_item<R, ONE, C::kThreads, S>(p, s_pre, per, c.i1);
     }
     there = __ballot_sync(0xFFFFFFFFu, src != nullptr);
   };
@@ -267,8 +263,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   const Unpack un;
 #pragma unroll 1
   while (at < mine && alive) {
-    const Item it = find_item<R, ONE, C::kThreads>(p, s_pre, per, u0 + at);
-    const int stop = (int)(min(it.i1, u1) - u0);
+    const Item<S> it = find_item<R, ONE, C::kThreads, S>(p, s_pre, per, u0 + at);
+    const int stop = (int)(min(it.i1, u1) - u0), before = (int)(u0 - it.i0);
     // the block's query rows, asked for before the first copies
     constexpr int QV = SPLIT == 2 ? D / 16 : D / 32;  // 16-byte loads a row and thread
     uint4 qraw[NT][QV];
@@ -379,7 +375,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
       arrived(at);
       uint8_t *tile = ring + (at & (C::kSlots - 1)) * C::kSlot;
       if (it.real) {  // not filling, which has no keys
-      const int key = it.key_of(u0 + at);
+      const int key = it.key_of(at + before);
       if (key + kStepKeys > end) {
         // tokens past the last key may hold anything: V's scales there count as zero (K's are
         // masked)
@@ -635,10 +631,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   }
 
   // ---- the join: items that cross warps, each by the warp that has its first part ----
-  const unsigned e0 = share.bound(w0), e1 = share.bound(w0 + W);  // this CTA's steps
+  const S e0 = share.bound(w0), e1 = share.bound(w0 + W);  // this CTA's steps
   if (__syncthreads_or(!alive)) {
     if (whole_items) return;
-    if (tid == 0) keep_owed<R, ONE, W>(p, e0, e1, s_edge);
+    if (tid == 0) keep_owed<R, ONE, W, S>(p, e0, e1, s_edge);
     __syncthreads();
   }
   constexpr int E = R * D / 4, Q = D / 4;             // quads of an item's rows, of a row
@@ -648,7 +644,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   auto add4 = [](float4 &v, float f, const float4 x) {
     v = make_float4(fmaf(f, x.x, v.x), fmaf(f, x.y, v.y), fmaf(f, x.z, v.z), fmaf(f, x.w, v.w));
   };
-  auto write4 = [&](const Edge &ed, int r, int d, const float4 v, float inv) {
+  auto write4 = [&](const Edge<S> &ed, int r, int d, const float4 v, float inv) {
     const int row = ed.row0 + r;
     if (row >= ed.rows) return;
     const int tok = by_group(p, row);
@@ -660,7 +656,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   {
     // a bit per warp: whose first edge, whose last edge is used
     const bool used = lane < W && s_edge[lane % W][0].used;
-    const unsigned begin = s_edge[lane % W][0].begin;
+    const S begin = s_edge[lane % W][0].begin;
     const unsigned firsts = __ballot_sync(0xFFFFFFFFu, used);
     unsigned starts = __ballot_sync(0xFFFFFFFFu, lane < W && s_edge[lane % W][1].used);
     // items here: the one that began before this CTA or at its first warp's first step, and each
@@ -676,12 +672,12 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
       }
       const bool head = (firsts & 1) && j < UNITS;
       const int w = head ? 0 : __ffs(starts) - 1, r = j % UNITS * U;
-      const Edge &ed = s_edge[w][head ? 0 : 1];
+      const Edge<S> &ed = s_edge[w][head ? 0 : 1];
       // its parts: this one and the first edges of the warps that follow
       const int n =
           __popc(__ballot_sync(0xFFFFFFFFu, used && lane > w && begin == ed.begin)) + 1;
       const float *first = part_of(w, head ? 0 : 1), *rest = part_of(w, 0);
-      constexpr int S = C::kWarpSmem / 4;  // from a warp's part to the next one's
+      constexpr int kNext = C::kWarpSmem / 4;  // from a warp's part to the next one's
       if constexpr (!ONE) {
         // lane: row r + lane % U, parts lane / U + i KG
         constexpr int KG = 32 / U, KR = (W + KG - 1) / KG;
@@ -689,7 +685,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
 #pragma unroll
         for (int i = 0; i < KR; i++) {
           const int k = lane / U + i * KG;
-          const float *mine = (k ? rest + min(k, n - 1) * S : first) + R * D + r + lane % U;
+          const float *mine = (k ? rest + min(k, n - 1) * kNext : first) + R * D + r + lane % U;
           m[i] = k < n ? mine[0] : -INFINITY, l[i] = k < n ? mine[R] : 0.0f;
           top = fmaxf(top, m[i]);
         }
@@ -719,7 +715,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
           for (int k = 1; k < W; k++) {
             if (k >= n) break;
             add4(v, __shfl_sync(0xFFFFFFFFu, f[k / KG], u + U * (k % KG)),
-                 *reinterpret_cast<const float4 *>(rest + k * S + (r + u) * D + d));
+                 *reinterpret_cast<const float4 *>(rest + k * kNext + (r + u) * D + d));
           }
           const float inv = __shfl_sync(0xFFFFFFFFu, scale, u);
           if (whole) write4(ed, r + u, d, v, inv);
@@ -727,7 +723,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
         }
         continue;
       }
-      const float *mine = (lane ? rest + min(lane, n - 1) * S : first) + R * D + r;
+      const float *mine = (lane ? rest + min(lane, n - 1) * kNext : first) + R * D + r;
       const float m = lane < n ? mine[0] : -INFINITY, l = lane < n ? mine[R] : 0.0f;
       float top = m;
 #pragma unroll
@@ -745,7 +741,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
 #pragma unroll 4
       for (int k = 1; k < n; k++)
         add4(v, __shfl_sync(0xFFFFFFFFu, f, k),
-             *reinterpret_cast<const float4 *>(rest + k * S + r * D + d));
+             *reinterpret_cast<const float4 *>(rest + k * kNext + r * D + d));
       if (lane >= Q) continue;
       if (ed.begin >= e0 && ed.end <= e1) {
         write4(ed, r, d, v, sum == 0.0f ? 0.0f : 1.0f / sum);
@@ -762,7 +758,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   // ---- items that cross CTAs: the CTA that arrives last joins their parts, in their order ----
   if (whole_items) return;
   int out_of_cta = 0;  // bit 0: an item began before this CTA; bit 1: one goes on after it
-  Edge edge0 = s_edge[0][0], edge1;
+  Edge<S> edge0 = s_edge[0][0], edge1;
   if (edge0.used && edge0.begin < e0) out_of_cta = 1;
   {
     const unsigned any = __ballot_sync(0xFFFFFFFFu, lane < W && (s_edge[lane % W][0].used ||
@@ -779,8 +775,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   if (tid < 2) {
     int n = 0;
     if (out_of_cta >> tid & 1) {
-      const unsigned begin = tid ? edge1.begin : edge0.begin;
-      const unsigned end = tid ? edge1.end : edge0.end;
+      const S begin = tid ? edge1.begin : edge0.begin;
+      const S end = tid ? edge1.end : edge0.end;
       const int a = share.cta_of(begin), all = share.cta_of(end - 1) - a + 1;
       if (atomicAdd(p.count + a, 1u) == (unsigned)all - 1) {
         n = all;
@@ -795,7 +791,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   for (int e = 0; e < 2; e++) {
     const int n = s_last[e];
     if (!n) continue;
-    const Edge ed = e ? edge1 : edge0;
+    const Edge<S> ed = e ? edge1 : edge0;
     const float *first = p.part + ((size_t)share.cta_of(ed.begin) * 2 + 1) * C::kPart;
     auto src_of = [&](int k) { return first + (k ? (size_t)(2 * k - 1) * C::kPart : 0); };
     // the parts' factors, then their sum by groups of threads, each a share of the parts; a
@@ -860,10 +856,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
   }
 }
 
-template <int D, int NT, int TYPE>
+template <int D, int NT, typename S, int TYPE>
 cudaError_t launch_split(const AttnArgs &p, int grid, cudaStream_t stream) {
   using C = Cfg<D, NT>;
-  auto kern = attn_split_kernel<D, NT, TYPE>;
+  auto kern = attn_split_kernel<D, NT, TYPE, S>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
@@ -879,11 +875,19 @@ cudaError_t launch_split(const AttnArgs &p, int grid, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-template <int D, int NT>
+template <int D, int NT, typename S>
 cudaError_t launch_type(const AttnArgs &p, int grid, cudaStream_t stream) {
-  if (p.type == APX_DTYPE_F32) return launch_split<D, NT, APX_DTYPE_F32>(p, grid, stream);
-  if (p.type == APX_DTYPE_F16) return launch_split<D, NT, APX_DTYPE_F16>(p, grid, stream);
-  return launch_split<D, NT, APX_DTYPE_BF16>(p, grid, stream);
+  if (p.type == APX_DTYPE_F32) return launch_split<D, NT, S, APX_DTYPE_F32>(p, grid, stream);
+  if (p.type == APX_DTYPE_F16) return launch_split<D, NT, S, APX_DTYPE_F16>(p, grid, stream);
+  return launch_split<D, NT, S, APX_DTYPE_BF16>(p, grid, stream);
+}
+
+template <int D>
+cudaError_t launch_rows(const AttnArgs &p, int grid, cudaStream_t stream) {
+  if ((long long)p.max_q * p.group <= Cfg<D, 1>::kRows && steps_fit<Cfg<D, 1>::kRows, true>(p))
+    return launch_type<D, 1, unsigned>(p, grid, stream);
+  if (steps_fit<Cfg<D, 2>::kRows, false>(p)) return launch_type<D, 2, unsigned>(p, grid, stream);
+  return launch_type<D, 2, unsigned long long>(p, grid, stream);
 }
 
 }  // namespace
@@ -927,10 +931,7 @@ cudaError_t launch_attn_kv4(const apx_attn_args &a, const apx_kv4_cache &c,
   p.group_mul = (unsigned)(0x100000000ull / (unsigned)p.group + 1);
   const int grid = std::min(sms, kCountBytes / 4);
   if (attn_tc_serves(p, c.head_dim, b.max_q)) return launch_attn_tc(p, c.head_dim, b.max_q, stream);
-  const bool one = (size_t)b.max_q * p.group <= 8;
-  if (c.head_dim == 128)
-    return one ? launch_type<128, 1>(p, grid, stream) : launch_type<128, 2>(p, grid, stream);
-  return one ? launch_type<64, 1>(p, grid, stream) : launch_type<64, 2>(p, grid, stream);
+  return c.head_dim == 128 ? launch_rows<128>(p, grid, stream) : launch_rows<64>(p, grid, stream);
 }
 
 }  // namespace apx

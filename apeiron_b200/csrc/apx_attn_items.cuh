@@ -8,6 +8,7 @@
 
 namespace apx {
 
+// S, throughout: the type of a step's number in its call (steps_fit).
 constexpr int kStepKeys = 32;
 // What a warp loses at an item's end (its rows to keep or write, the next one's to read), in steps:
 // items of single tokens carry as many steps without keys, so that warps with a boundary get fewer
@@ -44,41 +45,44 @@ struct SeqShape : SeqRows<R, kStepKeys> {
   __host__ __device__ __forceinline__ int pairs() const {
     return ONE ? (this->nblk > 0 ? 1 : 0) : (this->nblk + 1) / 2;
   }
+  template <typename S>
+  __host__ __device__ __forceinline__ S all(const AttnArgs &p) const {
+    return (S)pairs() * (unsigned)pair * (unsigned)p.kv_heads;
+  }
 };
 
 // One item: the steps [i0, i1) of a block of query rows of a KV head.  `real` is false for a pair's
 // filling, steps without keys.
+template <typename S>
 struct Item {
-  unsigned i0, i1;
+  S i0, i1;
   int seq, first, rows, p0;  // of its sequence: first query token, rows, position of row 0
   int head, row0;            // its KV head and first row
   int end, sink, from;       // its keys (SeqRows::range)
   bool real;
-  __host__ __device__ __forceinline__ int key_of(unsigned step) const {
-    const int st = (int)(step - i0);
+  __host__ __device__ __forceinline__ int key_of(int st) const {  // its step st
     return (st < sink ? st : st - sink + from) * kStepKeys;
   }
 };
 
 // The item of step g, which is a step of sequence `seq` or of one behind it; seq0: the steps of the
 // call before that sequence.
-template <int R, bool ONE>
-__host__ __device__ __forceinline__ Item item_from(const AttnArgs &p, int seq, unsigned seq0,
-                                                   unsigned g) {
-  unsigned seq1 = seq0;
+template <int R, bool ONE, typename S>
+__host__ __device__ __forceinline__ Item<S> item_from(const AttnArgs &p, int seq, S seq0, S g) {
+  S seq1 = seq0;
   SeqShape<R, ONE> q;
-  Item it;
+  Item<S> it;
   it.seq = seq - 1;
   do {
     seq0 = seq1;
     q.load(p, ++it.seq);
-    seq1 = seq0 + (unsigned)q.pairs() * q.pair * p.kv_heads;
+    seq1 = seq0 + q.template all<S>(p);
   } while (g >= seq1);
-  const unsigned nth = (g - seq0) / (unsigned)q.pair, n = q.pairs();
+  const unsigned nth = (unsigned)((g - seq0) / (unsigned)q.pair), n = q.pairs();
   it.head = (int)(ONE ? nth : nth / n);
   int blk = ONE ? 0 : (int)(nth - it.head * n);
-  it.i0 = seq0 + nth * q.pair;
-  const unsigned end = it.i0 + q.pair;
+  it.i0 = seq0 + (S)nth * q.pair;
+  const S end = it.i0 + q.pair;
   it.i1 = it.i0 + q.steps(p, blk);
   if (!ONE && g >= it.i1 && blk != q.nblk - 1 - blk) {
     blk = q.nblk - 1 - blk;
@@ -97,38 +101,50 @@ __host__ __device__ __forceinline__ Item item_from(const AttnArgs &p, int seq, u
 
 // The steps [c0, c1) dealt to `warps` warps of CTAs of W, in equal shares of `base`, the first
 // `rem` one more.
-template <int W>
+template <int W, typename S>
 struct Shares {
-  unsigned c0, warps, base, rem;
+  S c0, base;
+  unsigned warps, rem;
 
-  __host__ __device__ __forceinline__ Shares(unsigned c0, unsigned c1, unsigned warps)
-      : c0(c0), warps(warps), base((c1 - c0) / warps), rem((c1 - c0) - base * warps) {}
-  __host__ __device__ __forceinline__ unsigned bound(unsigned w) const {
+  __host__ __device__ __forceinline__ Shares(S c0, S c1, unsigned warps)
+      : c0(c0), base((c1 - c0) / warps), warps(warps), rem((unsigned)((c1 - c0) - base * warps)) {}
+  __host__ __device__ __forceinline__ S bound(unsigned w) const {
     return c0 + min(w, warps) * base + min(w, rem);
   }
   // The CTA that has `step`, where c0 is 0.
-  __host__ __device__ __forceinline__ int cta_of(unsigned step) const {
-    const unsigned wide = rem * (base + 1);
+  __host__ __device__ __forceinline__ int cta_of(S step) const {
+    const S wide = rem * (base + 1);
     return (int)((step < wide ? step / (base + 1) : rem + (step - wide) / base) / W);
   }
 };
 
 // One item that crosses a warp's boundary, kept for the join at the end of the CTA.
+template <typename S>
 struct Edge {
-  unsigned begin, end;          // the item's steps, numbered over the whole call
+  S begin, end;                 // the item's steps, numbered over the whole call
   int first, rows, head, row0;  // its sequence's first token and rows, its KV head and first row
   int used;
 };
-__host__ __device__ __forceinline__ Edge edge_of(const Item &it) {
-  return Edge{it.i0, it.i1, it.first, it.rows, it.head, it.row0, 1};
+template <typename S>
+__host__ __device__ __forceinline__ Edge<S> edge_of(const Item<S> &it) {
+  return Edge<S>{it.i0, it.i1, it.first, it.rows, it.head, it.row0, 1};
+}
+
+// Whether a call's steps, in blocks of R rows (ONE: one a sequence at most), stay below 2^32 whatever
+// its lengths are.  A prompt of a quarter of a million tokens with 8 KV heads of 8 query heads each
+// does not; with 64-bit numbers the windowed chunks in f32 take 50.2 us in place of 48.9.
+template <int R, bool ONE>
+inline bool steps_fit(const AttnArgs &p) {
+  const double room = (double)p.max_pages * (1 << p.page_shift);
+  const double blocks = ONE ? p.n_seqs : (double)p.n_tokens * p.group / R + 2.0 * p.n_seqs;
+  return blocks * p.kv_heads * (room / kStepKeys + 3 + kItemCost) < 4294967296.0;
 }
 
 // What the CTA of steps [e0, e1) owes to items that cross its ends, from the lengths alone: bit 0
 // for one that began before it (edge0), bit 1 for one that begins in it and goes on after (edge1).
-template <int R, bool ONE>
-__host__ __device__ inline int owed(const AttnArgs &p, unsigned e0, unsigned e1, Edge &edge0,
-                                    Edge &edge1) {
-  const Item a = item_from<R, ONE>(p, 0, 0, e0), b = item_from<R, ONE>(p, 0, 0, e1 - 1);
+template <int R, bool ONE, typename S>
+__host__ __device__ inline int owed(const AttnArgs &p, S e0, S e1, Edge<S> &edge0, Edge<S> &edge1) {
+  const Item<S> a = item_from<R, ONE, S>(p, 0, 0, e0), b = item_from<R, ONE, S>(p, 0, 0, e1 - 1);
   edge0 = edge_of(a);
   edge1 = edge_of(b);
   return (a.real && a.i0 < e0 ? 1 : 0) | (b.real && b.i0 >= e0 && b.i1 > e1 ? 2 : 0);

@@ -70,3 +70,35 @@ def test_attention_more_queries_than_max_q(ops, kind, q_lens, max_q):
         if n <= max_q:
             a, b = (t[cu[i]: cu[i + 1]].double() for t in (out, want))
             assert (a - b).abs().max() <= 2.0 ** -7 * b.abs().max()
+
+
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+@pytest.mark.parametrize("q_lens", [[70], [3, 1, 2], [1, 1, 1]])
+@pytest.mark.parametrize("window", [0, 50])
+def test_attention_steps_numbered_in_64_bits(ops, kind, q_lens, window):
+    """A table with room for more keys than 32 bits of steps: the call that numbers them in 64.  A
+    prompt's blocks get the bits they get with a small table; single tokens, which then go in blocks
+    of more rows, the same to f32's or the type's roundings."""
+    import torch
+    from apeiron_b200.step import KV4Cache, SeqBatch
+
+    rng = np.random.default_rng(len(q_lens))
+    n, heads = len(q_lens), 16
+    kv_lens = [n_q + 300 + 17 * i for i, n_q in enumerate(q_lens)]
+    small, table, n_pages = batch_of(q_lens, kv_lens, 128, rng)
+    wide = torch.zeros(n, 25_000_000 if n > 1 else 60_000_000, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = gpu(table)
+    batch = SeqBatch(small.cu, small.kv_len, wide, small.n_tokens, max(q_lens))
+    blocks = n if max(q_lens) == 1 else sum(q_lens) // 16 + 2 * n
+    assert blocks * heads * (wide.shape[1] * 128 // 32) >= 2 ** 32
+    cache = KV4Cache(gpu(random_pages(n_pages, heads, 64, 128, rng)), heads, 64, 128)
+    q = torch.randn(sum(q_lens), heads, 64, device="cuda").to(getattr(torch, kind))
+    status = ops.new_status()
+    got = ops.attn_kv4(q, cache, batch, 0.125, window=window, status=status)
+    want = ops.attn_kv4(q, cache, small, 0.125, window=window)
+    assert ops.check_status(status) is None
+    if max(q_lens) > 8:
+        assert torch.equal(got, want)
+    else:
+        off = (got.double() - want.double()).abs().max() / want.double().abs().max()
+        assert off <= (2.0 ** -16 if kind == "float32" else 2.0 ** -7)
