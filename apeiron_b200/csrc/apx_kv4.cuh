@@ -16,6 +16,8 @@ namespace apx {
 
 constexpr int kKvTile = 16;   // tokens of a tile
 constexpr int kKvGroup = 32;  // dims that share a scale
+// Cached tokens of a sequence at most: a step of keys past them still has its number in an int.
+constexpr int kMaxKvLen = INT32_MAX - 511;
 
 __host__ __device__ constexpr int kv4_tile_bytes(int dim) {
   return kKvTile * dim + 2 * kKvTile * (dim / kKvGroup) * 2;
@@ -117,7 +119,8 @@ struct SeqRows {
   __host__ __device__ void load(const AttnArgs &p, int s) {
     const int a = p.cu[s], b = p.cu[s + 1], n = p.kv_len[s];
     const long long room = (long long)p.max_pages << p.page_shift;
-    bad = a < 0 || b < a || b > p.n_tokens || b - a > p.max_q || n < 0 || n > room;
+    bad = a < 0 || b < a || b > p.n_tokens || b - a > p.max_q || n < 0 || n > room ||
+          n > kMaxKvLen;
     first = a;
     rows = bad ? 0 : (b - a) * p.group;
     kv = bad ? 0 : n;

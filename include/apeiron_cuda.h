@@ -551,7 +551,7 @@ APX_API size_t apx_kv4_page_bytes(int head_dim, int page_tokens);
 
 /* The requests of one call.  Sequence s has the query tokens d_cu[s] .. d_cu[s + 1] - 1 of the
  * call's n_tokens rows (d_cu[0] = 0, ascending, d_cu[n_seqs] = n_tokens) and d_kv_len[s] cached
- * tokens, the query tokens being the last of them: query i stands at position
+ * tokens (2^31 - 512 at most), the query tokens being the last of them: query i stands at position
  * d_kv_len[s] - (d_cu[s + 1] - d_cu[s]) + i.  max_q bounds a sequence's query tokens: attention
  * refuses a sequence with more. */
 typedef struct apx_seq_batch {

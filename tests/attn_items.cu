@@ -158,7 +158,33 @@ static void check_long_calls() {
   if (!steps_fit<8, true>(d.p)) fail("requests", 0, 60, 0);
 }
 
+// Lengths up to the limit have their steps in ints, on both kernels; past it a sequence is refused.
+static void check_longest() {
+  Call c;
+  c.cu.push_back(40);
+  c.kv.push_back(kMaxKvLen);
+  c.finish(1, 1, 7);
+  for (int window : {0, 1, kMaxKvLen - 3, INT32_MAX}) {
+    c.p.window = window;
+    SeqShape<16, false> q;
+    q.load(c.p, 0);
+    SeqRows<256, 128> t;
+    t.load(c.p, 0);
+    int end, sink, from;
+    t.range(c.p, 0, end, sink, from);
+    if (q.bad || t.bad || q.steps(c.p, 0) <= 0 || q.pair < q.steps(c.p, 0) + q.steps(c.p, 1) ||
+        end != kMaxKvLen || t.steps_to(end) <= from)
+      fail("the longest", window, q.pair, from);
+  }
+  c.kv[0]++;
+  c.p.max_pages++;
+  SeqRows<256, 128> t;
+  t.load(c.p, 0);
+  if (!t.bad) fail("past the longest", 0, c.kv[0], 0);
+}
+
 int main() {
+  check_longest();
   check_long_calls();
   for (int round = 0; round < 400; round++) {
     std::mt19937 rng(round);
