@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
     while (true) {
       if (c.real && g >= c.i0 && g < min(c.i1, u1)) {
         const int key = c.key_of((int)(g - c.i0)) + lane % 2 * kKvTile;
-        if (key < c.end) {
+        if (key < c.end && !unseen(p, key, kKvTile, c.low)) {
           const int page = p.table[(size_t)c.seq * p.max_pages + (key >> p.page_shift)];
           if (page >= 0 && page < p.n_pages)
             src = p.pages + ((unsigned long long)page * p.kv_heads + c.head) * p.page_bytes +
@@ -376,11 +376,12 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
       uint8_t *tile = ring + (at & (C::kSlots - 1)) * C::kSlot;
       if (it.real) {  // not filling, which has no keys
       const int key = it.key_of(at + before);
-      if (key + kStepKeys > end) {
-        // tokens past the last key may hold anything: V's scales there count as zero (K's are
-        // masked)
+      const bool behind = key < all_lo && key + kStepKeys > p.sinks;  // some row's window
+      if (key + kStepKeys > end || behind) {
+        // tokens past the last key or behind the window may hold anything: V's scales there count
+        // as zero (K's are masked)
         __syncwarp();
-        if (key + lane >= end)
+        if (key + lane >= end || unseen(p, key + lane, 1, it.low))
 #pragma unroll
           for (int g = 0; g < D / kKvGroup; g++)
             *reinterpret_cast<uint16_t *>(tile + lane / kKvTile * C::kTile + kv4_vs_off(D) +
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1) attn_split_kernel(con
               s[t][n][j] = (SPLIT == 2 ? s[t][n][j] + lo[t][n][j] : s[t][n][j]) * cq[n][j & 1];
       }
       // masks, where some row does not see all 32 keys
-      if (key + kStepKeys - 1 > all_hi || (key < all_lo && key + kStepKeys > p.sinks)) {
+      if (key + kStepKeys - 1 > all_hi || behind) {
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll

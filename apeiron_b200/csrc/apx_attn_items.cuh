@@ -38,9 +38,9 @@ struct SeqShape : SeqRows<R, kStepKeys> {
     }
   }
   __host__ __device__ __forceinline__ int steps(const AttnArgs &p, int b) const {
-    int end, sink, from;
-    this->range(p, b, end, sink, from);
-    return max(sink + max(Base::steps_to(end) - from, 0), 1);  // one writes unseeing rows' zeros
+    int end, sink, low;
+    this->range(p, b, end, sink, low);
+    return max(sink + max(Base::steps_to(end) - low / kStepKeys, 0), 1);  // one writes unseeing rows' zeros
   }
   __host__ __device__ __forceinline__ int pairs() const {
     return ONE ? (this->nblk > 0 ? 1 : 0) : (this->nblk + 1) / 2;
@@ -58,10 +58,10 @@ struct Item {
   S i0, i1;
   int seq, first, rows, p0;  // of its sequence: first query token, rows, position of row 0
   int head, row0;            // its KV head and first row
-  int end, sink, from;       // its keys (SeqRows::range)
+  int end, sink, low;        // its keys (SeqRows::range)
   bool real;
   __host__ __device__ __forceinline__ int key_of(int st) const {  // its step st
-    return (st < sink ? st : st - sink + from) * kStepKeys;
+    return (st < sink ? st : st - sink + (int)((unsigned)low / kStepKeys)) * kStepKeys;
   }
 };
 
@@ -95,7 +95,7 @@ __host__ __device__ __forceinline__ Item<S> item_from(const AttnArgs &p, int seq
   it.rows = q.rows;
   it.p0 = q.p0;
   it.row0 = blk * R;
-  q.range(p, blk, it.end, it.sink, it.from);
+  q.range(p, blk, it.end, it.sink, it.low);
   return it;
 }
 

@@ -146,8 +146,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     attn_refuse(p, seq, APX_ERR_INVALID_ARGUMENT);
   const int blk = (int)(gridDim.y - 1 - blockIdx.y);  // the longest first
   if (blk >= q.nblk) return;  // with its whole cluster
-  int end, sink, from;
-  q.range(p, blk, end, sink, from);
+  int end, sink, low;
+  q.range(p, blk, end, sink, low);
+  const int from = low / kKeys;
   // this CTA's share of the block's steps: [j0, j0 + n)
   const int all = sink + max(q.steps_to(end) - from, 0);
   const int split = all >= ctas ? ctas : 1;  // too few steps: all of them here
@@ -489,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int *table = p.table + (size_t)seq * p.max_pages;
     auto find = [&](int j) {  // the page of this thread's tile at step j
       const int key = key_of(j) + tile * kKvTile;
-      if (j >= n || key >= end) return -1;
+      if (j >= n || key >= end || unseen(p, key, kKvTile, low)) return -1;
       const int pg = table[key >> p.page_shift];
       if (pg >= 0 && pg < p.n_pages) return pg;
       attn_refuse(p, seq, APX_ERR_INVALID_ARGUMENT);
@@ -572,13 +573,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             a[0][4 + k] = un.low2(w >> 8, u2h(s1));
             a[1][4 + k] = un.high2(w >> 8, u2h(s1));
           }
-          if (!have || first + kKvTile > end) {  // tokens past the last key may hold anything
+          if (!have || first + kKvTile > end || first < low) {
+            // tokens past the last key or behind the window may hold anything
+            auto gone = [&](int key) { return !have || key >= end || unseen(p, key, 1, low); };
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
               for (int k = 0; k < 8; k++) {
-                if (!have || first + 2 * k >= end) a[h][k] &= 0xFFFF0000u;
-                if (!have || first + 2 * k + 1 >= end) a[h][k] &= 0x0000FFFFu;
+                if (gone(first + 2 * k)) a[h][k] &= 0xFFFF0000u;
+                if (gone(first + 2 * k + 1)) a[h][k] &= 0x0000FFFFu;
               }
           }
 #pragma unroll

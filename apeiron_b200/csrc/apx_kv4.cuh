@@ -102,6 +102,11 @@ __host__ __device__ __forceinline__ int window_start(const AttnArgs &p, int pos)
   return p.window == 0 || pos < p.window ? 0 : pos - p.window + 1;
 }
 
+// Whether the n keys from `key` on are all behind every window that starts at `low` or later.
+__host__ __device__ __forceinline__ bool unseen(const AttnArgs &p, int key, int n, int low) {
+  return key + n <= low && key >= p.sinks;
+}
+
 // A power of two that brings a row's largest |q| to [2^9, 2^10) (exponents outside the f32
 // normals are clamped), as its exponent's distance: q 2^(9 - e).
 __device__ __forceinline__ int row_exponent(float top) {
@@ -128,15 +133,13 @@ struct SeqRows {
     nblk = (rows + R - 1) / R;
   }
   __host__ __device__ static int steps_to(int n) { return (max(n, 0) + KEYS - 1) / KEYS; }
-  // Block b sees keys below `end`: those of the sinks' steps [0, sink) and of steps `from` on.
-  __host__ __device__ void range(const AttnArgs &p, int b, int &end, int &sink, int &from) const {
+  // Block b sees keys below `end`: those of the sinks' steps [0, sink) and of steps low / KEYS on;
+  // of these none from the sinks' end up to `low`, whose pages may be gone (unseen).
+  __host__ __device__ void range(const AttnArgs &p, int b, int &end, int &sink, int &low) const {
     const int lo = p0 + by_group(p, b * R), hi = p0 + by_group(p, min((b + 1) * R - 1, rows - 1));
     end = max(min(kv, hi + 1), 0);
-    sink = from = 0;
-    if (p.window) {
-      from = window_start(p, lo) / KEYS;
-      sink = min(steps_to(min(p.sinks, end)), from);
-    }
+    low = window_start(p, lo);
+    sink = p.window ? min(steps_to(min(p.sinks, end)), low / KEYS) : 0;
   }
 };
 

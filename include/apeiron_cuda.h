@@ -615,8 +615,9 @@ APX_API int apx_rope_kv4_append_async(apx_ctx *ctx, const apx_rope_args *args,
 /* Attention of the batch's query tokens over the cache: out = softmax(scale * q k^T) v per query
  * head (n_heads a multiple of n_kv_heads; query head h reads KV head h / (n_heads /
  * n_kv_heads)).  The query at position p sees key j <= p when window is 0 or j > p - window or
- * j < sinks.  A query that sees no key gets zeros.  Keys past d_kv_len never take part, whatever
- * the pages hold there.  q and out share one type.  For APX_DTYPE_F32 the products carry 22 bits
+ * j < sinks.  A query that sees no key gets zeros.  Keys past d_kv_len, and those behind the windows
+ * of all queries of their sequence, never take part, whatever the pages hold there; a page of such
+ * keys alone may be gone, its number in the table anything.  q and out share one type.  For APX_DTYPE_F32 the products carry 22 bits
  * of q and of the probabilities (one below 2^-38 of its row's largest counts as zero), the sums
  * f32; for the 16-bit types the probabilities are rounded to 11 bits before the product with v.
  * Uses a context workspace: calls on one context must not overlap in time.

@@ -170,11 +170,11 @@ static void check_longest() {
     q.load(c.p, 0);
     SeqRows<256, 128> t;
     t.load(c.p, 0);
-    int end, sink, from;
-    t.range(c.p, 0, end, sink, from);
+    int end, sink, low;
+    t.range(c.p, 0, end, sink, low);
     if (q.bad || t.bad || q.steps(c.p, 0) <= 0 || q.pair < q.steps(c.p, 0) + q.steps(c.p, 1) ||
-        end != kMaxKvLen || t.steps_to(end) <= from)
-      fail("the longest", window, q.pair, from);
+        end != kMaxKvLen || t.steps_to(end) <= low / 128)
+      fail("the longest", window, q.pair, low);
   }
   c.kv[0]++;
   c.p.max_pages++;

@@ -102,3 +102,52 @@ def test_attention_steps_numbered_in_64_bits(ops, kind, q_lens, window):
     else:
         off = (got.double() - want.double()).abs().max() / want.double().abs().max()
         assert off <= (2.0 ** -16 if kind == "float32" else 2.0 ** -7)
+
+
+# ---- pages behind every window ---------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["float32", "float16"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (64, 32), (128, 64), (64, 128)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (33, 0), (100, 5), (64, 20), (250, 16)])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1, 1], [300, 7, 1000]), ([9, 3], [400, 350]),
+                                            ([60, 20], [500, 300]), ([260], [800])])
+def test_attention_without_the_pages_behind_the_window(ops, kind, dim, page, window, sinks, q_lens,
+                                                       kv_lens):
+    """Pages of which no query sees a key are out of the table: numbers outside the cache, or a page
+    whose scales are NaN.  The other values behind the windows are NaN too."""
+    import torch
+    from apeiron_b200.step import KV4Cache, SeqBatch
+
+    rng = np.random.default_rng(window + dim)
+    b, table, n_pages = batch_of(q_lens, kv_lens, page, rng)
+    pages = random_pages(n_pages, 2, dim, page, rng)
+    q = gpu(rng.standard_normal((sum(q_lens), 4, dim)).astype(np.float32)).to(getattr(torch, kind))
+    want, reach, spread = ref.attention(q.double().cpu().numpy(), pages, table, q_lens, kv_lens,
+                                        page, 0.2, window, sinks)
+    left = table.copy()
+    free = [p for p in range(n_pages) if p not in table]
+    pages[free] = 0xFF
+    tiles = pages.reshape(n_pages, 2, page // 16, -1)
+    for s, (nq, nk) in enumerate(zip(q_lens, kv_lens)):
+        low = nk - nq - window + 1
+        for j in range(sinks, low):  # the scales of every unseen token
+            at = 16 * dim + (np.arange(2 * dim // 32)[:, None] * 16 + j % 16) * 2 + np.arange(2)
+            tiles[table[s, j // page], :, j % page // 16, at.ravel()] = 0xFF
+        for i in range(table.shape[1]):
+            if i * page >= sinks and (i + 1) * page <= low:
+                left[s, i] = rng.choice([-1, n_pages, 1 << 30, free[0]])
+    if max(q_lens) < 100:
+        assert (left != table).any() or window == 250
+    cache = KV4Cache(gpu(pages), 2, dim, page)
+    status = ops.new_status()
+    out = ops.attn_kv4(q, cache, SeqBatch(b.cu, b.kv_len, gpu(left), sum(q_lens), max(q_lens)), 0.2,
+                       window=window, sinks=sinks, status=status)
+    assert ops.check_status(status) is None
+    got = out.double().cpu().numpy()
+    # check_attention's bounds
+    most = 8 * 0.3 * np.exp(0.4 * 6)
+    tol = (2.0 ** -21 * spread + 2.0 ** -20)[..., None] * reach + 2.0 ** -38 * max(kv_lens) * most
+    if kind != "float32":
+        tol = tol + 2.0 ** -11 * reach + 2.0 ** -25 * max(kv_lens) * most
+        tol = tol + 2.0 ** -11 * np.abs(want) + 2.0 ** -24
+    assert np.isfinite(got).all() and (np.abs(got - want) <= tol).all()
