@@ -501,14 +501,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       return p.pages + ((unsigned long long)pg * p.kv_heads + head) * p.page_bytes +
              (unsigned)((key & ((1 << p.page_shift) - 1)) / kKvTile) * kv4_tile_bytes(D);
     };
+    // plain loads: the kernel that writes the pages may still run when this one starts, and the
+    // read-only path promises nothing then
     auto load_k = [&](int j) {
       if (page < 0) return;
       const uint8_t *src = source(j, page);
 #pragma unroll
       for (int i = 0; i < K16; i++) {
-        kraw[i] = __ldg(reinterpret_cast<const uint4 *>(src + tok * (D / 2) + part * (D / 4)) + i);
-        ksc[i] = __ldg(reinterpret_cast<const __half *>(src + kv4_ks_off(D)) +
-                       (part * K16 + i) * kKvTile + tok);
+        kraw[i] = reinterpret_cast<const uint4 *>(src + tok * (D / 2) + part * (D / 4))[i];
+        ksc[i] = reinterpret_cast<const __half *>(
+            src + kv4_ks_off(D))[(part * K16 + i) * kKvTile + tok];
       }
     };
     auto load_v = [&](int j) {
@@ -516,12 +518,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint8_t *src = source(j, page);
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        vraw[i] = __ldg(reinterpret_cast<const uint2 *>(src + kv4_v_off(D)) +
-                        (mq * 32 + g * 4 + i) * 2 + part);
+        vraw[i] = reinterpret_cast<const uint2 *>(
+            src + kv4_v_off(D))[(mq * 32 + g * 4 + i) * 2 + part];
 #pragma unroll
       for (int i = 0; i < 2; i++)  // a group of 32 dims, 16 tokens
-        vsc[i] = __ldg(reinterpret_cast<const uint4 *>(src + kv4_vs_off(D)) +
-                       (mq * 2 + part) * 2 + i);
+        vsc[i] = reinterpret_cast<const uint4 *>(src + kv4_vs_off(D))[(mq * 2 + part) * 2 + i];
     };
     page = find(0);
     load_k(0);

@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM)
     const unsigned i = v0 + 4 * (j * kThreads + tid);
     float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     if (quads && i + 4 <= v1) {
-      f = __ldg(reinterpret_cast<const float4 *>(x + i));
+      f = *reinterpret_cast<const float4 *>(x + i);  // not the read-only path: pdl_wait's data
     } else {
       if (i < v1) f.x = x[i];
       if (i + 1 < v1) f.y = x[i + 1];

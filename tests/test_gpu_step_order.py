@@ -47,3 +47,60 @@ def test_norm_weights_from_the_call_before(ops, n, rows, before):
         torch.cuda.synchronize()
         ops.add_rms_norm_quant(x, weights, 1e-6, y=want)
         assert torch.equal(out[i], want)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 1000), (1, 16000), (3, 40000), (40, 32003)])
+def test_sampler_logits_from_the_call_before(ops, rows, vocab):
+    """The logits are what the norm before has written."""
+    import torch
+
+    rng = np.random.default_rng(vocab)
+    sources = gpu(rng.standard_normal((30, rows, vocab)).astype(np.float32))
+    logits = torch.zeros(rows, vocab, device="cuda")
+    u = torch.rand(30, rows, device="cuda")
+    token = torch.empty(30, rows, dtype=torch.int32, device="cuda")
+    top_k = torch.full((rows,), 40, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    for i in range(30):
+        ops.add_rms_norm_quant(sources[i], None, 1e-6, y=logits)
+        ops.sample(logits, u[i], top_k=top_k, token=token[i])
+    torch.cuda.synchronize()
+    for i in range(30):
+        ops.add_rms_norm_quant(sources[i], None, 1e-6, y=logits)
+        torch.cuda.synchronize()
+        assert torch.equal(ops.sample(logits, u[i], top_k=top_k), token[i])
+
+
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+@pytest.mark.parametrize("nq", [1, 16, 200])
+def test_attention_over_pages_of_the_call_before(ops, kind, nq):
+    """The keys and values are those that the append before has written over others."""
+    import torch
+    from apeiron_b200.step import KV4Cache, SeqBatch
+
+    rng = np.random.default_rng(nq)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    dt = getattr(torch, kind)
+    batch = SeqBatch(torch.tensor([0, nq], **i32), torch.tensor([nq], **i32),
+                     torch.arange(-(-nq // 16), **i32)[None].contiguous(), nq, nq)
+    cache = KV4Cache.empty(-(-nq // 16), 2, 64, 16)
+    qkv = gpu(rng.standard_normal((30, nq, 12, 64)).astype(np.float32))
+    table = ops.rope_table(nq, 64)
+    q = torch.empty(nq, 8, 64, device="cuda", dtype=dt)
+    out = torch.empty(30, nq, 8, 64, device="cuda", dtype=dt)
+    torch.cuda.synchronize()
+
+    def step(i, out, wait):
+        ops.rope_kv4_append(qkv[i, :, :8], qkv[i, :, 8:10], qkv[i, :, 10:], table, cache, batch,
+                            rot_dim=64, q_out=q)
+        if wait:
+            torch.cuda.synchronize()
+        ops.attn_kv4(q, cache, batch, 0.125, out=out)
+
+    for i in range(30):
+        step(i, out[i], False)
+    torch.cuda.synchronize()
+    want = torch.empty_like(q)
+    for i in range(30):
+        step(i, want, True)
+        assert torch.equal(out[i], want)
