@@ -561,7 +561,9 @@ apx_ctx *apx_open(int device, apx_err *err) {
   }
   const size_t attn = attn_work_bytes(ctx->sm_count);
   e = ctx->attn_work.ensure(attn);
-  if (e == cudaSuccess) e = cudaMemset(ctx->attn_work.p, 0, attn);
+  if (e == cudaSuccess) e = cudaMemsetAsync(ctx->attn_work.p, 0, attn, ctx->stream);
+  // the first call may come on any stream
+  if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
   if (e != cudaSuccess) {
     ctx->attn_work.release();
     cudaStreamDestroy(ctx->stream);

@@ -104,3 +104,27 @@ def test_attention_over_pages_of_the_call_before(ops, kind, nq):
     for i in range(30):
         step(i, want, True)
         assert torch.equal(out[i], want)
+
+
+def test_attention_in_a_context_just_opened(ops):
+    """The first call of a context, at once and on a stream that waits for no other: its keys are
+    split over the GPU and joined through counters that start at zero."""
+    import torch
+    from apeiron_b200 import Backend
+    from apeiron_b200.step import KV4Cache, SeqBatch, StepOps
+
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cache = KV4Cache(torch.randint(0, 100, (200, 1, 1152), dtype=torch.uint8, device="cuda"), 1, 64, 16)
+    batch = SeqBatch(torch.tensor([0, 1], **i32), torch.tensor([3200], **i32),
+                     torch.arange(200, **i32)[None].contiguous(), 1, 1)
+    q = torch.randn(1, 4, 64, device="cuda")
+    want = ops.attn_kv4(q, cache, batch, 0.1)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        be = Backend(0)
+        out = StepOps(be).attn_kv4(q, cache, batch, 0.1, out=torch.empty_like(q),
+                                   stream=side.cuda_stream)
+        side.synchronize()
+        assert torch.equal(out, want)
+        be.close()
