@@ -4,7 +4,8 @@ and the sampler (include/apeiron_cuda.h states each of them).
 
 ``StepOps`` checks its tensors, queues one asynchronous call on the current torch stream (or the
 ``stream`` given, a raw handle) and returns without waiting; outputs may be passed in and are
-allocated otherwise.  A refused argument raises ``ValueError``, a backend condition
+allocated otherwise, for the stream that the call goes to (as under ``torch.cuda.stream``: to use
+them on another one, wait for it and tell the allocator with ``record_stream``).  A refused argument raises ``ValueError``, a backend condition
 ``BackendError``.  What only the device sees (a page number outside the cache, a value that has no
 4-bit image) goes to the optional ``status`` words of ``new_status``, read with ``check_status``.
 """
@@ -83,12 +84,11 @@ class DeviceAct:
         self.k, self.n = codes.shape[0], n
 
     @classmethod
-    def empty(cls, ops: "StepOps", k: int, n: int) -> "DeviceAct":
+    def empty(cls, ops: "StepOps", k: int, n: int, stream=None) -> "DeviceAct":
         pad = ops.lib.apx_act_padded_len(n)
-        dev = ops.device
-        return cls(torch.empty(k, pad, dtype=torch.int8, device=dev),
-                   torch.empty(k, pad // 32, dtype=torch.uint8, device=dev),
-                   torch.empty(k, 8, dtype=torch.int32, device=dev), n)
+        return cls(ops._empty((k, pad), torch.int8, stream),
+                   ops._empty((k, pad // 32), torch.uint8, stream),
+                   ops._empty((k, 8), torch.int32, stream), n)
 
 
 class KV4Cache:
@@ -150,6 +150,13 @@ class StepOps:
     def _stream(self, stream):
         return _raw_stream(self._index) if stream is None else stream
 
+    def _empty(self, shape, dtype, stream):
+        """An output of a call on `stream`: memory that earlier work on that stream is done with."""
+        if stream is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
+            return torch.empty(shape, dtype=dtype, device=self.device)
+
     @staticmethod
     def _failed(rc, name):
         if rc in (_abi.APX_ERR_INVALID_ARGUMENT, _abi.APX_ERR_LAYOUT_MISMATCH,
@@ -177,7 +184,7 @@ class StepOps:
         shape = x.shape
         k, n = shape
         if act is None and deq is None and y is None:
-            act = DeviceAct.empty(self, k, n)
+            act = DeviceAct.empty(self, k, n, stream)
         codes = exps = descs = 0
         if act is not None:
             _need(act.n == n and act.k == k, f"act: ({k}, {n}) is wanted")
@@ -200,7 +207,7 @@ class StepOps:
                    high=4.0, original=0.0, mscale=1.0, stream=None):
         """(n_pos, rot_dim / 2, 2) f32 cosines and sines; ``scaling``: None, "linear", "bands" or
         "ramp" (``low`` and ``high``: turns within the ``original`` length)."""
-        table = torch.empty(n_pos, rot_dim // 2, 2, dtype=_F32, device=self.device)
+        table = self._empty((n_pos, rot_dim // 2, 2), _F32, stream)
         _need(scaling in _SCALINGS, f"scaling: one of {list(_SCALINGS)} is wanted")
         f = _abi.RopeFreqs(base, factor, low, high, original, mscale, rot_dim,
                            _SCALINGS[scaling])
@@ -222,7 +229,7 @@ class StepOps:
         if q is not None:
             shape = (t, q.shape[1], dim)
             if q_out is None:
-                q_out = torch.empty(shape, dtype=q_type, device=q.device)
+                q_out = self._empty(shape, q_type, stream)
             ldq, n_heads = _rows(q, shape, "q", _F32), shape[1]
             ld_out, kind = _rows(q_out, shape, "q_out", q_out.dtype), _TYPES.get(q_out.dtype, -1)
             q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
@@ -245,7 +252,7 @@ class StepOps:
         heads, dtype = q.shape[1], q.dtype
         shape = (batch.n_tokens, heads, cache.head_dim)
         if out is None:
-            out = torch.empty(shape, dtype=dtype, device=q.device)
+            out = self._empty(shape, dtype, stream)
         rc = self._attn(self.ctx, _ATTN(
             q.data_ptr(), out.data_ptr(), _vector(status, 2, _I64, "status"),
             _rows(q, shape, "q", dtype), _rows(out, shape, "out", dtype),
@@ -262,7 +269,7 @@ class StepOps:
         shape = logits.shape
         rows, vocab = shape
         if token is None:
-            token = torch.empty(rows, dtype=_I32, device=logits.device)
+            token = self._empty(rows, _I32, stream)
         rc = self._sample(self.ctx, _SAMPLE(
             logits.data_ptr(), _vector(u, rows, _F32, "u"),
             _vector(temperature, rows, _F32, "temperature"), _vector(top_p, rows, _F32, "top_p"),

@@ -128,3 +128,51 @@ def test_attention_in_a_context_just_opened(ops):
         side.synchronize()
         assert torch.equal(out, want)
         be.close()
+
+
+@pytest.mark.parametrize("call", ["norm", "table", "append", "attention", "sample"])
+def test_outputs_on_another_stream(ops, call):
+    """What a call on a given stream allocates is not memory that the current stream, which it does
+    not wait for, still has to write: here late, over blocks of the same sizes that are free again."""
+    import torch
+    from apeiron_b200.step import KV4Cache, SeqBatch
+
+    rng = np.random.default_rng(0)
+    t = 300
+    i32 = dict(dtype=torch.int32, device="cuda")
+    x = gpu(rng.standard_normal((t, 12, 64)).astype(np.float32))
+    cache = KV4Cache.empty(20, 2, 64, 16)
+    batch = SeqBatch(torch.tensor([0, t], **i32), torch.tensor([t], **i32),
+                     torch.arange(20, **i32)[None].contiguous(), t, t)
+    table = ops.rope_table(t, 64)
+    u = torch.rand(t, device="cuda")
+    side = torch.cuda.Stream()
+
+    def run(stream):
+        if call == "norm":
+            act = ops.add_rms_norm_quant(x.flatten(1), None, 1e-6, stream=stream)
+            return act.codes, act.exps, act.descs
+        if call == "table":
+            return (ops.rope_table(t, 64, stream=stream),)
+        if call == "append":
+            return (ops.rope_kv4_append(x[:, :8], x[:, 8:10], x[:, 10:], table, cache, batch,
+                                        rot_dim=64, stream=stream),)
+        if call == "attention":
+            return (ops.attn_kv4(x[:, :8], cache, batch, 0.1, stream=stream),)
+        return (ops.sample(x.flatten(1), u, stream=stream),)
+
+    ops.rope_kv4_append(None, x[:, 8:10], x[:, 10:], table, cache, batch, rot_dim=64)
+    torch.cuda.synchronize()
+    want = [w.clone() for w in run(None)]
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    late = [torch.empty_like(w) for w in want for _ in range(3)]
+    torch.cuda._sleep(100_000_000)
+    for m in late:
+        m.fill_(1)
+    del m, late
+    got = run(side.cuda_stream)
+    side.synchronize()
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
