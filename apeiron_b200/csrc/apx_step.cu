@@ -9,6 +9,19 @@ namespace {
 
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+// Queues a launch on the context's device, whichever is current: kernels go to the current one, and
+// a default stream says nothing of it.
+template <typename Launch>
+int on_device(const apx_ctx *ctx, Launch launch) {
+  const int dev = apx::context_device(ctx);
+  int now = -1;
+  if (cudaGetDevice(&now) != cudaSuccess || (now != dev && cudaSetDevice(dev) != cudaSuccess))
+    return APX_ERR_CUDA;
+  const cudaError_t e = launch();
+  if (now != dev) cudaSetDevice(now);
+  return e == cudaSuccess ? APX_OK : APX_ERR_CUDA;
+}
+
 // The cache's geometry: APX_OK, or why it is not served.
 int check_cache(const apx_kv4_cache *c) {
   if (!c || c->n_kv_heads <= 0) return APX_ERR_INVALID_ARGUMENT;
@@ -51,8 +64,7 @@ int apx_add_rms_norm_quant_async(apx_ctx *ctx, const apx_norm_args *a, void *str
       (any && !(a->d_codes && a->d_exps && a->d_descs)) || !aligned(a->d_codes, 4) ||
       !aligned(a->d_descs, 16) || !(a->eps >= 0.0f))
     return APX_ERR_INVALID_ARGUMENT;
-  return apx::launch_add_rms_norm_quant(*a, (cudaStream_t)stream) == cudaSuccess ? APX_OK
-                                                                                 : APX_ERR_CUDA;
+  return on_device(ctx, [&] { return apx::launch_add_rms_norm_quant(*a, (cudaStream_t)stream); });
 }
 
 int apx_rope_table_async(apx_ctx *ctx, const apx_rope_freqs *f, size_t n_pos, float *d_table,
@@ -66,9 +78,8 @@ int apx_rope_table_async(apx_ctx *ctx, const apx_rope_freqs *f, size_t n_pos, fl
   if (n_pos > (size_t)INT32_MAX || f->rot_dim > 4096) return APX_ERR_TOO_LARGE;
   if (n_pos == 0 || f->rot_dim == 0) return APX_OK;
   if (!d_table || !aligned(d_table, 8)) return APX_ERR_INVALID_ARGUMENT;
-  return apx::launch_rope_table(*f, n_pos, d_table, (cudaStream_t)stream) == cudaSuccess
-             ? APX_OK
-             : APX_ERR_CUDA;
+  return on_device(
+      ctx, [&] { return apx::launch_rope_table(*f, n_pos, d_table, (cudaStream_t)stream); });
 }
 
 int apx_rope_kv4_append_async(apx_ctx *ctx, const apx_rope_args *a, const apx_kv4_cache *c,
@@ -94,9 +105,8 @@ int apx_rope_kv4_append_async(apx_ctx *ctx, const apx_rope_args *a, const apx_kv
        !aligned(a->d_q, 16) || !aligned(a->d_q_out, 16) || a->q_type < APX_DTYPE_F32 ||
        a->q_type > APX_DTYPE_BF16))
     return APX_ERR_INVALID_ARGUMENT;
-  return apx::launch_rope_kv4_append(*a, *c, *b, (cudaStream_t)stream) == cudaSuccess
-             ? APX_OK
-             : APX_ERR_CUDA;
+  return on_device(
+      ctx, [&] { return apx::launch_rope_kv4_append(*a, *c, *b, (cudaStream_t)stream); });
 }
 
 int apx_attn_kv4_async(apx_ctx *ctx, const apx_attn_args *a, const apx_kv4_cache *c,
@@ -117,9 +127,8 @@ int apx_attn_kv4_async(apx_ctx *ctx, const apx_attn_args *a, const apx_kv4_cache
     return APX_ERR_INVALID_ARGUMENT;
   int sms;
   void *work = apx::context_attn_work(ctx, &sms);
-  return apx::launch_attn_kv4(*a, *c, *b, work, sms, (cudaStream_t)stream) == cudaSuccess
-             ? APX_OK
-             : APX_ERR_CUDA;
+  return on_device(
+      ctx, [&] { return apx::launch_attn_kv4(*a, *c, *b, work, sms, (cudaStream_t)stream); });
 }
 
 int apx_sample_async(apx_ctx *ctx, const apx_sample_args *a, void *stream) {
@@ -128,7 +137,7 @@ int apx_sample_async(apx_ctx *ctx, const apx_sample_args *a, void *stream) {
   if (a->rows == 0) return APX_OK;
   if (!a->d_logits || !a->d_u || !a->d_token || a->vocab == 0 || a->ld < a->vocab)
     return APX_ERR_INVALID_ARGUMENT;
-  return apx::launch_sample(*a, (cudaStream_t)stream) == cudaSuccess ? APX_OK : APX_ERR_CUDA;
+  return on_device(ctx, [&] { return apx::launch_sample(*a, (cudaStream_t)stream); });
 }
 
 }  // extern "C"

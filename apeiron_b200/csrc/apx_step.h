@@ -25,6 +25,8 @@ cudaError_t launch_attn_kv4(const apx_attn_args &a, const apx_kv4_cache &c,
 // apx_runtime.cu: the context's attention workspace (attn_work_bytes, zeroed when the context was
 // opened) and its SM count.
 void *context_attn_work(apx_ctx *ctx, int *sms);
+// The context's device.
+int context_device(const apx_ctx *ctx);
 
 // apx_sample.cu
 cudaError_t launch_sample(const apx_sample_args &a, cudaStream_t stream);

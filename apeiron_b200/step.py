@@ -5,9 +5,10 @@ and the sampler (include/apeiron_cuda.h states each of them).
 ``StepOps`` checks its tensors, queues one asynchronous call on the current torch stream (or the
 ``stream`` given, a raw handle) and returns without waiting; outputs may be passed in and are
 allocated otherwise, for the stream that the call goes to (as under ``torch.cuda.stream``: to use
-them on another one, wait for it and tell the allocator with ``record_stream``).  A refused argument raises ``ValueError``, a backend condition
-``BackendError``.  What only the device sees (a page number outside the cache, a value that has no
-4-bit image) goes to the optional ``status`` words of ``new_status``, read with ``check_status``.
+them on another one, wait for it and tell the allocator with ``record_stream``).  A refused argument
+raises ``ValueError``, a backend condition ``BackendError``.  What only the device sees (a page number
+outside the cache, a value that has no 4-bit image) goes to the optional ``status`` words of
+``new_status``, read with ``check_status``.
 """
 from __future__ import annotations
 
@@ -41,19 +42,20 @@ def _need(ok, what):
         raise ValueError(what)
 
 
-def _vector(t, n, dtype, name):
-    """The address of a contiguous vector of n elements; 0 for None."""
+def _vector(t, n, dtype, name, dev):
+    """The address of a contiguous vector of n elements on GPU `dev`; 0 for None."""
     if t is None:
         return 0
-    if not (t.dtype is dtype and t.numel() == n and t.is_cuda and t.is_contiguous()):
-        raise ValueError(f"{name}: a contiguous CUDA tensor of {n} {dtype} elements is wanted")
+    if not (t.dtype is dtype and t.numel() == n and t.get_device() == dev and t.is_contiguous()):
+        raise ValueError(f"{name}: a contiguous tensor of {n} {dtype} elements on cuda:{dev} is "
+                         "wanted")
     return t.data_ptr()
 
 
-def _rows(t, shape, name, dtype):
-    """The elements between rows of a tensor of `shape` (2 or 3 dims, rows first) whose rows are
-    each contiguous."""
-    if t.dtype is dtype and t.is_cuda and t.shape == shape:
+def _rows(t, shape, name, dtype, dev):
+    """The elements between rows of a tensor of `shape` (2 or 3 dims, rows first) on GPU `dev` whose
+    rows are each contiguous."""
+    if t.dtype is dtype and t.get_device() == dev and t.shape == shape:
         st = t.stride()
         if len(st) == 2:
             width = shape[1]
@@ -69,8 +71,8 @@ def _rows(t, shape, name, dtype):
                     return st[0]
                 if shape[0] <= 1:
                     return width
-    raise ValueError(f"{name}: a CUDA tensor {tuple(shape)} of {dtype} is wanted, its rows "
-                     "contiguous and apart")
+    raise ValueError(f"{name}: a tensor {tuple(shape)} of {dtype} on cuda:{dev} is wanted, its "
+                     "rows contiguous and apart")
 
 
 class DeviceAct:
@@ -94,7 +96,7 @@ class DeviceAct:
 class KV4Cache:
     """A layer's paged 4-bit cache over ``pages``: uint8 (n_pages, n_kv_heads, page bytes)."""
 
-    __slots__ = ("pages", "struct", "ref", "n_kv_heads", "head_dim")
+    __slots__ = ("pages", "struct", "ref", "n_kv_heads", "head_dim", "dev")
 
     def __init__(self, pages, n_kv_heads: int, head_dim: int, page_tokens: int):
         size = self.page_bytes(head_dim, page_tokens)
@@ -103,6 +105,7 @@ class KV4Cache:
               and pages.shape[1:] == (n_kv_heads, size) and pages.data_ptr() % 16 == 0,
               f"pages: a contiguous CUDA uint8 tensor (n, {n_kv_heads}, {size}) is wanted")
         self.pages, self.n_kv_heads, self.head_dim = pages, n_kv_heads, head_dim
+        self.dev = pages.get_device()
         self.struct = _abi.Kv4Cache(pages.data_ptr(), pages.shape[0], n_kv_heads, head_dim,
                                     page_tokens, 0)
         self.ref = C.byref(self.struct)
@@ -123,21 +126,24 @@ class SeqBatch:
     the query tokens last, ``table`` (n, max_pages) page numbers, all int32; ``n_tokens`` query
     tokens in all, at most ``max_q`` of one request."""
 
-    __slots__ = ("cu", "kv_len", "table", "n_tokens", "struct", "ref")
+    __slots__ = ("cu", "kv_len", "table", "n_tokens", "struct", "ref", "dev")
 
     def __init__(self, cu, kv_len, table, n_tokens: int, max_q: int):
-        n = kv_len.numel()
+        n, dev = kv_len.numel(), kv_len.get_device()
+        _need(dev >= 0, "kv_len: a CUDA tensor is wanted")
         _need(table.dim() == 2 and table.shape[0] == n, "table: one row per request is wanted")
         self.cu, self.kv_len, self.table, self.n_tokens = cu, kv_len, table, n_tokens
-        self.struct = _abi.SeqBatch(_vector(cu, n + 1, torch.int32, "cu"),
-                                    _vector(kv_len, n, torch.int32, "kv_len"),
-                                    _vector(table, table.numel(), torch.int32, "table"),
+        self.dev = dev
+        self.struct = _abi.SeqBatch(_vector(cu, n + 1, torch.int32, "cu", dev),
+                                    _vector(kv_len, n, torch.int32, "kv_len", dev),
+                                    _vector(table, table.numel(), torch.int32, "table", dev),
                                     n_tokens, n, table.shape[1], max_q, 0)
         self.ref = C.byref(self.struct)
 
 
 class StepOps:
-    """The calls, on one backend context.  Calls on one context must not overlap in time."""
+    """The calls, on one backend context and its GPU, whichever is current.  Calls on one context
+    must not overlap in time."""
 
     def __init__(self, backend: Backend):
         self.backend, self.lib, self.ctx = backend, backend.lib, backend.ctx
@@ -149,6 +155,10 @@ class StepOps:
 
     def _stream(self, stream):
         return _raw_stream(self._index) if stream is None else stream
+
+    def _here(self, cache, batch):
+        if not (cache.dev == batch.dev == self._index):
+            raise ValueError(f"cache and batch on cuda:{self._index} are wanted")
 
     def _empty(self, shape, dtype, stream):
         """An output of a call on `stream`: memory that earlier work on that stream is done with."""
@@ -181,7 +191,7 @@ class StepOps:
         """h = x + add into ``resid`` (may be x), h * weight / rms(h) into ``y`` (f32), ``act``
         (a DeviceAct, allocated when no output is given) and ``deq`` (the activation's values,
         f32 or bf16).  x, add: (k, n) f32; weight: n f32, or None.  Returns act."""
-        shape = x.shape
+        shape, dev = x.shape, self._index
         k, n = shape
         if act is None and deq is None and y is None:
             act = DeviceAct.empty(self, k, n, stream)
@@ -190,14 +200,15 @@ class StepOps:
             _need(act.n == n and act.k == k, f"act: ({k}, {n}) is wanted")
             codes, exps, descs = act.codes.data_ptr(), act.exps.data_ptr(), act.descs.data_ptr()
         rc = self._norm(self.ctx, _NORM(
-            x.data_ptr(), 0 if add is None else add.data_ptr(), _vector(weight, n, _F32, "weight"),
+            x.data_ptr(), 0 if add is None else add.data_ptr(),
+            _vector(weight, n, _F32, "weight", dev),
             0 if resid is None else resid.data_ptr(), 0 if y is None else y.data_ptr(),
             0 if deq is None else deq.data_ptr(), codes, exps, descs, n, k,
-            _rows(x, shape, "x", _F32),
-            0 if add is None else _rows(add, shape, "add", _F32),
-            0 if resid is None else _rows(resid, shape, "resid", _F32),
-            0 if y is None else _rows(y, shape, "y", _F32),
-            0 if deq is None else _rows(deq, shape, "deq", deq.dtype), eps,
+            _rows(x, shape, "x", _F32, dev),
+            0 if add is None else _rows(add, shape, "add", _F32, dev),
+            0 if resid is None else _rows(resid, shape, "resid", _F32, dev),
+            0 if y is None else _rows(y, shape, "y", _F32, dev),
+            0 if deq is None else _rows(deq, shape, "deq", deq.dtype, dev), eps,
             0 if deq is None else _TYPES.get(deq.dtype, -1)), self._stream(stream))
         if rc:
             self._failed(rc, "add_rms_norm_quant")
@@ -223,22 +234,25 @@ class StepOps:
         """q (tokens, heads, dim; None to leave out) turned into ``q_out``; k turned and v
         (tokens, kv heads, dim) appended to the cache in 4 bits.  ``k_deq`` / ``v_deq`` (f16):
         the values the cache now holds.  Returns q_out."""
-        t, heads, dim = batch.n_tokens, cache.n_kv_heads, cache.head_dim
+        self._here(cache, batch)
+        t, heads, dim, dev = batch.n_tokens, cache.n_kv_heads, cache.head_dim, self._index
         kv = (t, heads, dim)
         ldq = ld_out = n_heads = kind = q_ptr = out_ptr = 0
         if q is not None:
             shape = (t, q.shape[1], dim)
             if q_out is None:
                 q_out = self._empty(shape, q_type, stream)
-            ldq, n_heads = _rows(q, shape, "q", _F32), shape[1]
-            ld_out, kind = _rows(q_out, shape, "q_out", q_out.dtype), _TYPES.get(q_out.dtype, -1)
+            ldq, n_heads = _rows(q, shape, "q", _F32, dev), shape[1]
+            ld_out = _rows(q_out, shape, "q_out", q_out.dtype, dev)
+            kind = _TYPES.get(q_out.dtype, -1)
             q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         n_pos, n = table.shape[0], t * heads * dim
         rc = self._rope(self.ctx, _ROPE(
-            q_ptr, k.data_ptr(), v.data_ptr(), _vector(table, n_pos * rot_dim, _F32, "table"),
-            out_ptr, _vector(k_deq, n, torch.float16, "k_deq"),
-            _vector(v_deq, n, torch.float16, "v_deq"), _vector(status, 2, _I64, "status"),
-            n_pos, ldq, _rows(k, kv, "k", _F32), _rows(v, kv, "v", _F32), ld_out,
+            q_ptr, k.data_ptr(), v.data_ptr(),
+            _vector(table, n_pos * rot_dim, _F32, "table", dev),
+            out_ptr, _vector(k_deq, n, torch.float16, "k_deq", dev),
+            _vector(v_deq, n, torch.float16, "v_deq", dev), _vector(status, 2, _I64, "status", dev),
+            n_pos, ldq, _rows(k, kv, "k", _F32, dev), _rows(v, kv, "v", _F32, dev), ld_out,
             rot_dim, _LAYOUTS.get(layout, -1), n_heads, kind), cache.ref, batch.ref,
             self._stream(stream))
         if rc:
@@ -249,13 +263,14 @@ class StepOps:
                  out=None, status=None, stream=None):
         """softmax(scale * q k^T) v of q (tokens, heads, dim; f32, f16 or bf16) over the cache,
         causal, within ``window`` keys (0: all) and the first ``sinks``.  Returns out."""
-        heads, dtype = q.shape[1], q.dtype
+        self._here(cache, batch)
+        heads, dtype, dev = q.shape[1], q.dtype, self._index
         shape = (batch.n_tokens, heads, cache.head_dim)
         if out is None:
             out = self._empty(shape, dtype, stream)
         rc = self._attn(self.ctx, _ATTN(
-            q.data_ptr(), out.data_ptr(), _vector(status, 2, _I64, "status"),
-            _rows(q, shape, "q", dtype), _rows(out, shape, "out", dtype),
+            q.data_ptr(), out.data_ptr(), _vector(status, 2, _I64, "status", dev),
+            _rows(q, shape, "q", dtype, dev), _rows(out, shape, "out", dtype, dev),
             _TYPES.get(dtype, -1), heads, scale, window, sinks, 0), cache.ref, batch.ref,
             self._stream(stream))
         if rc:
@@ -266,17 +281,18 @@ class StepOps:
                token=None, prob=None, kept=None, stream=None):
         """One token per row of f32 ``logits`` (rows, vocab) from ``u`` (rows) in [0, 1); the
         filters are per row, None to leave out.  Returns token (int32)."""
-        shape = logits.shape
+        shape, dev = logits.shape, self._index
         rows, vocab = shape
         if token is None:
             token = self._empty(rows, _I32, stream)
         rc = self._sample(self.ctx, _SAMPLE(
-            logits.data_ptr(), _vector(u, rows, _F32, "u"),
-            _vector(temperature, rows, _F32, "temperature"), _vector(top_p, rows, _F32, "top_p"),
-            _vector(min_p, rows, _F32, "min_p"), _vector(top_k, rows, _I32, "top_k"),
-            _vector(token, rows, _I32, "token"), _vector(prob, rows, _F32, "prob"),
-            _vector(kept, rows, _I32, "kept"), rows, vocab,
-            _rows(logits, shape, "logits", _F32)), self._stream(stream))
+            logits.data_ptr(), _vector(u, rows, _F32, "u", dev),
+            _vector(temperature, rows, _F32, "temperature", dev),
+            _vector(top_p, rows, _F32, "top_p", dev), _vector(min_p, rows, _F32, "min_p", dev),
+            _vector(top_k, rows, _I32, "top_k", dev),
+            _vector(token, rows, _I32, "token", dev), _vector(prob, rows, _F32, "prob", dev),
+            _vector(kept, rows, _I32, "kept", dev), rows, vocab,
+            _rows(logits, shape, "logits", _F32, dev)), self._stream(stream))
         if rc:
             self._failed(rc, "sample")
         return token
