@@ -76,14 +76,20 @@ def _rows(t, shape, name, dtype, dev):
 
 
 class DeviceAct:
-    """An activation as the projections read it: int8 codes, exponent bytes and descriptors of k
-    columns (the layout of ``apx_quant_f32_cols_async``)."""
+    """An activation as the projections read it: int8 codes (k, padded n), exponent bytes and
+    descriptors (k, 8 int32) of k columns (the layout of ``apx_quant_f32_cols_async``)."""
 
-    __slots__ = ("codes", "exps", "descs", "k", "n")
+    __slots__ = ("codes", "exps", "descs", "k", "n", "dev")
 
     def __init__(self, codes, exps, descs, n):
         self.codes, self.exps, self.descs = codes, exps, descs
-        self.k, self.n = codes.shape[0], n
+        self.k, self.n, self.dev = codes.shape[0], n, codes.get_device()
+        pad = _abi.load().apx_act_padded_len(n)
+        _need(self.dev >= 0 and codes.shape == (self.k, pad), f"codes: int8 ({self.k}, {pad}) on a "
+              "GPU are wanted")
+        _vector(codes, self.k * pad, torch.int8, "codes", self.dev)
+        _vector(exps, self.k * (pad // 32), torch.uint8, "exps", self.dev)
+        _vector(descs, self.k * 8, torch.int32, "descs", self.dev)
 
     @classmethod
     def empty(cls, ops: "StepOps", k: int, n: int, stream=None) -> "DeviceAct":
@@ -197,7 +203,8 @@ class StepOps:
             act = DeviceAct.empty(self, k, n, stream)
         codes = exps = descs = 0
         if act is not None:
-            _need(act.n == n and act.k == k, f"act: ({k}, {n}) is wanted")
+            _need(act.n == n and act.k == k and act.dev == dev,
+                  f"act: ({k}, {n}) on cuda:{dev} is wanted")
             codes, exps, descs = act.codes.data_ptr(), act.exps.data_ptr(), act.descs.data_ptr()
         rc = self._norm(self.ctx, _NORM(
             x.data_ptr(), 0 if add is None else add.data_ptr(),

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from apeiron_b200 import _abi, build
-from apeiron_b200.step import KV4Cache, SeqBatch, StepOps
+from apeiron_b200.step import DeviceAct, KV4Cache, SeqBatch, StepOps
 
 
 class Fake:
@@ -119,3 +119,30 @@ def test_caches_and_batches_of_another_gpu(ops):
     for kw in (dict(table_dev=0), dict(cu_dev=0), dict(dev=-1)):
         with pytest.raises(ValueError):
             batch(**kw)
+
+
+def test_activations_of_the_wrong_size(ops):
+    """A DeviceAct from a caller's own tensors holds what the kernels write."""
+    pad = ops.lib.apx_act_padded_len(100)
+    right = dict(codes=Fake((3, pad), torch.int8, 1), exps=Fake((3, pad // 32), torch.uint8, 1),
+                 descs=Fake((3, 8), I32, 1))
+    x = Fake((3, 100), dev=1)
+    act = DeviceAct(**right, n=100)
+    ops.reached.clear()
+    assert ops.add_rms_norm_quant(x, None, 1e-6, act=act, stream=0) is act
+    assert ops.reached == ["_norm"]
+    for name, wrong in (
+            ("codes", Fake((3, 100), torch.int8, 1)), ("codes", Fake((3, pad), torch.uint8, 1)),
+            ("codes", Fake((3, pad), torch.int8, -1)), ("codes", Fake((3 * pad,), torch.int8, 1)),
+            ("exps", Fake((3, pad // 32 - 1), torch.uint8, 1)), ("exps", Fake((3, pad), torch.int8, 1)),
+            ("exps", Fake((3, pad // 32), torch.uint8, 0)),
+            ("descs", Fake((3, 4), I32, 1)), ("descs", Fake((2, 8), I32, 1)),
+            ("descs", Fake((3, 8), torch.int64, 1))):
+        with pytest.raises(ValueError):
+            DeviceAct(**{**right, name: wrong}, n=100)
+    other = DeviceAct(**{k: Fake(t.shape, t.dtype, 0) for k, t in right.items()}, n=100)
+    with pytest.raises(ValueError):
+        ops.add_rms_norm_quant(x, None, 1e-6, act=other, stream=0)
+    with pytest.raises(ValueError):  # of 100 lanes for rows of 99
+        ops.add_rms_norm_quant(Fake((3, 99), dev=1), None, 1e-6, act=act, stream=0)
+    assert ops.reached == ["_norm"]
