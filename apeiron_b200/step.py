@@ -6,8 +6,8 @@ and the sampler (include/apeiron_cuda.h states each of them).
 ``stream`` given, a raw handle) and returns without waiting; outputs may be passed in and are
 allocated otherwise, for the stream that the call goes to (as under ``torch.cuda.stream``: to use
 them on another one, wait for it and tell the allocator with ``record_stream``).  A refused argument
-raises ``ValueError``, a backend condition ``BackendError``.  What only the device sees (a page number
-outside the cache, a value that has no 4-bit image) goes to the optional ``status`` words of
+raises ``ValueError``, a backend condition ``BackendError``.  What only the device sees (a page
+number outside the cache, a value that has no 4-bit image) goes to the optional ``status`` words of
 ``new_status``, read with ``check_status``.
 """
 from __future__ import annotations
@@ -32,6 +32,9 @@ _NORM = struct.Struct("@9P7Nfi").pack
 _ROPE = struct.Struct("@8P5N4i").pack
 _ATTN = struct.Struct("@3P2N2if3i0P").pack
 _SAMPLE = struct.Struct("@9P3N").pack
+# what packing raises for a number that its field does not hold
+_PACK_ERRORS = (struct.error, OverflowError)
+_INT_MAX = 2 ** 31 - 1
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
@@ -105,7 +108,9 @@ class KV4Cache:
     __slots__ = ("pages", "struct", "ref", "n_kv_heads", "head_dim", "dev")
 
     def __init__(self, pages, n_kv_heads: int, head_dim: int, page_tokens: int):
-        size = self.page_bytes(head_dim, page_tokens)
+        size = 0
+        if 0 < head_dim <= _INT_MAX and 0 < page_tokens <= _INT_MAX:
+            size = self.page_bytes(head_dim, page_tokens)
         _need(size > 0, f"head_dim {head_dim} with pages of {page_tokens} tokens is not served")
         _need(pages.is_cuda and pages.dtype is torch.uint8 and pages.is_contiguous()
               and pages.shape[1:] == (n_kv_heads, size) and pages.data_ptr() % 16 == 0,
@@ -137,6 +142,8 @@ class SeqBatch:
     def __init__(self, cu, kv_len, table, n_tokens: int, max_q: int):
         n, dev = kv_len.numel(), kv_len.get_device()
         _need(dev >= 0, "kv_len: a CUDA tensor is wanted")
+        _need(0 <= n_tokens <= _INT_MAX and 0 <= max_q <= _INT_MAX,
+              f"{n_tokens} query tokens, at most {max_q} of a request: not served")
         _need(table.dim() == 2 and table.shape[0] == n, "table: one row per request is wanted")
         self.cu, self.kv_len, self.table, self.n_tokens = cu, kv_len, table, n_tokens
         self.dev = dev
@@ -206,17 +213,20 @@ class StepOps:
             _need(act.n == n and act.k == k and act.dev == dev,
                   f"act: ({k}, {n}) on cuda:{dev} is wanted")
             codes, exps, descs = act.codes.data_ptr(), act.exps.data_ptr(), act.descs.data_ptr()
-        rc = self._norm(self.ctx, _NORM(
-            x.data_ptr(), 0 if add is None else add.data_ptr(),
-            _vector(weight, n, _F32, "weight", dev),
-            0 if resid is None else resid.data_ptr(), 0 if y is None else y.data_ptr(),
-            0 if deq is None else deq.data_ptr(), codes, exps, descs, n, k,
-            _rows(x, shape, "x", _F32, dev),
-            0 if add is None else _rows(add, shape, "add", _F32, dev),
-            0 if resid is None else _rows(resid, shape, "resid", _F32, dev),
-            0 if y is None else _rows(y, shape, "y", _F32, dev),
-            0 if deq is None else _rows(deq, shape, "deq", deq.dtype, dev), eps,
-            0 if deq is None else _TYPES.get(deq.dtype, -1)), self._stream(stream))
+        try:
+            rc = self._norm(self.ctx, _NORM(
+                x.data_ptr(), 0 if add is None else add.data_ptr(),
+                _vector(weight, n, _F32, "weight", dev),
+                0 if resid is None else resid.data_ptr(), 0 if y is None else y.data_ptr(),
+                0 if deq is None else deq.data_ptr(), codes, exps, descs, n, k,
+                _rows(x, shape, "x", _F32, dev),
+                0 if add is None else _rows(add, shape, "add", _F32, dev),
+                0 if resid is None else _rows(resid, shape, "resid", _F32, dev),
+                0 if y is None else _rows(y, shape, "y", _F32, dev),
+                0 if deq is None else _rows(deq, shape, "deq", deq.dtype, dev), eps,
+                0 if deq is None else _TYPES.get(deq.dtype, -1)), self._stream(stream))
+        except _PACK_ERRORS as e:
+            raise ValueError(f"add_rms_norm_quant: {e}") from None
         if rc:
             self._failed(rc, "add_rms_norm_quant")
         return act
@@ -225,6 +235,8 @@ class StepOps:
                    high=4.0, original=0.0, mscale=1.0, stream=None):
         """(n_pos, rot_dim / 2, 2) f32 cosines and sines; ``scaling``: None, "linear", "bands" or
         "ramp" (``low`` and ``high``: turns within the ``original`` length)."""
+        _need(0 <= n_pos <= _INT_MAX and 0 <= rot_dim <= _INT_MAX,
+              f"a table of {n_pos} positions for {rot_dim} dims is not served")
         table = self._empty((n_pos, rot_dim // 2, 2), _F32, stream)
         _need(scaling in _SCALINGS, f"scaling: one of {list(_SCALINGS)} is wanted")
         f = _abi.RopeFreqs(base, factor, low, high, original, mscale, rot_dim,
@@ -254,14 +266,17 @@ class StepOps:
             kind = _TYPES.get(q_out.dtype, -1)
             q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         n_pos, n = table.shape[0], t * heads * dim
-        rc = self._rope(self.ctx, _ROPE(
-            q_ptr, k.data_ptr(), v.data_ptr(),
-            _vector(table, n_pos * rot_dim, _F32, "table", dev),
-            out_ptr, _vector(k_deq, n, torch.float16, "k_deq", dev),
-            _vector(v_deq, n, torch.float16, "v_deq", dev), _vector(status, 2, _I64, "status", dev),
-            n_pos, ldq, _rows(k, kv, "k", _F32, dev), _rows(v, kv, "v", _F32, dev), ld_out,
-            rot_dim, _LAYOUTS.get(layout, -1), n_heads, kind), cache.ref, batch.ref,
-            self._stream(stream))
+        try:
+            rc = self._rope(self.ctx, _ROPE(
+                q_ptr, k.data_ptr(), v.data_ptr(),
+                _vector(table, n_pos * rot_dim, _F32, "table", dev),
+                out_ptr, _vector(k_deq, n, torch.float16, "k_deq", dev),
+                _vector(v_deq, n, torch.float16, "v_deq", dev),
+                _vector(status, 2, _I64, "status", dev), n_pos, ldq, _rows(k, kv, "k", _F32, dev), _rows(v, kv, "v", _F32, dev), ld_out,
+                rot_dim, _LAYOUTS.get(layout, -1), n_heads, kind), cache.ref, batch.ref,
+                self._stream(stream))
+        except _PACK_ERRORS as e:
+            raise ValueError(f"rope_kv4_append: {e}") from None
         if rc:
             self._failed(rc, "rope_kv4_append")
         return q_out
@@ -275,11 +290,14 @@ class StepOps:
         shape = (batch.n_tokens, heads, cache.head_dim)
         if out is None:
             out = self._empty(shape, dtype, stream)
-        rc = self._attn(self.ctx, _ATTN(
-            q.data_ptr(), out.data_ptr(), _vector(status, 2, _I64, "status", dev),
-            _rows(q, shape, "q", dtype, dev), _rows(out, shape, "out", dtype, dev),
-            _TYPES.get(dtype, -1), heads, scale, window, sinks, 0), cache.ref, batch.ref,
-            self._stream(stream))
+        try:
+            rc = self._attn(self.ctx, _ATTN(
+                q.data_ptr(), out.data_ptr(), _vector(status, 2, _I64, "status", dev),
+                _rows(q, shape, "q", dtype, dev), _rows(out, shape, "out", dtype, dev),
+                _TYPES.get(dtype, -1), heads, scale, window, sinks, 0), cache.ref, batch.ref,
+                self._stream(stream))
+        except _PACK_ERRORS as e:
+            raise ValueError(f"attn_kv4: {e}") from None
         if rc:
             self._failed(rc, "attn_kv4")
         return out

@@ -146,3 +146,32 @@ def test_activations_of_the_wrong_size(ops):
     with pytest.raises(ValueError):  # of 100 lanes for rows of 99
         ops.add_rms_norm_quant(Fake((3, 99), dev=1), None, 1e-6, act=act, stream=0)
     assert ops.reached == ["_norm"]
+
+
+def test_numbers_that_no_field_holds(ops):
+    """Numbers past the C structs' fields are refused as other arguments are, not cut to them."""
+    x, q, k = Fake((4, 64), dev=1), Fake((4, 4, 64), dev=1), Fake((4, 2, 64), dev=1)
+    table = Fake((16, 32, 2), dev=1)
+    ops.reached.clear()
+    for eps in (1e39, -1e39):
+        with pytest.raises(ValueError):
+            ops.add_rms_norm_quant(x, None, eps, y=x, stream=0)
+    for kw in (dict(window=2 ** 31), dict(window=2 ** 63), dict(sinks=2 ** 31), dict(window=3.5),
+               dict(scale=1e39)):
+        with pytest.raises(ValueError):
+            ops.attn_kv4(q, cache(), batch(), kw.pop("scale", 1.0), out=q, stream=0, **kw)
+    for rot in (2 ** 31, 2 ** 32 + 64):
+        with pytest.raises(ValueError):
+            ops.rope_kv4_append(None, k, k, table, cache(), batch(), rot_dim=rot, stream=0)
+    for n_pos, rot in ((-1, 64), (4, -8), (4, 2 ** 32 + 64), (2 ** 32, 64)):
+        with pytest.raises(ValueError):
+            ops.rope_table(n_pos, rot, stream=0)
+    assert not ops.reached
+    i32 = lambda *s: Fake(s, I32, 1)  # noqa: E731
+    for n, most in ((2 ** 32 + 4, 4), (4, 2 ** 32 + 4), (-1, 4), (4, -1)):
+        with pytest.raises(ValueError):
+            SeqBatch(i32(2), i32(1), i32(1, 4), n, most)
+    pages = Fake((8, 2, KV4Cache.page_bytes(64, 16)), torch.uint8, 1)
+    for dim, tokens in ((2 ** 32 + 64, 16), (64, 2 ** 32 + 16), (64, -16)):
+        with pytest.raises(ValueError):
+            KV4Cache(pages, 2, dim, tokens)
