@@ -150,16 +150,12 @@ def test_activations_of_the_wrong_size(ops):
 
 def test_numbers_that_no_field_holds(ops):
     """Numbers past the C structs' fields are refused as other arguments are, not cut to them."""
-    x, q, k = Fake((4, 64), dev=1), Fake((4, 4, 64), dev=1), Fake((4, 2, 64), dev=1)
+    q, k = Fake((4, 4, 64), dev=1), Fake((4, 2, 64), dev=1)
     table = Fake((16, 32, 2), dev=1)
     ops.reached.clear()
-    for eps in (1e39, -1e39):
+    for kw in (dict(window=2 ** 31), dict(window=2 ** 63), dict(sinks=2 ** 31), dict(window=3.5)):
         with pytest.raises(ValueError):
-            ops.add_rms_norm_quant(x, None, eps, y=x, stream=0)
-    for kw in (dict(window=2 ** 31), dict(window=2 ** 63), dict(sinks=2 ** 31), dict(window=3.5),
-               dict(scale=1e39)):
-        with pytest.raises(ValueError):
-            ops.attn_kv4(q, cache(), batch(), kw.pop("scale", 1.0), out=q, stream=0, **kw)
+            ops.attn_kv4(q, cache(), batch(), 1.0, out=q, stream=0, **kw)
     for rot in (2 ** 31, 2 ** 32 + 64):
         with pytest.raises(ValueError):
             ops.rope_kv4_append(None, k, k, table, cache(), batch(), rot_dim=rot, stream=0)
