@@ -63,10 +63,16 @@ __device__ __forceinline__ void store4f(float *p, size_t j, size_t n, bool quads
   if (j + 3 < n) p[j + 3] = v.w;
 }
 
-// (s, c) += h^2, c the rest of the roundings: s - t is exact once s is half its end.
+// (s, c) += h^2, c the rest of the roundings, for s >= h^2: then t <= 2 s and s - t is exact.
 __device__ __forceinline__ void add_square(float &s, float &c, float h) {
   const float t = __fmaf_rn(h, h, s);
   c += __fmaf_rn(h, h, __fsub_rn(s, t));
+  s = t;
+}
+// The same for any s: the sum's rest by Knuth's two-sum, the square's by the fused product.
+__device__ __forceinline__ void add_any_square(float &s, float &c, float h) {
+  const float p = __fmul_rn(h, h), t = __fadd_rn(s, p), b = __fsub_rn(t, s);
+  c += __fadd_rn(__fadd_rn(__fsub_rn(s, __fsub_rn(t, b)), __fsub_rn(p, b)), __fmaf_rn(h, h, -p));
   s = t;
 }
 
@@ -139,13 +145,7 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
     }
     return v;
   };
-  float s = 0.0f, c = 0.0f;
-  auto square = [&](const float4 v) {
-    add_square(s, c, v.x);
-    add_square(s, c, v.y);
-    add_square(s, c, v.z);
-    add_square(s, c, v.w);
-  };
+  float s = 0.0f, c = 0.0f, s0 = 0.0f;
   if (QUADS) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
@@ -153,13 +153,31 @@ __global__ void __launch_bounds__(THREADS) norm_quant_kernel(const __grid_consta
       h[i] = value(j);
       if (kFewRows) w[kFewRows ? i : 0] = a.d_weight ? load4<FULL>(a.d_weight, j, a.n, vw) : one;
     }
+    // the sum starts at (no less than) its largest square, and gives it back
+    float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; i++) square(h[i]);
+    for (int i = 0; i < N; i++)
+      top = fmaxf(top, fmaxf(fmaxf(fabsf(h[i].x), fabsf(h[i].y)),
+                             fmaxf(fabsf(h[i].z), fabsf(h[i].w))));
+    s = s0 = __fmul_ru(top, top);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      add_square(s, c, h[i].x);
+      add_square(s, c, h[i].y);
+      add_square(s, c, h[i].z);
+      add_square(s, c, h[i].w);
+    }
   } else {
-    for (size_t j = 4 * (size_t)tid; j < a.n; j += 4 * THREADS) square(value(j));
+    for (size_t j = 4 * (size_t)tid; j < a.n; j += 4 * THREADS) {
+      const float4 v = value(j);
+      add_any_square(s, c, v.x);
+      add_any_square(s, c, v.y);
+      add_any_square(s, c, v.z);
+      add_any_square(s, c, v.w);
+    }
   }
   // squares near f32's ends (or a value that is not finite) leave no rest: the sum in f64
-  double sum = (double)s + (double)c;
+  double sum = ((double)s - (double)s0) + (double)c;
   if (!(s > 1e-25f && s < 3e38f)) {
     sum = 0.0;
     for (size_t j = 4 * (size_t)tid; j < a.n; j += 4 * THREADS) {
