@@ -176,3 +176,50 @@ def test_outputs_on_another_stream(ops, call):
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert torch.equal(g, w)
+
+
+@pytest.mark.parametrize("call", ["norm", "append", "attention", "prompt", "sample"])
+def test_captured_behind_a_copy(ops, call):
+    """A captured call behind a copy from the host reads what the copy brings, at every replay."""
+    import torch
+    from apeiron_b200.step import KV4Cache, SeqBatch
+
+    rng = np.random.default_rng(1)
+    t = 120
+    i32 = dict(dtype=torch.int32, device="cuda")
+    batch = SeqBatch(torch.tensor([0, t], **i32), torch.tensor([t], **i32),
+                     torch.arange(8, **i32)[None].contiguous(), t, t)
+    cache = KV4Cache.empty(8, 2, 64, 16)
+    table, u = ops.rope_table(t, 64), torch.rand(t, device="cuda")
+    kv = gpu(rng.standard_normal((t, 2, 64)).astype(np.float32))
+    ops.rope_kv4_append(None, kv, kv, table, cache, batch, rot_dim=64)
+    dt = torch.bfloat16 if call == "prompt" else torch.float32
+    x, y = (torch.zeros(t, 8, 64, dtype=dt, device="cuda") for _ in range(2))
+    token = torch.zeros(t, **i32)
+    fresh = torch.from_numpy(rng.standard_normal((6, t, 8, 64)).astype(np.float32)).to(dt)
+    host = torch.empty(t, 8, 64, dtype=dt).pin_memory()
+
+    def run():
+        if call == "norm":
+            ops.add_rms_norm_quant(x.flatten(1), None, 1e-6, y=y.view(t, 512))
+        elif call == "append":
+            ops.rope_kv4_append(x, kv, kv, table, cache, batch, rot_dim=64, q_out=y)
+        elif call == "sample":
+            ops.sample(x.flatten(1), u, token=token)
+        else:
+            ops.attn_kv4(x, cache, batch, 0.1, out=y)
+
+    run()
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        x.copy_(host, non_blocking=True)
+        run()
+    for v in fresh:
+        host.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = (y.clone(), token.clone())
+        x.copy_(v)
+        run()
+        assert torch.equal(got[0], y) and torch.equal(got[1], token)

@@ -42,3 +42,38 @@ def test_norm_with_dominant_channels(ops, n, k, large):
     assert np.all(np.abs(got - want) <= 2.0 ** -23 * np.abs(want))
     turned = (got != want.astype(np.float32)).sum()
     assert turned <= max(2, n * k * 2.0 ** -10)
+
+
+@pytest.mark.parametrize("n", [1, 33, 896, 1537, 4096, 20000])
+@pytest.mark.parametrize("k,extra", [(1, 0), (5, 0), (5, 3), (200, 4)])
+def test_norm_values_in_f32(ops, n, k, extra):
+    """The activation that the codes stand for, as f32: code * S to the bit, in rows apart."""
+    import torch
+
+    rng = np.random.default_rng(n + k)
+    x = (rng.standard_normal((k, n)) * np.exp(2 * rng.standard_normal((k, 1)))).astype(np.float32)
+    x[k // 2] = 0
+    deq = torch.full((k, n + extra), 7.0, device="cuda")
+    act = ops.add_rms_norm_quant(gpu(x), None, 1e-5)
+    assert ops.add_rms_norm_quant(gpu(x), None, 1e-5, deq=deq[:, :n]) is None
+    e = act.exps[:, : -(-n // 32)].cpu().numpy().astype(np.int64)
+    s = np.where(e == 0xFF, 0.0, np.ldexp(1.0, e - 32)).repeat(32, 1)[:, :n]
+    want = act.codes[:, :n].cpu().numpy() * s
+    assert np.array_equal(deq[:, :n].cpu().numpy().astype(np.float64), want)
+    assert (deq[:, n:] == 7.0).all()
+
+
+# ---- sampler --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,vocab", [(5, 40), (12, 5003), (12, 32003), (60, 33000), (9, 151936)])
+def test_sample_filters_of_each_row(ops, rows, vocab):
+    """A served batch: every row has filters and a temperature of its own, some none at all."""
+    from test_gpu_step import check_sample
+
+    rng = np.random.default_rng(rows + vocab)
+    logits = (rng.standard_normal((rows, vocab)) * 2).astype(np.float32)
+    logits[1::2, :: max(1, vocab // 60)] += 8
+    pick = lambda *v: rng.choice(v, rows)  # noqa: E731
+    check_sample(ops, logits, rng.random(rows), pad=3,
+                 temperature=pick(0.0, 0.3, 1.0, 1.0, 2.5), top_k=pick(0, 1, 40, 40, 1000, 3000),
+                 top_p=pick(1.0, 1.0, 0.1, 0.9, 0.97), min_p=pick(0.0, 0.0, 0.02, 0.3))
