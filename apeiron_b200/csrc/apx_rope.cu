@@ -71,7 +71,7 @@ struct RopeArgs {
   const int *cu, *kv_len, *table;
   uint8_t *pages;
   size_t n_pages, page_bytes;
-  int n_seqs, max_pages, kv_heads, dim, page_tokens;
+  int n_seqs, max_pages, kv_heads, dim, page_shift;
 };
 
 // Four dims of a head at x, turned.  i: the first dim, a multiple of 4 (rot is a multiple of 8).
@@ -128,9 +128,12 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
   pdl_launch_dependents();
   pdl_wait();
   const int seq = find_seq(r.cu, r.n_seqs, t);
-  const int pos = r.kv_len[seq] - r.cu[seq + 1] + t;
-  const int slot = pos / r.page_tokens;
-  bool ok = pos >= 0 && slot < r.max_pages && (a.rot_dim == 0 || (size_t)pos < a.n_pos);
+  const int begin = r.cu[seq], end = r.cu[seq + 1], kv = r.kv_len[seq];
+  const int pos = kv - (end - t);
+  const int slot = pos >> r.page_shift;
+  // a token that the lengths leave to no request has no position
+  bool ok = begin <= t && t < end && kv >= end - t && slot < r.max_pages &&
+            (a.rot_dim == 0 || (size_t)pos < a.n_pos);
   int page = -1;
   if (ok) {
     page = r.table[(size_t)seq * r.max_pages + slot];
@@ -143,7 +146,7 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
     return;
   }
   const float2 *cs = reinterpret_cast<const float2 *>(a.d_table) + (size_t)pos * (a.rot_dim / 2);
-  const int row = pos % kKvTile, tile = pos % r.page_tokens / kKvTile;
+  const int row = pos % kKvTile, tile = (pos & ((1 << r.page_shift) - 1)) / kKvTile;
   const int nq = a.d_q ? a.n_heads : 0, heads = nq + 2 * r.kv_heads;
   for (int w = blockIdx.y * blockDim.x + threadIdx.x; w < heads * per;
        w += gridDim.y * blockDim.x) {  // whole groups of 8 lanes
@@ -232,7 +235,8 @@ cudaError_t launch_rope_kv4_append(const apx_rope_args &a, const apx_kv4_cache &
   r.max_pages = b.max_pages;
   r.kv_heads = c.n_kv_heads;
   r.dim = c.head_dim;
-  r.page_tokens = c.page_tokens;
+  r.page_shift = 0;
+  while (1 << r.page_shift < c.page_tokens) r.page_shift++;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -592,8 +592,8 @@ APX_API int apx_rope_table_async(apx_ctx *ctx, const apx_rope_freqs *freqs, size
  * when d = 0.  Token t's head h starts at d_q[t * ldq + h * head_dim].  Optional: d_q (with
  * d_q_out), and d_k_deq / d_v_deq = the values the cache now holds, f16
  * [n_tokens][n_kv_heads][head_dim].  d_status (optional, all ones on entry): the first token
- * refused, in row order, with APX_ERR_INVALID_ARGUMENT (its position outside the table or the
- * cache, its page not one of n_pages) or APX_ERR_QUANT_REFUSED (a k or v value that is not
+ * refused, in row order, with APX_ERR_INVALID_ARGUMENT (not a token of any sequence, its position
+ * outside the table or the cache, its page not one of n_pages) or APX_ERR_QUANT_REFUSED (a k or v value that is not
  * finite or past 65280 in magnitude: its group is stored as zeros). */
 #define APX_ROPE_HALF 0
 #define APX_ROPE_INTERLEAVED 1

@@ -151,3 +151,40 @@ def test_attention_without_the_pages_behind_the_window(ops, kind, dim, page, win
         tol = tol + 2.0 ** -11 * reach + 2.0 ** -25 * max(kv_lens) * most
         tol = tol + 2.0 ** -11 * np.abs(want) + 2.0 ** -24
     assert np.isfinite(got).all() and (np.abs(got - want) <= tol).all()
+
+
+# ---- the append's lengths -------------------------------------------------------------------
+
+@pytest.mark.parametrize("cu,kv_len,first", [
+    ([0, 2, 4], [10, 20], 4),                     # two tokens behind the last request
+    ([0, 0, 0], [10, 20], 0),                     # none of them in a request
+    ([3, 4, 6], [10, 20], 0),                     # three before the first
+    ([0, 2, 6], [10, -2 ** 31], 2), ([0, 2, 6], [-1, 20], 0), ([0, 2, 6], [10, 3], 2)])
+def test_append_tokens_of_no_request(ops, cu, kv_len, first):
+    """Tokens that the lengths leave to no request, or to a place before its first, are refused;
+    those beside them are appended, and nothing else is written."""
+    import torch
+    from apeiron_b200.step import KV4Cache, SeqBatch
+
+    rng = np.random.default_rng(5)
+    k = gpu(rng.standard_normal((6, 1, 64)).astype(np.float32))
+    cache = KV4Cache.empty(8, 1, 64, 16)
+    cache.pages.fill_(0x11)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = np.arange(8, dtype=np.int32).reshape(2, 4)
+    batch = SeqBatch(torch.tensor(cu, **i32), torch.tensor(kv_len, **i32), gpu(table), 6, 6)
+    status = ops.new_status()
+    ops.rope_kv4_append(None, k, k, ops.rope_table(64, 64), cache, batch, rot_dim=64, status=status)
+    assert ops.check_status(status) == (first, 20)
+    pages = cache.pages.cpu().numpy()
+    right = KV4Cache.empty(8, 1, 64, 16)
+    right.pages.fill_(0x11)
+    for s in range(2):
+        for t in range(cu[s], cu[s + 1]):
+            pos = kv_len[s] - cu[s + 1] + t
+            if pos >= 0:
+                one = SeqBatch(torch.tensor([0, 1], **i32), torch.tensor([pos + 1], **i32),
+                               gpu(table[s: s + 1]), 1, 1)
+                ops.rope_kv4_append(None, k[t: t + 1], k[t: t + 1], ops.rope_table(64, 64), right,
+                                    one, rot_dim=64)
+    assert np.array_equal(pages, right.pages.cpu().numpy())
