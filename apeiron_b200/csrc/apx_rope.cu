@@ -155,6 +155,8 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
       const float4 v = turn4(a.d_q + (size_t)t * a.ldq + (size_t)head * r.dim, i, a.rot_dim,
                              a.layout, cs);
       const size_t at = (size_t)t * a.ldq_out + (size_t)head * r.dim + i;
+      // the head's lanes, all of one warp, have read it before one writes where it stands
+      if (a.d_q_out == a.d_q) __syncwarp(per == 32 ? 0xFFFFFFFFu : 0xFFFFu << (threadIdx.x & 16));
       if (a.q_type == APX_DTYPE_F32)
         *reinterpret_cast<float4 *>(static_cast<float *>(a.d_q_out) + at) = v;
       else

@@ -105,6 +105,9 @@ int apx_rope_kv4_append_async(apx_ctx *ctx, const apx_rope_args *a, const apx_kv
        !aligned(a->d_q, 16) || !aligned(a->d_q_out, 16) || a->q_type < APX_DTYPE_F32 ||
        a->q_type > APX_DTYPE_BF16))
     return APX_ERR_INVALID_ARGUMENT;
+  if (a->d_q && a->d_q_out == a->d_q &&
+      (a->q_type != APX_DTYPE_F32 || (a->ldq_out != a->ldq && b->n_tokens > 1)))
+    return APX_ERR_INVALID_ARGUMENT;  // another token's values would be written over
   return on_device(
       ctx, [&] { return apx::launch_rope_kv4_append(*a, *c, *b, (cudaStream_t)stream); });
 }

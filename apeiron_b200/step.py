@@ -250,7 +250,7 @@ class StepOps:
     def rope_kv4_append(self, q, k, v, table, cache: KV4Cache, batch: SeqBatch, *, rot_dim,
                         layout="half", q_out=None, q_type=_F32, k_deq=None, v_deq=None,
                         status=None, stream=None):
-        """q (tokens, heads, dim; None to leave out) turned into ``q_out``; k turned and v
+        """q (tokens, heads, dim; None to leave out) turned into ``q_out`` (may be q); k turned and v
         (tokens, kv heads, dim) appended to the cache in 4 bits.  ``k_deq`` / ``v_deq`` (f16):
         the values the cache now holds.  Returns q_out."""
         self._here(cache, batch)

@@ -590,7 +590,7 @@ APX_API int apx_rope_table_async(apx_ctx *ctx, const apx_rope_freqs *freqs, size
  * each operation rounded once.  Per 32 dims of k and v: m the value of largest magnitude (the
  * positive one of two), d = f16(bf16(-m / 8)), c = clamp(rint(x * (1 / d)) + 8, 0, 15), c = 8
  * when d = 0.  Token t's head h starts at d_q[t * ldq + h * head_dim].  Optional: d_q (with
- * d_q_out), and d_k_deq / d_v_deq = the values the cache now holds, f16
+ * d_q_out, which may be d_q itself where it is f32 of the same ldq), and d_k_deq / d_v_deq = the values the cache now holds, f16
  * [n_tokens][n_kv_heads][head_dim].  d_status (optional, all ones on entry): the first token
  * refused, in row order, with APX_ERR_INVALID_ARGUMENT (not a token of any sequence, its position
  * outside the table or the cache, its page not one of n_pages) or APX_ERR_QUANT_REFUSED (a k or v value that is not

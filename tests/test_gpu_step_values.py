@@ -77,3 +77,41 @@ def test_sample_filters_of_each_row(ops, rows, vocab):
     check_sample(ops, logits, rng.random(rows), pad=3,
                  temperature=pick(0.0, 0.3, 1.0, 1.0, 2.5), top_k=pick(0, 1, 40, 40, 1000, 3000),
                  top_p=pick(1.0, 1.0, 0.1, 0.9, 0.97), min_p=pick(0.0, 0.0, 0.02, 0.3))
+
+
+# ---- positions ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(5, 1, 64), (64, 8, 128), (12, 2, 128), (14, 2, 64)])
+@pytest.mark.parametrize("rot,layout", [(64, "half"), (64, "interleaved"), (24, "half"), (8, "half")])
+def test_append_turns_q_in_place(ops, heads, kv_heads, dim, rot, layout):
+    """q_out = q, in the fused rows of a projection: the bits of an output of its own."""
+    import torch
+    from apeiron_b200.step import KV4Cache, SeqBatch
+
+    t = 200
+    i32 = dict(dtype=torch.int32, device="cuda")
+    rows = torch.randn(t, (heads + 2 * kv_heads) * dim, device="cuda")
+    batch = SeqBatch(torch.tensor([0, t], **i32), torch.tensor([t], **i32),
+                     torch.arange(13, **i32)[None].contiguous(), t, t)
+    cache = KV4Cache.empty(13, kv_heads, dim, 16)
+    table = ops.rope_table(t, rot)
+
+    def run(rows, q_out):
+        q, k, v = (p.unflatten(1, (-1, dim)) for p in
+                   rows.split([heads * dim, kv_heads * dim, kv_heads * dim], 1))
+        return ops.rope_kv4_append(q, k, v, table, cache, batch, rot_dim=rot, layout=layout,
+                                   q_out=q if q_out else None)
+
+    want = run(rows, False)
+    for _ in range(5):
+        copy = rows.clone()
+        run(copy, True)
+        assert torch.equal(copy[:, : heads * dim], want.flatten(1))
+        assert torch.equal(copy[:, heads * dim:], rows[:, heads * dim:])
+    q = rows[:, : heads * dim].unflatten(1, (heads, dim))
+    k = torch.randn(t, kv_heads, dim, device="cuda")
+    for other in (rows.view(torch.bfloat16)[:, : heads * dim],  # the same place, another type
+                  rows.view(-1)[: t * heads * dim].view(t, -1)):  # or other rows
+        with pytest.raises(ValueError):
+            ops.rope_kv4_append(q, k, k, table, cache, batch, rot_dim=rot, layout=layout,
+                                q_out=other.unflatten(1, (heads, dim)))
