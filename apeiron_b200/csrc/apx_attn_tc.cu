@@ -366,12 +366,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (issues) {
         outputs(j);
         if (j + 1 < steps) scores(j + 1);
-        else if (leader && ok) mma_commit(o_full + tile);
+        else if (leader) mma_commit(o_full + tile);
       }
       __syncwarp();
     }
     // ---- the output rows ----
-    if (steps > 0) ok = ok && mbar_wait(o_full + tile, 0);
+    // (after a wait that gave up, too: tensor memory is given back once its products are done)
+    if (steps > 0) ok = mbar_wait(o_full + tile, 0) && ok;
     __syncwarp();
     tc_fence_after();
     const float2 la = unpack2(l2[0]), lb = unpack2(l2[1]);
