@@ -330,7 +330,7 @@ cudaError_t launch(const apx_norm_args &a, size_t padded, int vec, cudaStream_t 
 
 }  // namespace
 
-cudaError_t launch_add_rms_norm_quant(const apx_norm_args &a, cudaStream_t stream) {
+cudaError_t launch_add_rms_norm_quant(const apx_norm_args &a, int sms, cudaStream_t stream) {
   const size_t padded = apx_act_padded_len(a.n);
   // which arrays have 16-byte (the 16-bit values: 8-byte) aligned rows
   auto whole = [](const void *p, size_t ld, size_t bytes) {
@@ -348,8 +348,9 @@ cudaError_t launch_add_rms_norm_quant(const apx_norm_args &a, cudaStream_t strea
   // fill the GPU with smaller CTAs of more quads a thread (512 rows of 8192: 4 quads of 512 threads
   // 20.0 us, 8 of 256 19.5).
   if (quads <= 256) return launch<1, 256>(a, padded, vec, stream);
-  if (a.k <= 148 && quads <= 1024) return launch<1, 1024>(a, padded, vec, stream);
-  if (a.k <= 148 && quads <= 2048) return launch<2, 1024>(a, padded, vec, stream);
+  const bool few = a.k <= (size_t)sms;
+  if (few && quads <= 1024) return launch<1, 1024>(a, padded, vec, stream);
+  if (few && quads <= 2048) return launch<2, 1024>(a, padded, vec, stream);
   if (quads <= 512) return launch<2, 256>(a, padded, vec, stream);
   if (quads <= 1024) return launch<4, 256>(a, padded, vec, stream);
   if (quads <= 2048) return launch<8, 256>(a, padded, vec, stream);

@@ -528,10 +528,9 @@ bool tensor_launch_info(apx_ctx *ctx, uint64_t handle, uint32_t *type, const uin
 
 int context_device(const apx_ctx *ctx) { return ctx->device; }
 
-void *context_attn_work(apx_ctx *ctx, int *sms) {
-  *sms = ctx->sm_count;
-  return ctx->attn_work.p;
-}
+int context_sms(const apx_ctx *ctx) { return ctx->sm_count; }
+
+void *context_attn_work(apx_ctx *ctx) { return ctx->attn_work.p; }
 }  // namespace apx
 
 extern "C" {

@@ -702,7 +702,7 @@ cudaError_t launch(const apx_sample_args &a, int ctas, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t launch_sample(const apx_sample_args &a, cudaStream_t stream) {
+cudaError_t launch_sample(const apx_sample_args &a, int sms, cudaStream_t stream) {
   // the fewest CTAs that hold the row in 20 tokens a thread, in 32 past 16 x 20; twice
   // as many while all rows still run at once (one row of 151936: 8 CTAs 15.5 us, 16 CTAs 13.6)
   int ctas = 1;
@@ -712,7 +712,7 @@ cudaError_t launch_sample(const apx_sample_args &a, cudaStream_t stream) {
   if (per <= 4) return launch<4, false, 1>(a, ctas, stream);
   // more CTAs than SMs: two an SM, one's barriers behind the other's work (a nucleus, min-p: 64
   // rows of 151936 71.5 us with one an SM, 61.0 with two; 512 rows of 32003 125 and 97)
-  if (a.rows * ctas > 148 && per <= 20)
+  if (a.rows * ctas > (size_t)sms && per <= 20)
     return per <= 12 ? launch<12, true, 2>(a, ctas, stream) : launch<20, true, 2>(a, ctas, stream);
   // more than 12 tokens a thread leave the levels too few registers (16 rows of 151936, a nucleus of
   // thousands: 60 us in registers, 54 in shared memory; one row of 524288, top-k 50: 20.0 and 21.0)

@@ -64,7 +64,9 @@ int apx_add_rms_norm_quant_async(apx_ctx *ctx, const apx_norm_args *a, void *str
       (any && !(a->d_codes && a->d_exps && a->d_descs)) || !aligned(a->d_codes, 4) ||
       !aligned(a->d_descs, 16) || !(a->eps >= 0.0f))
     return APX_ERR_INVALID_ARGUMENT;
-  return on_device(ctx, [&] { return apx::launch_add_rms_norm_quant(*a, (cudaStream_t)stream); });
+  const int sms = apx::context_sms(ctx);
+  return on_device(
+      ctx, [&] { return apx::launch_add_rms_norm_quant(*a, sms, (cudaStream_t)stream); });
 }
 
 int apx_rope_table_async(apx_ctx *ctx, const apx_rope_freqs *f, size_t n_pos, float *d_table,
@@ -128,8 +130,8 @@ int apx_attn_kv4_async(apx_ctx *ctx, const apx_attn_args *a, const apx_kv4_cache
   if (!a->d_q || !a->d_out || a->ldq < nq || a->ldo < nq || a->ldq * el % 16 ||
       a->ldo * el % 16 || !aligned(a->d_q, 16) || !aligned(a->d_out, 16))
     return APX_ERR_INVALID_ARGUMENT;
-  int sms;
-  void *work = apx::context_attn_work(ctx, &sms);
+  void *work = apx::context_attn_work(ctx);
+  const int sms = apx::context_sms(ctx);
   return on_device(
       ctx, [&] { return apx::launch_attn_kv4(*a, *c, *b, work, sms, (cudaStream_t)stream); });
 }
@@ -140,7 +142,8 @@ int apx_sample_async(apx_ctx *ctx, const apx_sample_args *a, void *stream) {
   if (a->rows == 0) return APX_OK;
   if (!a->d_logits || !a->d_u || !a->d_token || a->vocab == 0 || a->ld < a->vocab)
     return APX_ERR_INVALID_ARGUMENT;
-  return on_device(ctx, [&] { return apx::launch_sample(*a, (cudaStream_t)stream); });
+  const int sms = apx::context_sms(ctx);
+  return on_device(ctx, [&] { return apx::launch_sample(*a, sms, (cudaStream_t)stream); });
 }
 
 }  // extern "C"
