@@ -12,7 +12,9 @@ namespace apx {
 constexpr int kStepKeys = 32;
 // What a warp loses at an item's end (its rows to keep or write, the next one's to read), in steps:
 // items of single tokens carry as many steps without keys, so that warps with a boundary get fewer
-// keys (64 ragged requests: 53.2 us without, 51.4 at 2, 48.7 at 5; prompts lose by it).
+// keys (without, at 2, 5 and 8: 64 requests of 100-4096 keys, 64 / 8 heads of 128 53.6 51.1 48.0 49.9
+// us; 32 of up to 8000, 12 / 2 of 128 23.4 22.8 21.6 21.2; 48 of 1000, 32 / 4 of 128 20.3 19.6 19.3
+// 19.6; 64 of 200-600, 16 / 16 of 64 24.4 25.1 23.7 25.2; prompts lose by it).
 constexpr int kItemCost = 5;
 
 // A sequence's steps.  Its blocks of rows pair first with last: a pair has `pair` steps, the

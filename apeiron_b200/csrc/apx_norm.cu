@@ -11,7 +11,7 @@
 //
 // What bounds it: for many rows the bytes, 4 n read (8 n and 4 n written with a residual) and
 // 1 + 1/32 n written, and some 65 instructions an element beside them: 512 rows of 8192 with
-// residual and 16-bit values move 63 MB in 19.5 us, 3.2 TB/s, half of what a large copy reaches,
+// residual and 16-bit values move 63 MB in 19.7 us, 3.2 TB/s, half of what a large copy reaches,
 // with half of the issue slots used.  One row: the chain load, sum over the CTA, root, quantize,
 // store (896 wide: 2.4 us).
 #include <cuda_bf16.h>
@@ -346,7 +346,7 @@ cudaError_t launch_add_rms_norm_quant(const apx_norm_args &a, int sms, cudaStrea
   const size_t quads = padded / 4;  // padded is what has to be written
   // Few rows: as many threads as the row has quads, the loads of a row one round trip.  Many rows
   // fill the GPU with smaller CTAs of more quads a thread (512 rows of 8192: 4 quads of 512 threads
-  // 20.0 us, 8 of 256 19.5).
+  // 20.0 us, 8 of 256 19.7).
   if (quads <= 256) return launch<1, 256>(a, padded, vec, stream);
   const bool few = a.k <= (size_t)sms;
   if (few && quads <= 1024) return launch<1, 1024>(a, padded, vec, stream);

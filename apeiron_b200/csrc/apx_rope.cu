@@ -6,11 +6,11 @@
 // attention's operand conversion loses nothing), c = clamp(rint(x (1 / d)) + 8, 0, 15).
 //
 // What bounds it: 4 bytes read a value and 2 or 4 (q) or 9/16 (K, V) written; 512 tokens of 64 + 2 x
-// 8 heads of 128 move 41 MB in 12.3 us, 3.3 TB/s, with three quarters of the issue slots used.  A
+// 8 heads of 128 move 41 MB in 12.8 us, 3.2 TB/s, with three quarters of the issue slots used.  A
 // thread takes four dims, the eight lanes of a scale's group reduce by shuffles; it has two heads
 // at most to go round, so that eight CTAs an SM (32 registers) hide the chain position, page,
 // values (the coefficients kept over more heads, the next head's values loaded ahead: 48 to 62
-// registers, 12.6 to 14 us).  32 decoded tokens: 3.5 us, all of it that chain.
+// registers, 12.6 to 14 us).  32 decoded tokens: 3.7 us, all of it that chain.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -17,11 +17,11 @@
 // decide every filter at once, and a second sort, by index, the token.  It takes two cluster
 // barriers instead of two for each of up to five more levels.
 //
-// What bounds it: 4 bytes a logit is the floor (64 rows of 151936: 5.9 us); measured 61 to 75 us by
-// the logits, with half of the issue slots of the SMs that hold a CTA in use (some 90 instructions
+// What bounds it: 4 bytes a logit is the floor (64 rows of 151936: 5.9 us); measured 54 us (top-k) to
+// 71 us (a nucleus with min-p), with half of the issue slots of the SMs that hold a CTA in use (some 90 instructions
 // a token: e in separately rounded steps, three shared-memory additions, the comparisons) and
 // barriers the first reason to wait.  One row: the chain of barriers, scans and the list's sorts,
-// 13.6 us.
+// 13.8 us.
 #include <algorithm>
 #include <climits>
 
@@ -703,15 +703,17 @@ cudaError_t launch(const apx_sample_args &a, int ctas, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_sample(const apx_sample_args &a, int sms, cudaStream_t stream) {
-  // the fewest CTAs that hold the row in 20 tokens a thread, in 32 past 16 x 20; twice
-  // as many while all rows still run at once (one row of 151936: 8 CTAs 15.5 us, 16 CTAs 13.6)
+  // the fewest CTAs that hold the row in 20 tokens a thread, in 32 past 16 x 20; twice as many while
+  // that makes 64 CTAs at most (four rows of 151936: 8 CTAs a row 16.2 us, 16 CTAs 13.9; eight rows,
+  // whose clusters of 16 no longer all run at once: 16.3 and 23.2; five to seven would gain still)
   int ctas = 1;
   while (ctas < kMaxCluster && (size_t)ctas * kThreads * 20 < a.vocab) ctas *= 2;
   if (ctas < kMaxCluster && a.rows * ctas * 2 <= 64 && a.vocab > 8192 * (size_t)ctas) ctas *= 2;
   const size_t per = ((a.vocab + 4 * ctas - 1) / (4 * ctas) * 4 + kThreads - 1) / kThreads;
   if (per <= 4) return launch<4, false, 1>(a, ctas, stream);
-  // more CTAs than SMs: two an SM, one's barriers behind the other's work (a nucleus, min-p: 64
-  // rows of 151936 71.5 us with one an SM, 61.0 with two; 512 rows of 32003 125 and 97)
+  // more CTAs than SMs: two an SM, one's barriers behind the other's work (a nucleus with min-p: 64
+  // rows of 151936 81.5 us with one an SM, 68.2 with two; 512 rows of 32003 135 and 102, with top-k
+  // 119 and 88; 24 rows of 151936 43.7 and 42.4)
   if (a.rows * ctas > (size_t)sms && per <= 20)
     return per <= 12 ? launch<12, true, 2>(a, ctas, stream) : launch<20, true, 2>(a, ctas, stream);
   // more than 12 tokens a thread leave the levels too few registers (16 rows of 151936, a nucleus of

@@ -501,7 +501,9 @@ APX_API int apx_gather_publish_async(apx_ctx *ctx, const apx_gather_desc *gd, vo
  * stream, for an engine that keeps the whole step on the GPU (the reference runs them on the
  * CPU around its projections: src/engine/step.rs, src/engine/attn.rs, src/engine/ops/).  They
  * take the projections' f32 outputs and write the activations the projections read.  All sums
- * and softmax statistics are held in 32 bits or more.  A call over no rows does nothing. */
+ * and softmax statistics are held in 32 bits or more.  A call over no rows does nothing.  A call
+ * goes to the context's device, whichever is current, and any of its inputs may be what work queued
+ * before it on the stream writes. */
 
 #define APX_DTYPE_F32 0
 #define APX_DTYPE_F16 1
@@ -539,7 +541,7 @@ APX_API int apx_add_rms_norm_quant_async(apx_ctx *ctx, const apx_norm_args *args
  *     g < 8, and t < 4, word ((m / 4) * 32 + g * 4 + t) * 4 + m % 4 holds tokens
  *     2t, 2t + 8, 2t + 1, 2t + 9 in its bytes 0..3 (the operand order of the matrix unit);
  *   K scales, then V scales: f16 [D / 32][16 tokens] each.
- * page_tokens: 16, 32, 64 or 128.  head_dim: 64 or 128.  Sequence s's token j lives in page
+ * page_tokens: 16, 32, 64 or 128.  head_dim: 64 or 128.  65535 heads at most.  Sequence s's token j lives in page
  * d_table[s * max_pages + j / page_tokens], at j % page_tokens. */
 typedef struct apx_kv4_cache {
   void *d_pages; /* 16-byte aligned */
@@ -553,7 +555,7 @@ APX_API size_t apx_kv4_page_bytes(int head_dim, int page_tokens);
  * call's n_tokens rows (d_cu[0] = 0, ascending, d_cu[n_seqs] = n_tokens) and d_kv_len[s] cached
  * tokens (2^31 - 512 at most), the query tokens being the last of them: query i stands at position
  * d_kv_len[s] - (d_cu[s + 1] - d_cu[s]) + i.  max_q bounds a sequence's query tokens: attention
- * refuses a sequence with more. */
+ * refuses a sequence with more.  65535 sequences at most. */
 typedef struct apx_seq_batch {
   const int32_t *d_cu;     /* n_seqs + 1 */
   const int32_t *d_kv_len; /* n_seqs */
@@ -647,11 +649,11 @@ APX_API int apx_attn_kv4_async(apx_ctx *ctx, const apx_attn_args *args,
  *              the weights of all (in f64; the first always stays);
  *   min_p > 0: of those, a token stays when w_i >= min_p * 2^31 (in f64).
  * token = the first index, in vocabulary order, at which the running sum of the weights that
- * stay passes floor(u * W), W their sum; prob = w / W; kept = the tokens that stay with w > 0.
- * T <= 0 takes the largest logit (lowest index).  NaN logits count as -inf, -inf as excluded;
+ * stay passes floor(u * W) (in f64), W their sum; prob = w / W; kept = the tokens that stay with
+ * w > 0.  T <= 0 takes the largest logit (lowest index).  NaN logits count as -inf, -inf as excluded;
  * where +inf occurs, only +inf tokens have weight.  A row with nothing left gives token -1,
  * prob 0, kept 0.  Absent (NULL) parameter arrays: T = 1, no filter.  d_prob, d_kept: optional.
- * vocab <= APX_SAMPLE_MAX_VOCAB. */
+ * vocab <= APX_SAMPLE_MAX_VOCAB, 65535 rows at most. */
 #define APX_SAMPLE_MAX_VOCAB 524288u
 typedef struct apx_sample_args {
   const float *d_logits, *d_u;
