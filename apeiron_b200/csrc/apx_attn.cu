@@ -15,10 +15,10 @@
 //
 // Numbers.  d (c - 8) is exact in f16 (the append's d has 8 significant bits).  A query row is
 // scaled by a power of two to the top of f16's range and, for f32, split in two halves of 11 bits
-// each; so are the probabilities, taken at 2^13 e^(s - m): 22 bits down to 2^-38 of the largest.  With
-// 16-bit q the probabilities go to the product in one half of 11 bits (their sum keeps f32): below
-// what the output's rounding costs, and half of the products (against 64 bits, relative: bf16 1.7e-3
-// as the plain form in f32, f16 2.1e-4 against the plain form's 2.0e-4).
+// each; so are the probabilities, taken at 2^13 e^(s - m): 22 bits down to 2^-38 of the largest.
+// With 16-bit q the probabilities go to the product in one half of 11 bits (their sum keeps f32):
+// below what the output's rounding costs, and half of the products (against 64 bits, relative:
+// bf16 1.7e-3 as the plain form in f32, f16 2.1e-4 against the plain form's 2.0e-4).
 // The unit's f32 accumulation is cut into short chains joined by f32 additions.
 //
 // Split.  Work is counted in steps of 32 keys of one item (sequence, KV head, block of query

@@ -6,9 +6,10 @@
 // into probabilities in place (f16), O += P V with P read from TMEM.  A tile's first softmax warp
 // issues its products.  The tiles' softmaxes take turns: while one is in its softmax the other's
 // products run (left to themselves they fall into step and both wait for their products: two
-// prompts of up to 2048 66 us against 60.5 with turns; now 59, 585 TFLOP/s of what they see).  Both read the same
-// keys and values, which eight warps unpack from the cache's pages to f16 operands in shared memory
-// (exact: d (c - 8) fits f16), two buffers each, registers holding the bytes in flight.
+// prompts of up to 2048 66 us against 60.5 with turns; now 59, 585 TFLOP/s of what they see).
+// Both read the same keys and values, which eight warps unpack from the cache's pages to f16
+// operands in shared memory (exact: d (c - 8) fits f16), two buffers each, registers holding the
+// bytes in flight.
 //
 // What bounds it, per 128 x 128 step of a tile at D = 128: the products 1024 cycles, the
 // exponentials 1024 (16 a cycle), shared memory 1024 (S reads both operands, P V one, the unpacked
@@ -22,8 +23,8 @@
 // The running maximum is a stale one: O (in TMEM) and the row sum turn only when a row's maximum
 // has grown by more than 2^8 since the last turn; probabilities are held at 2^6 e^(s - m), at most
 // 2^14, and rounded to f16's 11 bits for the product with V (their sum is not): below what the
-// output's rounding costs.  A row of q is scaled by a power of two to the top of f16's range: bf16 and
-// f16 both fit.
+// output's rounding costs.  A row of q is scaled by a power of two to the top of f16's range: bf16
+// and f16 both fit.
 //
 // K's dims are stored in the order the unpacking yields them (0 4 1 5 2 6 3 7 of every eight), Q's
 // the same.
@@ -680,11 +681,12 @@ cudaError_t launch(const AttnArgs &p, int max_q, cudaStream_t stream) {
 
 }  // namespace
 
-// Prompts in 16-bit numbers, from three quarters of a tile's rows on: a tile costs the same however
-// many of its rows are there.  One request over 30000 keys, 8 KV heads of 128: 87 us here for any of
-// 64 to 128 rows, apx_attn.cu's kernel 60 for 64, 77 for 80 and 96, 98 for 112 and 128; 32 requests
-// over 100 to 4000: 155 to 159, and 139 for 64, 203 for 96, 262 for 128.  Where one request has two KV
-// heads of 64 the other kernel stays ahead for longer (96 rows over 30000 keys: 62 and 28).
+// Prompts in 16-bit numbers, from three quarters of a tile's rows on: a tile costs the same
+// however many of its rows are there.  One request over 30000 keys, 8 KV heads of 128: 87 us here
+// for any of 64 to 128 rows, apx_attn.cu's kernel 60 for 64, 77 for 80 and 96, 98 for 112 and 128;
+// 32 requests over 100 to 4000: 155 to 159, and 139 for 64, 203 for 96, 262 for 128.  Where one
+// request has two KV heads of 64 the other kernel stays ahead for longer (96 rows over 30000 keys:
+// 62 and 28).
 bool attn_tc_serves(const AttnArgs &p, int dim, int max_q) {
   const long long rows = (long long)max_q * p.group;
   return p.type != APX_DTYPE_F32 && rows >= 96 && rows <= 65535ll * kRows &&

@@ -17,11 +17,11 @@
 // decide every filter at once, and a second sort, by index, the token.  It takes two cluster
 // barriers instead of two for each of up to five more levels.
 //
-// What bounds it: 4 bytes a logit is the floor (64 rows of 151936: 5.9 us); measured 54 us (top-k) to
-// 71 us (a nucleus with min-p), with half of the issue slots of the SMs that hold a CTA in use (some 90 instructions
-// a token: e in separately rounded steps, three shared-memory additions, the comparisons) and
-// barriers the first reason to wait.  One row: the chain of barriers, scans and the list's sorts,
-// 13.8 us.
+// What bounds it: 4 bytes a logit is the floor (64 rows of 151936: 5.9 us); measured 54 us (top-k)
+// to 71 us (a nucleus with min-p), with half of the issue slots of the SMs that hold a CTA in use
+// (some 90 instructions a token: e in separately rounded steps, three shared-memory additions, the
+// comparisons) and barriers the first reason to wait.  One row: the chain of barriers, scans and
+// the list's sorts, 13.8 us.
 #include <algorithm>
 #include <climits>
 

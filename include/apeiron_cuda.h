@@ -541,8 +541,8 @@ APX_API int apx_add_rms_norm_quant_async(apx_ctx *ctx, const apx_norm_args *args
  *     g < 8, and t < 4, word ((m / 4) * 32 + g * 4 + t) * 4 + m % 4 holds tokens
  *     2t, 2t + 8, 2t + 1, 2t + 9 in its bytes 0..3 (the operand order of the matrix unit);
  *   K scales, then V scales: f16 [D / 32][16 tokens] each.
- * page_tokens: 16, 32, 64 or 128.  head_dim: 64 or 128.  65535 heads at most.  Sequence s's token j lives in page
- * d_table[s * max_pages + j / page_tokens], at j % page_tokens. */
+ * page_tokens: 16, 32, 64 or 128.  head_dim: 64 or 128.  65535 heads at most.  Sequence s's token
+ * j lives in page d_table[s * max_pages + j / page_tokens], at j % page_tokens. */
 typedef struct apx_kv4_cache {
   void *d_pages; /* 16-byte aligned */
   size_t n_pages;
@@ -592,11 +592,12 @@ APX_API int apx_rope_table_async(apx_ctx *ctx, const apx_rope_freqs *freqs, size
  * each operation rounded once.  Per 32 dims of k and v: m the value of largest magnitude (the
  * positive one of two), d = f16(bf16(-m / 8)), c = clamp(rint(x * (1 / d)) + 8, 0, 15), c = 8
  * when d = 0.  Token t's head h starts at d_q[t * ldq + h * head_dim].  Optional: d_q (with
- * d_q_out, which may be d_q itself where it is f32 of the same ldq), and d_k_deq / d_v_deq = the values the cache now holds, f16
- * [n_tokens][n_kv_heads][head_dim].  d_status (optional, all ones on entry): the first token
- * refused, in row order, with APX_ERR_INVALID_ARGUMENT (not a token of any sequence, its position
- * outside the table or the cache, its page not one of n_pages) or APX_ERR_QUANT_REFUSED (a k or v value that is not
- * finite or past 65280 in magnitude: its group is stored as zeros). */
+ * d_q_out, which may be d_q itself where it is f32 of the same ldq), and d_k_deq / d_v_deq = the
+ * values the cache now holds, f16 [n_tokens][n_kv_heads][head_dim].  d_status (optional, all ones
+ * on entry): the first token refused, in row order, with APX_ERR_INVALID_ARGUMENT (not a token of
+ * any sequence, its position outside the table or the cache, its page not one of n_pages) or
+ * APX_ERR_QUANT_REFUSED (a k or v value that is not finite or past 65280 in magnitude: its group
+ * is stored as zeros). */
 #define APX_ROPE_HALF 0
 #define APX_ROPE_INTERLEAVED 1
 typedef struct apx_rope_args {
@@ -617,12 +618,13 @@ APX_API int apx_rope_kv4_append_async(apx_ctx *ctx, const apx_rope_args *args,
 /* Attention of the batch's query tokens over the cache: out = softmax(scale * q k^T) v per query
  * head (n_heads a multiple of n_kv_heads; query head h reads KV head h / (n_heads /
  * n_kv_heads)).  The query at position p sees key j <= p when window is 0 or j > p - window or
- * j < sinks.  A query that sees no key gets zeros.  Keys past d_kv_len, and those behind the windows
- * of all queries of their sequence, never take part, whatever the pages hold there; a page of such
- * keys alone may be gone, its number in the table anything.  q and out share one type.  For APX_DTYPE_F32 the products carry 22 bits
- * of q and of the probabilities (one below 2^-38 of its row's largest counts as zero), the sums
- * f32; for the 16-bit types the probabilities are rounded to 11 bits before the product with v.
- * Uses a context workspace: calls on one context must not overlap in time.
+ * j < sinks.  A query that sees no key gets zeros.  Keys past d_kv_len, and those behind the
+ * windows of all queries of their sequence, never take part, whatever the pages hold there; a
+ * page of such keys alone may be gone, its number in the table anything.  q and out share one
+ * type.  For APX_DTYPE_F32 the products carry 22 bits of q and of the probabilities (one below
+ * 2^-38 of its row's largest counts as zero), the sums f32; for the 16-bit types the
+ * probabilities are rounded to 11 bits before the product with v. Uses a context workspace: calls
+ * on one context must not overlap in time.
  * d_status (optional, all ones on entry): APX_ERR_INVALID_ARGUMENT with the first sequence whose
  * lengths or page numbers lie outside the batch or the cache (its rows are then undefined), or
  * APX_ERR_DEVICE_TIMEOUT. */
