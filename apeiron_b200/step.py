@@ -159,12 +159,17 @@ class StepOps:
     must not overlap in time."""
 
     def __init__(self, backend: Backend):
-        self.backend, self.lib, self.ctx = backend, backend.lib, backend.ctx
+        self.backend, self.lib = backend, backend.lib
         self.device = torch.device("cuda", backend.device)
         self._index = backend.device
         lib = self.lib
         self._norm, self._rope = lib.apx_add_rms_norm_quant_async, lib.apx_rope_kv4_append_async
         self._attn, self._sample = lib.apx_attn_kv4_async, lib.apx_sample_async
+
+    @property
+    def ctx(self):
+        """The backend's context; None once it is closed, which the entry points refuse."""
+        return self.backend.ctx
 
     def _stream(self, stream):
         return _raw_stream(self._index) if stream is None else stream
@@ -189,12 +194,13 @@ class StepOps:
 
     # -- refusals that the device finds -------------------------------------------------------
     def new_status(self):
-        """Status words with nothing refused."""
+        """Status words with nothing refused, written on the current stream."""
         return torch.full((2,), -1, dtype=_I64, device=self.device)
 
     @staticmethod
     def check_status(status):
-        """None, or (row, code) of the first refusal; waits for the work queued before."""
+        """None, or (row, code) of the first refusal; waits for the current stream, which is to have
+        waited for the calls' own where that is another."""
         word = int(status[0].item()) & ((1 << 64) - 1)
         return None if word == (1 << 64) - 1 else (word >> 24, word >> 16 & 0xFF)
 
@@ -214,7 +220,7 @@ class StepOps:
                   f"act: ({k}, {n}) on cuda:{dev} is wanted")
             codes, exps, descs = act.codes.data_ptr(), act.exps.data_ptr(), act.descs.data_ptr()
         try:
-            rc = self._norm(self.ctx, _NORM(
+            rc = self._norm(self.backend.ctx, _NORM(
                 x.data_ptr(), 0 if add is None else add.data_ptr(),
                 _vector(weight, n, _F32, "weight", dev),
                 0 if resid is None else resid.data_ptr(), 0 if y is None else y.data_ptr(),
@@ -267,7 +273,7 @@ class StepOps:
             q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         n_pos, n = table.shape[0], t * heads * dim
         try:
-            rc = self._rope(self.ctx, _ROPE(
+            rc = self._rope(self.backend.ctx, _ROPE(
                 q_ptr, k.data_ptr(), v.data_ptr(),
                 _vector(table, n_pos * rot_dim, _F32, "table", dev),
                 out_ptr, _vector(k_deq, n, torch.float16, "k_deq", dev),
@@ -291,7 +297,7 @@ class StepOps:
         if out is None:
             out = self._empty(shape, dtype, stream)
         try:
-            rc = self._attn(self.ctx, _ATTN(
+            rc = self._attn(self.backend.ctx, _ATTN(
                 q.data_ptr(), out.data_ptr(), _vector(status, 2, _I64, "status", dev),
                 _rows(q, shape, "q", dtype, dev), _rows(out, shape, "out", dtype, dev),
                 _TYPES.get(dtype, -1), heads, scale, window, sinks, 0), cache.ref, batch.ref,
@@ -310,7 +316,7 @@ class StepOps:
         rows, vocab = shape
         if token is None:
             token = self._empty(rows, _I32, stream)
-        rc = self._sample(self.ctx, _SAMPLE(
+        rc = self._sample(self.backend.ctx, _SAMPLE(
             logits.data_ptr(), _vector(u, rows, _F32, "u", dev),
             _vector(temperature, rows, _F32, "temperature", dev),
             _vector(top_p, rows, _F32, "top_p", dev), _vector(min_p, rows, _F32, "min_p", dev),

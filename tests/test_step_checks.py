@@ -42,7 +42,7 @@ def ops():
     class Backend:
         lib, ctx, device = _abi.load(build.build()), None, 1
 
-    ops = StepOps(Backend)
+    ops = StepOps(Backend())
     ops.reached = []
     for name in ("_norm", "_rope", "_attn", "_sample"):
         setattr(ops, name, lambda *a, name=name: ops.reached.append(name) or 0)
@@ -171,3 +171,26 @@ def test_numbers_that_no_field_holds(ops):
     for dim, tokens in ((2 ** 32 + 64, 16), (64, 2 ** 32 + 16), (64, -16)):
         with pytest.raises(ValueError):
             KV4Cache(pages, 2, dim, tokens)
+
+
+def test_calls_on_a_closed_backend():
+    """A backend that was closed has no context: the entry points get none, and refuse."""
+    class Backend:
+        lib, ctx, device = _abi.load(build.build()), 77, 1
+
+    ops = StepOps(Backend())
+    given = []
+    names = ("_norm", "_rope", "_attn", "_sample")
+    for name in names:
+        setattr(ops, name, lambda ctx, *a: given.append(ctx) or 0)
+    here = lambda name, shape, dtype=torch.float32: Fake(shape, dtype, 1)  # noqa: E731
+    for call in (norm, rope, attn, sample):
+        call(ops, here)
+    ops.backend.ctx = None  # as Backend.close leaves it
+    for call in (norm, rope, attn, sample):
+        call(ops, here)
+    assert given == [77] * 4 + [None] * 4 and ops.ctx is None
+    real = StepOps(ops.backend)
+    for call in (norm, rope, attn, sample):
+        with pytest.raises(ValueError):
+            call(real, here)
