@@ -223,3 +223,22 @@ def test_captured_behind_a_copy(ops, call):
         x.copy_(v)
         run()
         assert torch.equal(got[0], y) and torch.equal(got[1], token)
+
+
+def test_default_and_current_stream_by_handle(ops):
+    """The handles of the default stream (0) and of the current one serve as streams too."""
+    import torch
+
+    x = torch.randn(6, 500, device="cuda")
+    u = torch.rand(6, device="cuda")
+    want = ops.sample(x, u)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    assert torch.equal(ops.sample(x, u, stream=0), want)
+    assert torch.equal(ops.sample(x, u, stream=torch.cuda.current_stream().cuda_stream), want)
+    with torch.cuda.stream(side):
+        got = ops.sample(x, u, stream=side.cuda_stream)
+        act = ops.add_rms_norm_quant(x, None, 1e-6, stream=0)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    assert torch.equal(act.codes, ops.add_rms_norm_quant(x, None, 1e-6).codes)
